@@ -443,6 +443,120 @@ int sile_hip_flash_attn_fwd(sile_dtype dtype, int64_t batch, int64_t heads, int6
                             int64_t head_dim, const void *q, const void *k, const void *v,
                             void *o, float scale, int causal, sile_hip_stream stream);
 
+/* ---- a paged key-value cache, for programs that answer token by token -------
+ * No counterpart in the reference: its DSL cannot index a page table.  A cache
+ * is, all of it in the caller's device memory:
+ *   pages    K's and V's, each [num_pages][kv_heads][page_size][head_dim] with
+ *            page_stride >= kv_heads * page_size * head_dim elements from page
+ *            to page (so that K, V and several layers may share a record);
+ *            page_size a power of two up to 65536, pages 16-byte aligned
+ *   tables   int32 [n_rows][ld_table] page numbers, a row a sequence; token
+ *            j of row r lies in page tables[r][j / page_size], slot
+ *            j % page_size; a number outside [0, num_pages) names no page
+ *   lengths  int32 [n_rows] tokens of the rows
+ *   refs     int32 [num_pages] table entries that hold the page; <= 0: free
+ * Page numbers, lengths and positions are looked at on the device only: one
+ * outside its range names nothing, and nothing is read or written for it.
+ * All calls only enqueue, on the current device, and can be captured into a
+ * graph (they are plain kernel launches); the same workspace serves calls
+ * that run one after another, never two that may run side by side. */
+
+/* Stores n_tokens new tokens: K's rows k + t * ldk and V's v + t * ldv, each
+ * [kv_heads][head_dim] (so both may point into one fused projection), at position
+ * positions[t] of row rows[t] (rows NULL: row t).  dtype f16 or bf16; cache_type the
+ * same (head_dim a multiple of 8), or f8e4m3 (a multiple of 16): x / scale to nearest
+ * even, saturating at 448, NaN kept.  head_dim <= 256; k, v 16-byte aligned,
+ * ldk, ldv multiples of 8.  A token whose row, position or page does not exist is
+ * left out.  Two tokens of one position: each 16 bytes are one of theirs. */
+int sile_hip_kv_append(sile_dtype dtype, sile_dtype cache_type, int64_t n_tokens, int64_t kv_heads,
+                       int64_t head_dim, const void *k, int64_t ldk, const void *v, int64_t ldv,
+                       const int32_t *rows, const int32_t *positions, void *k_pages, void *v_pages,
+                       int64_t num_pages, int64_t page_size, int64_t page_stride,
+                       const int32_t *tables, int64_t n_rows, int64_t ld_table, float k_scale,
+                       float v_scale, sile_hip_stream stream);
+
+/* Copies page src[i] to page dst[i] for i < n in each of n_pools (at most 128)
+ * pools, given as a host array of device pointers: page_bytes bytes of every page,
+ * pages page_stride_bytes apart (both multiples of 16).  A pair with a page outside
+ * the pool, or with src = dst, is left out.  No page may be both a source and a
+ * destination, or a destination twice: what it then holds is unspecified. */
+int sile_hip_kv_copy_pages(void *const *pools, int64_t n_pools, int64_t page_bytes,
+                           int64_t page_stride_bytes, int64_t num_pages, int64_t n,
+                           const int32_t *src, const int32_t *dst, sile_hip_stream stream);
+
+/* Frees the rows with drop[r] != 0: each of their entries gives its page's count
+ * back and becomes -1, their length 0.  The other rows stay.  Old and new tables,
+ * lengths and counts are each the same array or separate ones. */
+int sile_hip_kv_free(int64_t n_rows, int64_t ld_table, const int32_t *drop,
+                     const int32_t *tables_in, int32_t *tables_out, const int32_t *lengths_in,
+                     int32_t *lengths_out, int64_t num_pages, const int32_t *refs_in,
+                     int32_t *refs_out, sile_hip_stream stream);
+
+/* Forks rows: row i < n_out of the new table and lengths is row src[i] of the old ones
+ * (n_in rows), empty where src[i] is outside [0, n_in).  The pages are shared, not copied:
+ * a page's count changes by how many rows took its row, less one, so a row that none
+ * took is freed and a row that two took is forked (beam search's reordering is one call).
+ * Old and new tables and lengths must not overlap; the counts may be one array. */
+int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_t *src,
+                     const int32_t *tables_in, int32_t *tables_out, const int32_t *lengths_in,
+                     int32_t *lengths_out, int64_t num_pages, const int32_t *refs_in,
+                     int32_t *refs_out, sile_hip_stream stream);
+
+/* Workspace bytes that sile_hip_kv_reserve and sile_hip_kv_compact need. */
+int sile_hip_kv_workspace(int64_t n_rows, int64_t num_pages, size_t *bytes);
+
+/* Makes the next need[r] tokens of each row writable (need <= 0: nothing to do):
+ * every entry that positions lengths[r] .. lengths[r] + need[r] - 1 fall into and that
+ * holds no page, or one whose count is not 1, gets a free page of its own, with
+ * count 1; the shared page it held loses one count, and where it has tokens of the row
+ * its contents are copied first (pools as for sile_hip_kv_copy_pages; n_pools = 0 copies
+ * nothing).  Free pages (count <= 0 before the call) are handed out lowest number
+ * first, to the rows in order.  granted[r] is 1, or 0 for a row that its table cannot
+ * hold and for the first row that the free pages do not cover and every later one that
+ * needs any: those stay as they are.  lengths stay.  Old and new tables and counts are
+ * each the same array or separate ones. */
+int sile_hip_kv_reserve(int64_t n_rows, int64_t ld_table, int64_t page_size,
+                        const int32_t *lengths, const int32_t *need, const int32_t *tables_in,
+                        int32_t *tables_out, int64_t num_pages, const int32_t *refs_in,
+                        int32_t *refs_out, int32_t *granted, void *const *pools, int64_t n_pools,
+                        int64_t page_bytes, int64_t page_stride_bytes, void *workspace,
+                        size_t workspace_bytes, sile_hip_stream stream);
+
+/* Closes the pool up: with u pages in use (count > 0), *used (device) becomes u and the
+ * pages in use numbered u or higher move, in order, into the free ones below, with
+ * their contents, counts and table entries; free pages' counts become 0.  Old and new
+ * tables and counts are each the same array or separate ones. */
+int sile_hip_kv_compact(int64_t n_rows, int64_t ld_table, const int32_t *tables_in,
+                        int32_t *tables_out, int64_t num_pages, const int32_t *refs_in,
+                        int32_t *refs_out, int32_t *used, void *const *pools, int64_t n_pools,
+                        int64_t page_bytes, int64_t page_stride_bytes, void *workspace,
+                        size_t workspace_bytes, sile_hip_stream stream);
+
+/* Workspace bytes that sile_hip_paged_attn_decode needs (for any lengths). */
+int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, size_t *bytes);
+
+/* Attention of one new token a row over the cache: with len = lengths[b],
+ *   o[b][h] = softmax_j(q[b][h] . k_j * scale) . v_j
+ * over the keys j < len of row b's pages, of key head h / (q_heads / kv_heads); with
+ * window > 0 only j >= len - window or j < sinks (the token is at position len - 1 and
+ * its own key is in the cache).  q[b], o[b] at q + b * ldq, o + b * ldo, [q_heads][head_dim],
+ * f16 or bf16, 16-byte aligned, ldq and ldo multiples of 8.  The cache as for
+ * sile_hip_kv_append; an f8e4m3 one holds k / k_scale and v / v_scale (1 otherwise).  A key whose page does not
+ * exist counts as unseen; a row without any seen key gives zeros; what lies in
+ * unseen slots never reaches a result, NaN and Inf included.  fp32 throughout
+ * but for the products' operands, where the probabilities are two 16-bit parts.
+ * A row's keys may be split over workgroups, by the lengths of all rows, so its
+ * rounding can depend on the batch; the same call gives the same bits. */
+int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t batch,
+                               int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void *q,
+                               int64_t ldq, const void *k_pages, const void *v_pages,
+                               int64_t num_pages, int64_t page_size, int64_t page_stride,
+                               const int32_t *tables, int64_t ld_table, const int32_t *lengths,
+                               void *o, int64_t ldo, float scale, float k_scale, float v_scale,
+                               int64_t window, int64_t sinks, void *workspace,
+                               size_t workspace_bytes, sile_hip_stream stream);
+
 /* ---- pattern router: Tile IR -> hand-written kernels ---------------------
  * Generalises the reference's canonical-matmul detector
  * (crates/sile-tile-ir/src/passes/lowering/canonical_matmul.rs:446-666) to

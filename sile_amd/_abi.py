@@ -154,6 +154,19 @@ SIGNATURES = {
     "sile_hip_attention_f32_kt": [_I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _F32,
                                   _F32, _P],
     "sile_hip_matvec_f32": [_I64, _I64, _I64, _P, _I64, _P, _F32, _P, _P],
+    "sile_hip_kv_append": [_I32, _I32, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64,
+                           _I64, _I64, _P, _I64, _I64, _F32, _F32, _P],
+    "sile_hip_kv_copy_pages": [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P],
+    "sile_hip_kv_free": [_I64, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P],
+    "sile_hip_kv_fork": [_I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _P],
+    "sile_hip_kv_workspace": [_I64, _I64, ctypes.POINTER(_SZ)],
+    "sile_hip_kv_reserve": [_I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64,
+                            _P, _SZ, _P],
+    "sile_hip_kv_compact": [_I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _P, _SZ, _P],
+    "sile_hip_paged_attn_workspace": [_I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)],
+    "sile_hip_paged_attn_decode": [_I32, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _I64,
+                                   _I64, _P, _I64, _P, _P, _I64, _F32, _F32, _F32, _I64, _I64, _P,
+                                   _SZ, _P],
     "sile_hip_tile_ir_route": [ctypes.c_char_p, _P, _I64, _I64, ctypes.POINTER(Route)],
     "sile_hip_tile_ir_launch": [ctypes.POINTER(Route), _P, _I64, _P, _I64, _I64, _P],
 }
@@ -497,6 +510,74 @@ def attention_f32_kt(n_q, n_k, head_dim, q, ldq, kt, ldkt, v, ldv, o, ldo, scale
 
 def matvec_f32(m, k, bk, x, ldx, y, out, seed=0.0, stream=None):
     call("sile_hip_matvec_f32", m, k, bk, x, ldx, y, seed, out, _sh(stream))
+
+
+# ---------------------------------------------------------------------------
+# paged key-value cache (asynchronous on the stream; pointers are device
+# addresses, but `pools` is a list of them)
+# ---------------------------------------------------------------------------
+
+def kv_append(dtype, cache_type, n_tokens, kv_heads, head_dim, k, ldk, v, ldv, rows, positions,
+              k_pages, v_pages, num_pages, page_size, page_stride, tables, n_rows, ld_table,
+              k_scale=1.0, v_scale=1.0, stream=None):
+    call("sile_hip_kv_append", dtype, cache_type, n_tokens, kv_heads, head_dim, k, ldk, v, ldv,
+         rows or None, positions, k_pages, v_pages, num_pages, page_size, page_stride, tables,
+         n_rows, ld_table, k_scale, v_scale, _sh(stream))
+
+
+def kv_copy_pages(pools, page_bytes, page_stride_bytes, num_pages, n, src, dst, stream=None):
+    call("sile_hip_kv_copy_pages", _ptr_array(pools), len(pools), page_bytes, page_stride_bytes,
+         num_pages, n, src, dst, _sh(stream))
+
+
+def kv_free(n_rows, ld_table, drop, tables_in, tables_out, lengths_in, lengths_out, num_pages,
+            refs_in, refs_out, stream=None):
+    call("sile_hip_kv_free", n_rows, ld_table, drop, tables_in, tables_out, lengths_in, lengths_out,
+         num_pages, refs_in, refs_out, _sh(stream))
+
+
+def kv_fork(n_in, n_out, ld_table, src, tables_in, tables_out, lengths_in, lengths_out, num_pages,
+            refs_in, refs_out, stream=None):
+    call("sile_hip_kv_fork", n_in, n_out, ld_table, src, tables_in, tables_out, lengths_in,
+         lengths_out, num_pages, refs_in, refs_out, _sh(stream))
+
+
+def kv_workspace(n_rows, num_pages) -> int:
+    """Workspace bytes of kv_reserve and kv_compact."""
+    n = _SZ(0)
+    call("sile_hip_kv_workspace", n_rows, num_pages, ctypes.byref(n))
+    return n.value
+
+
+def kv_reserve(n_rows, ld_table, page_size, lengths, need, tables_in, tables_out, num_pages, refs_in,
+               refs_out, granted, pools, page_bytes, page_stride_bytes, workspace, workspace_bytes,
+               stream=None):
+    call("sile_hip_kv_reserve", n_rows, ld_table, page_size, lengths, need, tables_in, tables_out,
+         num_pages, refs_in, refs_out, granted, _ptr_array(pools), len(pools), page_bytes,
+         page_stride_bytes, workspace, workspace_bytes, _sh(stream))
+
+
+def kv_compact(n_rows, ld_table, tables_in, tables_out, num_pages, refs_in, refs_out, used, pools,
+               page_bytes, page_stride_bytes, workspace, workspace_bytes, stream=None):
+    call("sile_hip_kv_compact", n_rows, ld_table, tables_in, tables_out, num_pages, refs_in,
+         refs_out, used, _ptr_array(pools), len(pools), page_bytes, page_stride_bytes, workspace,
+         workspace_bytes, _sh(stream))
+
+
+def paged_attn_workspace(batch, q_heads, kv_heads, head_dim) -> int:
+    """Workspace bytes of paged_attn_decode on the current device."""
+    n = _SZ(0)
+    call("sile_hip_paged_attn_workspace", batch, q_heads, kv_heads, head_dim, ctypes.byref(n))
+    return n.value
+
+
+def paged_attn_decode(dtype, cache_type, batch, q_heads, kv_heads, head_dim, q, ldq, k_pages,
+                      v_pages, num_pages, page_size, page_stride, tables, ld_table, lengths, o, ldo,
+                      scale, k_scale=1.0, v_scale=1.0, window=0, sinks=0, workspace=0,
+                      workspace_bytes=0, stream=None):
+    call("sile_hip_paged_attn_decode", dtype, cache_type, batch, q_heads, kv_heads, head_dim, q, ldq,
+         k_pages, v_pages, num_pages, page_size, page_stride, tables, ld_table, lengths, o, ldo,
+         scale, k_scale, v_scale, window, sinks, workspace or None, workspace_bytes, _sh(stream))
 
 
 def dtype_bytes(t: int) -> int:

@@ -1,0 +1,523 @@
+// Attention of one new token a row over a paged key-value cache.
+//
+//   o[b][h] = softmax_j(q[b][h] . k_j * scale) v_j over the keys j the token at
+//   position lengths[b] - 1 sees (all, or the last `window` and the first `sinks`)
+//
+// K and V pages are [kv_heads][page][d]; key j of row b lies in page
+// tables[b][j / page], slot j % page.
+//
+// What bounds it: every key and value is read once (HBM), against 4 g flop for
+// each of their element pairs, g query heads a key head.  So the matrix cores run far below
+// their rate whatever the tile, and the layout serves the loads:
+//
+//  * a wave takes 32 keys at a time and a tile of 16 query heads (the query
+//    heads that share a key head, padded), v_mfma_f32_16x16x32.  S^T = K . Q^T
+//    takes K straight from memory to registers: lane l supplies 8 consecutive
+//    dims of key l % 16, as the A operand asks.  Its accumulator holds 4 keys of
+//    ONE query head (l % 16), so max and sum are in-lane folds and two exchanges.
+//  * O^T = V^T . P^T needs 8 keys of one dim a lane: V goes through the wave's
+//    own LDS tile and is read with ds_read_b64_tr_b16.  No wave waits for
+//    another until the end of its keys.
+//  * P enters the product as two 16-bit parts, value and rest (16 bits of it in
+//    bf16, 22 in f16): the matrix cores have the room, and the result is then as exact
+//    as an fp32 P's.
+//  * while a tile is computed the next one's loads are in flight, and the page
+//    numbers of the one after.
+//
+// The tiles of all rows and key heads are one flat list, dealt in equal shares to
+// a fixed grid of workgroups (deal_chunk): a long row is spread over many
+// workgroups and a batch of mixed lengths has no straggler, with the lengths
+// known only on the device.  A workgroup whose share covers a row's key head
+// whole writes its output; the others leave (O, m, l) in fp32 in the workspace, at
+// most two a workgroup, and a second launch joins them.
+//
+// An 8-bit cache (e4m3) is widened in registers, exactly: K into the operand, V on
+// its way into LDS; the scales go into the score's and the output's factor.
+#include "common.h"
+#include "paged_plan.h"
+
+using namespace sile;
+
+typedef unsigned int u32x2v __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr float kLowest = -3.402823466e38f;
+// The probabilities of a row carry a factor 2^kLift, its maximum's being exactly
+// that: f16 has no exponent below 2^-24, and a long row has many keys far below
+// its maximum.  l and O carry it too, so it drops out of O / l.
+template <bool kBF16>
+constexpr float kLift = kBF16 ? 0.0f : 15.0f;
+
+struct PagedArgs {
+  const uint16_t* q;
+  const uint8_t* k;
+  const uint8_t* v;
+  uint16_t* o;
+  const int32_t* tables;
+  const int32_t* lengths;
+  int32_t* plan;        // workspace: tiles of the rows before each row, then the total and the chunk
+  float* part_ml;       // workspace: [slots][rows][2]
+  float* part_o;        // workspace: [slots][rows][d]
+  int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
+  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, grid;
+  float scale_log2, v_scale;
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+template <bool kBF16>
+SILE_DEV f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (kBF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <bool kBF16>
+SILE_DEV uint32_t pack2(float lo, float hi) {
+  return kBF16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
+}
+
+// what is left of lo and hi beside their 16-bit values in `pk`, packed alike
+template <bool kBF16>
+SILE_DEV uint32_t rest2(float lo, float hi, uint32_t pk) {
+  if constexpr (kBF16) {
+    return pack2<kBF16>(lo - bits_f32(pk << 16), hi - bits_f32(pk & 0xffff0000u));
+  } else {
+    const f16x2 h = __builtin_bit_cast(f16x2, pk);
+    return pack2<kBF16>(lo - (float)h[0], hi - (float)h[1]);
+  }
+}
+
+// two e4m3 codes of `w` (bytes 0, 1 or 2, 3) as two 16-bit values, exactly
+template <bool kBF16, bool kHigh>
+SILE_DEV uint32_t widen2(uint32_t w) {
+  if constexpr (kBF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHigh));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHigh));
+}
+template <bool kBF16>
+SILE_DEV u32x4 widen8(uint32_t a, uint32_t b) {
+  return u32x4{widen2<kBF16, false>(a), widen2<kBF16, true>(a), widen2<kBF16, false>(b),
+               widen2<kBF16, true>(b)};
+}
+
+// max of v over lanes l, l ^ 16, l ^ 32, l ^ 48
+SILE_DEV float quad_max(float v) {
+  v = __builtin_fmaxf(v, swizzle_xor16(v));
+  float lo, hi;
+  half_swap(v, lo, hi);
+  return __builtin_fmaxf(lo, hi);
+}
+SILE_DEV float quad_sum(float v) { return pair32_sum(v + swizzle_xor16(v)); }
+
+template <int kDp, int kQT>
+struct Shape {
+  static constexpr int kRow = 2 * kDp;                        // bytes of a V row in LDS
+  static constexpr int kPitch = kDp + 4;                      // floats of an O row in LDS
+  static constexpr int kTileB = kTileKeys * kRow;
+  static constexpr int kMergeB = 16 * kPitch * 4;
+  static constexpr int kWaveB = kTileB > kMergeB ? kTileB : kMergeB;
+};
+
+// The row that holds flat tile x0: the tiles of the rows before row b number
+// before(b), H times each (H key heads' worth).  Every thread adds up a run of
+// rows, a scan over the 256 threads follows.  Workgroup 0 keeps the sums for the
+// join.
+struct DealLds {
+  int32_t wave_sum[4];
+  int32_t row, before;
+};
+
+template <bool kBF16, bool kFp8, int kDp, bool kExact, int kQT>
+__device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, float* ml,
+                                           DealLds* deal) {
+  using Sh = Shape<kDp, kQT>;
+  constexpr int kKK = kDp / 32;                      // d-steps of S^T
+  constexpr int kDT = kDp / 16;                      // 16-dim tiles of O^T
+  constexpr int kEs = kFp8 ? 1 : 2;                  // bytes of a cache element
+  constexpr int kCh = kDp * kEs / 16;                // 16-byte chunks of a cache row
+  constexpr int kKL = kFp8 ? kKK / 2 : kKK;          // K loads of a lane for 16 keys
+  constexpr int kVL = kTileKeys * kCh / 64;          // V loads of a lane
+  constexpr int kVRows = 64 / kCh;                   // V rows one load instruction covers
+  static_assert(kCh <= 64 && kKK % 2 == 0, "row width");
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, l16 = lane & 15;
+  const int heads = a.kv_heads * a.head_groups;      // units of a row
+  const int d = kExact ? kDp : a.d;
+  const int chunks = d * kEs / 16;
+
+  // ---- deal ----
+  const int per = (a.batch + 255) / 256;
+  int32_t mine = 0;
+  for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r)
+    mine += key_span(a.lengths[r], a.capacity, a.window, a.sinks).tiles;
+  int32_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int32_t up = __shfl_up(incl, off);
+    if (lane >= off) incl += up;
+  }
+  if (lane == 63) deal->wave_sum[wave] = incl;
+  __syncthreads();
+  int32_t before = incl - mine, rows_total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) before += deal->wave_sum[w];
+    rows_total += deal->wave_sum[w];
+  }
+  const int32_t total = rows_total * heads;
+  const int32_t chunk = deal_chunk(total, a.grid);
+  int32_t x = blockIdx.x * (int64_t)chunk < total ? blockIdx.x * chunk : total;
+  const int32_t x1 = total - x < chunk ? total : x + chunk;
+  if (blockIdx.x == 0 || x < x1) {
+    int32_t at = before;
+    for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r) {
+      const int32_t t = key_span(a.lengths[r], a.capacity, a.window, a.sinks).tiles;
+      if (blockIdx.x == 0) a.plan[r] = at;
+      if (x < x1 && x / heads >= at && x / heads < at + t) {
+        deal->row = r;
+        deal->before = at;
+      }
+      at += t;
+    }
+    if (blockIdx.x == 0 && tid == 0) a.plan[a.batch] = chunk;
+  }
+  if (x >= x1) return;
+  __syncthreads();
+  int row = __builtin_amdgcn_readfirstlane(deal->row);
+  int32_t base = __builtin_amdgcn_readfirstlane(deal->before) * heads;
+  uint8_t* const vt = smem + wave * Sh::kWaveB;
+
+  while (x < x1) {
+    const KeySpan span = key_span(a.lengths[row], a.capacity, a.window, a.sinks);
+    if (span.tiles == 0 || x >= base + span.tiles * heads) {   // on to the next row
+      base += span.tiles * heads;
+      ++row;
+      continue;
+    }
+    const int unit = (x - base) / span.tiles;
+    const int t0 = x - base - unit * span.tiles;
+    const int t1 = min(span.tiles, t0 + (x1 - x));
+    x += t1 - t0;
+    const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
+    const int rows = min(16 * kQT, a.group - hg * 16 * kQT);   // query heads of this unit
+    const int head0 = kvh * a.group + hg * 16 * kQT;
+    const int32_t* table = a.tables + (int64_t)row * a.ld_table;
+
+    // ---- Q^T fragments: query head l16 of tile qt, zeros past the heads and dims ----
+    u32x4 qf[kQT][kKK];
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+      const bool in = qt * 16 + l16 < rows;
+      const uint16_t* qr = a.q + (int64_t)row * a.ldq + (int64_t)(head0 + (in ? qt * 16 + l16 : 0)) * d;
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk) {
+        const int dim = kFp8 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+        u32x4 w = {0u, 0u, 0u, 0u};
+        if (in && (kExact || dim < d)) w = *reinterpret_cast<const u32x4*>(qr + dim);
+        qf[qt][kk] = w;
+      }
+    }
+    f32x4 oacc[kQT][kDT];
+    float m_run[kQT], l_run[kQT];
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+      m_run[qt] = -__builtin_inff();
+      l_run[qt] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) oacc[qt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // ---- loads ----
+    // table entry of key (lane & 31) of tile t (any entry of the row's past its
+    // keys); read a round ahead and looked at by load_tile alone, which then does
+    // not wait for it
+    auto page_of = [&](int t) {
+      const int key = span_key(span, min(t, t1 - 1)) + (lane & 31);
+      return table[min(key, span.len - 1) >> a.page_shift];
+    };
+    u32x4 kr[2][kKL], vr[kVL];
+    const int64_t head_off = (int64_t)kvh * d << a.page_shift;
+    // issues tile t's loads; returns the mask of its keys that are read
+    auto load_tile = [&](int t, int32_t id) -> uint32_t {
+      const int key0 = span_key(span, min(t, t1 - 1)) + (lane & 31);
+      const bool ok = t < t1 && span_sees(span, key0) && (uint32_t)id < (uint32_t)a.num_pages;
+      const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+      if (seen == 0) return 0;
+      const int slot = key0 & ((1 << a.page_shift) - 1);
+      // keys that are not read take page 0's row of the same slot, which is there
+      const int64_t off = ((int64_t)(ok ? id : 0) * a.page_stride + head_off + (int64_t)slot * d) * kEs;
+      const int off_lo = (int)(uint32_t)off, off_hi = (int)(off >> 32);
+      auto row_off = [&](int key) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * key, off_lo);
+        const int32_t hi = __builtin_amdgcn_ds_bpermute(4 * key, off_hi);
+        return (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo);
+      };
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint8_t* p = a.k + row_off(16 * s + l16);
+#pragma unroll
+        for (int i = 0; i < kKL; ++i) {
+          const int c = 4 * i + g;
+          u32x4 w = {0u, 0u, 0u, 0u};
+          if (kExact || c < chunks) w = *reinterpret_cast<const u32x4*>(p + 16 * c);
+          kr[s][i] = w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kVL; ++i) {
+        const int c = lane % kCh;   // a chunk past the dims reads chunk 0 (its O^T rows are not kept)
+        const uint8_t* p = a.v + row_off(kVRows * i + lane / kCh);
+        vr[i] = *reinterpret_cast<const u32x4*>(p + 16 * (kExact || c < chunks ? c : 0));
+      }
+      return seen;
+    };
+    auto vswz = [](int r) { return (kDp == 64 ? 2 : 4) * (r & 3); };
+
+    // one round of a wave: S and V of the tile that has arrived, the next tile's
+    // loads into the registers they leave, softmax and P V beside those.  A tile
+    // without any key (the round before the first; holes) is passed over.
+    int t = t0 + wave - kTileWaves;
+    int32_t id = page_of(t0 + wave);
+    uint32_t seen = 0;
+    while (true) {
+      const uint32_t now = seen;
+      f32x4 sacc[kQT][2];
+      if (now != 0) {
+      // S^T: keys 16 s + 4 g + i of query head l16
+#pragma unroll
+      for (int qt = 0; qt < kQT; ++qt)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) sacc[qt][s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kk = 0; kk < kKK; ++kk)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u32x4 kf;
+          if constexpr (kFp8)
+            kf = widen8<kBF16>(kr[s][kk / 2][2 * (kk & 1)], kr[s][kk / 2][2 * (kk & 1) + 1]);
+          else
+            kf = kr[s][kk];
+#pragma unroll
+          for (int qt = 0; qt < kQT; ++qt) sacc[qt][s] = mma16<kBF16>(kf, qf[qt][kk], sacc[qt][s]);
+        }
+      // V into the wave's LDS tile; a key that is not seen as zeros (0 times what
+      // lies there could be NaN)
+#pragma unroll
+      for (int i = 0; i < kVL; ++i) {
+        const int r = kVRows * i + lane / kCh, c = lane % kCh;
+        u32x4 w = vr[i];
+        if (now != 0xffffffffu && !((now >> r) & 1)) w = u32x4{0u, 0u, 0u, 0u};
+        if constexpr (kFp8) {
+          *reinterpret_cast<u32x4*>(vt + r * Sh::kRow + (((2 * c) ^ vswz(r)) << 4)) =
+              widen8<kBF16>(w[0], w[1]);
+          *reinterpret_cast<u32x4*>(vt + r * Sh::kRow + (((2 * c + 1) ^ vswz(r)) << 4)) =
+              widen8<kBF16>(w[2], w[3]);
+        } else {
+          *reinterpret_cast<u32x4*>(vt + r * Sh::kRow + ((c ^ vswz(r)) << 4)) = w;
+        }
+      }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      t += kTileWaves;
+      seen = load_tile(t, id);
+      id = page_of(t + kTileWaves);
+      __builtin_amdgcn_sched_barrier(0);
+
+      if (now != 0) {
+      // online softmax in units of log2 e; a seen key's score counts as at least
+      // the lowest float in the max, so that a row of -inf scores is told from an
+      // empty one (0 / 0 against zeros)
+      u32x4 pf[kQT], pr[kQT];
+      const uint32_t bits = ((now >> (4 * g)) & 0xfu) | (((now >> (16 + 4 * g)) & 0xfu) << 4);
+#pragma unroll
+      for (int qt = 0; qt < kQT; ++qt) {
+        float sc[8];
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v = sacc[qt][i >> 2][i & 3] * a.scale_log2;
+          const bool in = (bits >> i) & 1;
+          sc[i] = in ? v : -__builtin_inff();
+          mx = __builtin_fmaxf(mx, in ? __builtin_fmaxf(v, kLowest) : -__builtin_inff());
+        }
+        const float m_new = __builtin_fmaxf(m_run[qt], quad_max(mx));
+        const float alpha = exp2_fast(m_run[qt] - m_new);   // (m_new > -inf: a key is seen)
+        m_run[qt] = m_new;
+        float rs = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float p0 = exp2_fast(sc[i] - m_new + kLift<kBF16>);
+          const float p1 = exp2_fast(sc[i + 1] - m_new + kLift<kBF16>);
+          rs += p0 + p1;
+          const uint32_t pk = pack2<kBF16>(p0, p1);
+          pf[qt][i >> 1] = pk;
+          pr[qt][i >> 1] = rest2<kBF16>(p0, p1, pk);
+        }
+        l_run[qt] = l_run[qt] * alpha + rs;
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+          for (int dt = 0; dt < kDT; ++dt) oacc[qt][dt] *= alpha;
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+      // O^T += V^T . P^T: slots 0-3 keys 4 g + j, slots 4-7 keys 16 + 4 g + j
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) {
+        u32x4 vf;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = 16 * h + 4 * g + (l16 >> 2);
+          const int c = 2 * dt + ((l16 & 3) >> 1);
+          const s16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (lds_s16x4_ptr)(vt + key * Sh::kRow + ((c ^ vswz(key)) << 4) + 8 * (l16 & 1)));
+          const u32x2 w2 = __builtin_bit_cast(u32x2, w);
+          vf[2 * h] = w2[0];
+          vf[2 * h + 1] = w2[1];
+        }
+#pragma unroll
+        for (int qt = 0; qt < kQT; ++qt) {
+          oacc[qt][dt] = mma16<kBF16>(vf, pf[qt], oacc[qt][dt]);
+          oacc[qt][dt] = mma16<kBF16>(vf, pr[qt], oacc[qt][dt]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+      }
+      if (t >= t1) break;
+    }
+
+    // ---- the four waves' (m, l, O) added up ----
+    const bool whole = t0 == 0 && t1 == span.tiles;
+    const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int qt = 0; qt < kQT; ++qt) {
+      const float l = quad_sum(l_run[qt]);
+      if (g == 0) {
+        ml[(wave * 16 + l16) * 2] = m_run[qt];
+        ml[(wave * 16 + l16) * 2 + 1] = l;
+      }
+      float* ot = reinterpret_cast<float*>(vt) + l16 * Sh::kPitch + 4 * g;
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<f32x4*>(ot + 16 * dt) = oacc[qt][dt];
+      __syncthreads();
+      const int r = tid >> 4, head = qt * 16 + r;
+      float w[4], m = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, ml[(i * 16 + r) * 2]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float mi = ml[(i * 16 + r) * 2];
+        w[i] = mi == -__builtin_inff() ? 0.0f : exp2_fast(mi - m);
+        sum += w[i] * ml[(i * 16 + r) * 2 + 1];
+      }
+      if (head < rows) {
+        // a row without keys gives zeros; scores that are all -inf give 0 / 0
+        const float f = whole ? (m == -__builtin_inff() ? 0.0f : a.v_scale / sum) : 1.0f;
+        const int64_t at = (int64_t)slot * 16 * kQT + head;
+        for (int c = 4 * (tid & 15); c < d; c += 64) {
+          f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(
+                reinterpret_cast<const float*>(smem + i * Sh::kWaveB) + r * Sh::kPitch + c);
+            acc += v * w[i];
+          }
+          acc *= f;
+          if (whole) {
+            const u32x2 out = {pack2<kBF16>(acc[0], acc[1]), pack2<kBF16>(acc[2], acc[3])};
+            *reinterpret_cast<u32x2*>(a.o + (int64_t)row * a.ldo + (int64_t)(head0 + head) * d + c) = out;
+          } else {
+            *reinterpret_cast<f32x4*>(a.part_o + at * d + c) = acc;
+          }
+        }
+        if (!whole && (tid & 15) == 0) {
+          a.part_ml[at * 2] = m;
+          a.part_ml[at * 2 + 1] = sum;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Joins a unit's parts (row, key head, head group: blockIdx.x; four query heads a
+// workgroup, a wave each: blockIdx.y), or writes the zeros of a row without keys.
+template <bool kBF16, int kQT>
+__device__ __forceinline__ void paged_join(const PagedArgs& a) {
+  const int heads = a.kv_heads * a.head_groups;
+  const int row = blockIdx.x / heads, unit = blockIdx.x - row * heads;
+  const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
+  const int rows = min(16 * kQT, a.group - hg * 16 * kQT);
+  const int lane = threadIdx.x & 63;
+  const int r = 4 * blockIdx.y + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const KeySpan span = key_span(a.lengths[row], a.capacity, a.window, a.sinks);
+  uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)(kvh * a.group + hg * 16 * kQT + r) * a.d;
+  if (span.tiles == 0) {
+    for (int c = lane; c < a.d; c += 64) o[c] = 0;
+    return;
+  }
+  const int32_t chunk = a.plan[a.batch];
+  const int32_t x0 = a.plan[row] * heads + unit * span.tiles;
+  const int32_t g0 = x0 / chunk, g1 = (x0 + span.tiles - 1) / chunk;
+  if (g0 == g1) return;   // one workgroup had it whole
+  auto at = [&](int32_t w) { return ((int64_t)(2 * w + (w == g0 ? 1 : 0)) * 16 * kQT + r); };
+  float m = -__builtin_inff();
+  for (int32_t w = g0 + lane; w <= g1; w += 64) m = __builtin_fmaxf(m, a.part_ml[at(w) * 2]);
+  m = wave_max(m);
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+#pragma unroll 4
+  for (int32_t w = g0; w <= g1; ++w) {
+    const float mi = a.part_ml[at(w) * 2];
+    const float f = mi == -__builtin_inff() ? 0.0f : exp2_fast(mi - m);
+    sum += f * a.part_ml[at(w) * 2 + 1];
+    const float* p = a.part_o + at(w) * a.d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 64 * i < a.d) acc[i] += f * p[lane + 64 * i];
+  }
+  const float f = m == -__builtin_inff() ? 0.0f : a.v_scale / sum;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (lane + 64 * i < a.d)
+      o[lane + 64 * i] = kBF16 ? bf16_rne(acc[i] * f) : f16_rne(acc[i] * f);
+}
+
+}  // namespace
+
+#define SILE_PAGED_KERNEL(NAME, BF, F8, DP, EX, QT, EU)                                   \
+  extern "C" __global__ __launch_bounds__(256, EU) void NAME(PagedArgs a) {               \
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * Shape<DP, QT>::kWaveB];    \
+    __shared__ float ml[4 * 16 * 2];                                                      \
+    __shared__ DealLds deal;                                                              \
+    paged_attn<BF, F8, DP, EX, QT>(a, smem, ml, &deal);                                   \
+  }
+// d<D>: that head dimension; p<D>: any smaller one.  q<N>: N tiles of 16 query heads.
+#define SILE_PAGED_TYPES(SUFFIX, DP, EX, QT, EU)                                  \
+  SILE_PAGED_KERNEL(sile_paged_attn_f16_##SUFFIX, false, false, DP, EX, QT, EU)   \
+  SILE_PAGED_KERNEL(sile_paged_attn_bf16_##SUFFIX, true, false, DP, EX, QT, EU)   \
+  SILE_PAGED_KERNEL(sile_paged_attn_f16_fp8_##SUFFIX, false, true, DP, EX, QT, EU) \
+  SILE_PAGED_KERNEL(sile_paged_attn_bf16_fp8_##SUFFIX, true, true, DP, EX, QT, EU)
+#define SILE_PAGED_DIM(DP, QT, EU)                \
+  SILE_PAGED_TYPES(d##DP##_q##QT, DP, true, QT, EU)  \
+  SILE_PAGED_TYPES(p##DP##_q##QT, DP, false, QT, EU)
+SILE_PAGED_DIM(64, 1, 2)
+SILE_PAGED_DIM(64, 2, 2)
+SILE_PAGED_DIM(128, 1, 2)
+SILE_PAGED_DIM(128, 2, 1)
+SILE_PAGED_DIM(256, 1, 1)
+
+#define SILE_PAGED_JOIN(NAME, BF, QT) \
+  extern "C" __global__ __launch_bounds__(256) void NAME(PagedArgs a) { paged_join<BF, QT>(a); }
+SILE_PAGED_JOIN(sile_paged_attn_join_f16_q1, false, 1)
+SILE_PAGED_JOIN(sile_paged_attn_join_bf16_q1, true, 1)
+SILE_PAGED_JOIN(sile_paged_attn_join_f16_q2, false, 2)
+SILE_PAGED_JOIN(sile_paged_attn_join_bf16_q2, true, 2)

@@ -73,18 +73,6 @@ struct GemmPlan {
   double seconds;  // modelled time
 };
 
-// compute units of the current device (asked of the runtime once a device)
-int device_cus(int* cus) {
-  static std::atomic<int> known[64];
-  int dev = 0;
-  SILE_HIP_CHECK(hipGetDevice(&dev));
-  if (dev >= 0 && dev < 64 && (*cus = known[dev].load(std::memory_order_relaxed)) > 0) return SILE_OK;
-  SILE_HIP_CHECK(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev));
-  if (*cus <= 0) return fail(SILE_ERR_RUNTIME, "device %d reports no compute units", dev);
-  if (dev >= 0 && dev < 64) known[dev].store(*cus, std::memory_order_relaxed);
-  return SILE_OK;
-}
-
 // seconds per element of K' for one tile, with w workgroups of that size
 // running at once on `cus` CUs (fitted: 256 x 256 16 ns up to cus / 2
 // workgroups, 21.8 ns at cus; 128 x 128 7.2 ns up to cus / 2, 7.8 ns at cus,
@@ -295,28 +283,6 @@ uint32_t f16_bits_rne(float f) {
   if (rem > 0x1000u || (rem == 0x1000u && (h & 1u))) ++h;
   return sign | h;
 }
-
-const char* dtype_name(int t) {
-  switch (t) {
-    case SILE_F32: return "f32";
-    case SILE_F16: return "f16";
-    case SILE_BF16: return "bf16";
-    case SILE_F8E4M3: return "f8e4m3";
-    default: return "?";
-  }
-}
-
-size_t dtype_bytes(int t) {
-  switch (t) {
-    case SILE_F32: return 4;
-    case SILE_F16:
-    case SILE_BF16: return 2;
-    case SILE_F8E4M3: return 1;
-    default: return 0;
-  }
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Programs that execute a body: min(num_threadgroups * threads_per_group, total),
 // since programs with pid >= total_tiles are skipped by the wrapper guard

@@ -9,6 +9,7 @@
 // once, at library build time.
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -40,6 +41,8 @@ SILE_EMBED(sile_co_softmax, "softmax.hsaco")
 SILE_EMBED(sile_co_gemm, "gemm.hsaco")
 SILE_EMBED(sile_co_attention, "attention.hsaco")
 SILE_EMBED(sile_co_flash_attn, "flash_attn.hsaco")
+SILE_EMBED(sile_co_paged_attn, "paged_attn.hsaco")
+SILE_EMBED(sile_co_kv_cache, "kv_cache.hsaco")
 
 namespace sile_rt {
 namespace {
@@ -56,6 +59,8 @@ const Image kImages[static_cast<int>(Module::kCount)] = {
     {sile_co_gemm_begin, sile_co_gemm_end, "gemm"},
     {sile_co_attention_begin, sile_co_attention_end, "attention"},
     {sile_co_flash_attn_begin, sile_co_flash_attn_end, "flash_attn"},
+    {sile_co_paged_attn_begin, sile_co_paged_attn_end, "paged_attn"},
+    {sile_co_kv_cache_begin, sile_co_kv_cache_end, "kv_cache"},
 };
 
 struct DeviceState {
@@ -118,6 +123,17 @@ int ensure_device() {
   std::lock_guard<std::mutex> lk(g_mu);
   DeviceState* st = nullptr;
   return load_device_locked(dev, &st);
+}
+
+int device_cus(int* cus) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  SILE_HIP_CHECK(hipGetDevice(&dev));
+  if (dev >= 0 && dev < 64 && (*cus = known[dev].load(std::memory_order_relaxed)) > 0) return SILE_OK;
+  SILE_HIP_CHECK(hipDeviceGetAttribute(cus, hipDeviceAttributeMultiprocessorCount, dev));
+  if (*cus <= 0) return fail(SILE_ERR_RUNTIME, "device %d reports no compute units", dev);
+  if (dev >= 0 && dev < 64) known[dev].store(*cus, std::memory_order_relaxed);
+  return SILE_OK;
 }
 
 int get_function(Module m, const char* name, hipFunction_t* out) {

@@ -33,12 +33,38 @@ enum class Module : int {
   kGemm = 2,
   kAttention = 3,
   kFlashAttn = 4,
-  kCount = 5
+  kPagedAttn = 5,
+  kKvCache = 6,
+  kCount = 7
 };
+
+inline const char* dtype_name(int t) {
+  switch (t) {
+    case SILE_F32: return "f32";
+    case SILE_F16: return "f16";
+    case SILE_BF16: return "bf16";
+    case SILE_F8E4M3: return "f8e4m3";
+    default: return "?";
+  }
+}
+
+inline size_t dtype_bytes(int t) {
+  switch (t) {
+    case SILE_F32: return 4;
+    case SILE_F16:
+    case SILE_BF16: return 2;
+    case SILE_F8E4M3: return 1;
+    default: return 0;
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Makes sure the current device is initialised and its code objects are
 // loaded; returns a status.
 int ensure_device();
+// Compute units of the current device (asked of the runtime once a device).
+int device_cus(int* cus);
 // Looks up `name` in the given embedded module on the current device.
 int get_function(Module m, const char* name, hipFunction_t* out);
 // Number of workgroups of `block_threads` threads of kernel `name` that fit on

@@ -1,0 +1,168 @@
+"""The paged cache's host side without a GPU: refusals come before any device work, and
+the arithmetic that host and kernels share (tiles of a row, shares of the workgroups) is
+compiled for the CPU and held against counting."""
+import ctypes
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from sile_amd import _abi
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCE = r"""
+#include "%s"
+extern "C" {
+void span(int32_t len, int64_t cap, int64_t window, int64_t sinks, int32_t* out) {
+  const sile::KeySpan s = sile::key_span(len, cap, window, sinks);
+  out[0] = s.len; out[1] = s.tiles; out[2] = s.sink_tiles; out[3] = s.first_tile;
+}
+// how often each key 0 .. n - 1 is covered by a tile and seen
+void cover(int32_t len, int64_t cap, int64_t window, int64_t sinks, int32_t n, int32_t* out) {
+  const sile::KeySpan s = sile::key_span(len, cap, window, sinks);
+  for (int32_t t = 0; t < s.tiles; ++t)
+    for (int32_t i = 0; i < sile::kTileKeys; ++i) {
+      const int32_t key = sile::span_key(s, t) + i;
+      if (sile::span_sees(s, key) && key < n) ++out[key];
+    }
+}
+int32_t chunk(int32_t total, int32_t groups) { return sile::deal_chunk(total, groups); }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    d = tmp_path_factory.mktemp("plan")
+    src = d / "plan.cpp"
+    src.write_text(SOURCE % os.path.join(ROOT, "sile_amd", "csrc", "kernels", "paged_plan.h"))
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-shared", "-fPIC",
+                    "-o", str(d / "plan.so"), str(src)], check=True)
+    lib = ctypes.CDLL(str(d / "plan.so"))
+    i32, i64 = ctypes.c_int32, ctypes.c_int64
+    lib.span.argtypes = [i32, i64, i64, i64, ctypes.c_void_p]
+    lib.cover.argtypes = [i32, i64, i64, i64, i32, ctypes.c_void_p]
+    lib.chunk.argtypes, lib.chunk.restype = [i32, i32], i32
+    return lib
+
+
+def test_tiles_cover_the_seen_keys_once(plan):
+    r = np.random.default_rng(0)
+    cases = [(n, w, s) for n in (0, 1, 31, 32, 33, 64, 100, 257) for w in (0, 1, 5, 32, 33, 100, 400)
+             for s in (0, 1, 31, 32, 40, 300)]
+    cases += [tuple(int(x) for x in r.integers(0, 700, 3)) for _ in range(300)]
+    for n, w, s in cases:
+        got = np.zeros(800, np.int32)
+        plan.cover(n, 10 ** 9, w, s, 800, got.ctypes.data)
+        want = np.zeros(800, np.int32)
+        j = np.arange(n)
+        want[j[(w <= 0) | (j >= n - w) | (j < s)]] = 1
+        assert (got == want).all(), (n, w, s)
+
+
+def test_lengths_are_held_to_the_table(plan):
+    out = np.zeros(4, np.int32)
+    for length, cap, want in ((-1, 64, 0), (-2 ** 31, 64, 0), (65, 64, 64), (2 ** 31 - 1, 48, 48), (5, 0, 0),
+                              (2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1)):
+        for w, s in ((0, 0), (7, 3), (2 ** 62, 2 ** 62), (1, 2 ** 62)):
+            plan.span(length, cap, w, s, out.ctypes.data)
+            assert out[0] == want and 0 <= out[1] <= want // 32 + 1
+
+
+def test_shares_cover_the_tiles(plan):
+    for groups in (1, 256, 512):
+        for total in (0, 1, 3, 4, 5, 511, 512, 513, 2048, 2049, 99999, 2 ** 30):
+            c = plan.chunk(total, groups)
+            assert c % 4 == 0 and c >= 4 and c * groups >= total
+
+
+P = 4096   # an aligned address that nothing reads
+F16, BF16, F8, F32 = _abi.F16, _abi.BF16, _abi.F8E4M3, _abi.F32
+
+
+def refused(name, args, code, needle):
+    assert _abi.status(name, *args) == code, (_abi.last_error(), args)
+    assert needle in _abi.last_error(), _abi.last_error()
+
+
+APPEND = [F16, F16, 3, 2, 64, P, 128, P, 128, None, P, P, P, 10, 16, 2048, P, 4, 8, 1.0, 1.0, None]
+
+
+@pytest.mark.parametrize("at,value,code,needle", [
+    (0, F32, 2, "tokens of f32"), (1, BF16, 2, "under f16"), (1, F32, 2, "under f16"), (2, -1, 5, "negative"),
+    (3, 0, 5, "cache shape"), (4, 0, 5, "cache shape"), (4, 264, 2, "head_dim > 256"), (4, 60, 2, "no multiple"),
+    (5, None, 5, "NULL"), (5, P + 8, 5, "aligned"), (6, 120, 5, "leading dimension"), (6, 132, 5, "aligned"),
+    (8, 127, 5, "leading dimension"), (10, None, 5, "NULL"), (11, P + 4, 5, "aligned"), (13, -1, 5, "cache shape"),
+    (14, 24, 5, "power of two"), (14, 0, 5, "power of two"), (14, 131072, 5, "power of two"), (15, 2047, 5, "page_stride"),
+    (15, 2052, 5, "page_stride"), (17, -1, 5, "negative"), (18, -1, 5, "negative"), (17, 2 ** 31, 5, "too large"),
+    (18, 2 ** 30, 5, "too large")])
+def test_append_refusals(at, value, code, needle):
+    args = list(APPEND)
+    args[at] = value
+    refused("sile_hip_kv_append", args, code, needle)
+
+
+def test_append_e4m3_needs_whole_chunks():
+    args = list(APPEND)
+    args[1], args[4] = F8, 72
+    refused("sile_hip_kv_append", args, 2, "no multiple of 16")
+
+
+def test_nothing_to_do_is_fine():
+    """(no GPU is asked for)"""
+    args = list(APPEND)
+    args[2] = 0
+    assert _abi.status("sile_hip_kv_append", *args) == 0
+    assert _abi.status("sile_hip_kv_copy_pages", None, 0, 0, 0, 5, 3, P, P, None) == 0
+    assert _abi.status("sile_hip_kv_free", 0, 4, None, None, None, None, None, 0, None, None, None) == 0
+    assert _abi.status("sile_hip_kv_fork", 0, 0, 4, None, None, None, None, None, 0, None, None, None) == 0
+
+
+DECODE = [F16, F16, 2, 4, 2, 64, P, 256, P, P, 10, 16, 2048, P, 8, P, P, 256, 0.1, 1.0, 1.0, 0, 0, P, 1 << 30, None]
+
+
+@pytest.mark.parametrize("at,value,code,needle", [
+    (0, F32, 2, "tokens of f32"), (1, BF16, 2, "under f16"), (2, -1, 5, "batch"), (3, 5, 5, "query heads"),
+    (3, 0, 5, "query heads"), (5, 257, 2, "head_dim"), (6, None, 5, "NULL"), (6, P + 2, 5, "aligned"),
+    (7, 255, 5, "leading dimension"), (7, 260, 5, "aligned"), (8, None, 5, "NULL"), (9, P + 8, 5, "aligned"),
+    (11, 48, 5, "power of two"), (12, 8, 5, "page_stride"), (13, None, 5, "NULL"), (14, 2 ** 31, 5, "too large"),
+    (15, None, 5, "NULL"), (16, P + 8, 5, "aligned"), (17, 100, 5, "leading dimension"), (21, -1, 5, "negative"),
+    (22, -1, 5, "negative")])
+def test_decode_refusals(at, value, code, needle):
+    args = list(DECODE)
+    args[at] = value
+    refused("sile_hip_paged_attn_decode", args, code, needle)
+
+
+TABLES = 1 << 20
+
+
+@pytest.mark.parametrize("name,args,code,needle", [
+    ("sile_hip_kv_copy_pages", [None, 1, 16, 16, 4, 1, P, P, None], 5, "NULL"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 129, 16, 16, 4, 1, P, P, None], 5, "pools"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 8, 16, 4, 1, P, P, None], 5, "multiples of 16"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 32, 16, 4, 1, P, P, None], 5, "multiples of 16"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P + 8), 1, 16, 16, 4, 1, P, P, None], 5, "aligned"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 16, 16, 4, 1, None, P, None], 5, "NULL"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 16, 16, 4, -1, P, P, None], 5, "copies"),
+    ("sile_hip_kv_free", [4, 4, P, P, P + 4, P, P, 9, P, P, None], 5, "tables overlap"),
+    ("sile_hip_kv_free", [4, 4, P, P, P, P, P + 4, 9, P, P, None], 5, "lengths overlap"),
+    ("sile_hip_kv_free", [4, 4, P, P, P, P, P, 9, P, P + 4, None], 5, "counts overlap"),
+    ("sile_hip_kv_free", [4, 4, None, P, P, P, P, 9, P, P, None], 5, "NULL"),
+    ("sile_hip_kv_fork", [4, 4, 4, P, P, P, TABLES, 2 * TABLES, 9, P, P, None], 5, "must not overlap"),
+    ("sile_hip_kv_fork", [4, 4, 4, P, TABLES, 2 * TABLES, P, P, 9, P, P, None], 5, "must not overlap"),
+    ("sile_hip_kv_fork", [-1, 4, 4, P, TABLES, 2 * TABLES, P, P, 9, P, P, None], 5, "negative"),
+    ("sile_hip_kv_reserve", [4, 4, 3, P, P, P, P, 9, P, P, P, None, 0, 0, 0, P, 1 << 20, None], 5, "power of two"),
+    ("sile_hip_kv_reserve", [4, 4, 16, P, P, P, P, 9, P, P, P, None, 0, 0, 0, None, 0, None], 5, "workspace"),
+    ("sile_hip_kv_reserve", [4, 4, 16, P, P, P, P, 9, P, P, P, None, 0, 0, 0, P, 64, None], 5, "workspace"),
+    ("sile_hip_kv_reserve", [4, 4, 16, P, P, P, P, 9, P, P, None, None, 0, 0, 0, P, 1 << 20, None], 5, "NULL"),
+    ("sile_hip_kv_reserve", [4, 4, 16, P, P, P, P + 4, 9, P, P, P, None, 0, 0, 0, P, 1 << 20, None], 5, "tables overlap"),
+    ("sile_hip_kv_compact", [4, 4, P, P, 9, P, P, None, None, 0, 0, 0, P, 1 << 20, None], 5, "NULL"),
+    ("sile_hip_kv_compact", [4, 4, P, P, 9, P, P, P, None, 0, 0, 0, P + 4, 1 << 20, None], 5, "aligned"),
+    ("sile_hip_kv_workspace", [-1, 4, ctypes.byref(ctypes.c_size_t())], 5, "rows"),
+    ("sile_hip_kv_workspace", [4, 4, None], 5, "NULL"),
+    ("sile_hip_paged_attn_workspace", [1, 5, 2, 64, ctypes.byref(ctypes.c_size_t())], 5, "query heads"),
+])
+def test_bookkeeping_refusals(name, args, code, needle):
+    refused(name, args, code, needle)
