@@ -443,6 +443,27 @@ int sile_hip_flash_attn_fwd(sile_dtype dtype, int64_t batch, int64_t heads, int6
                             int64_t head_dim, const void *q, const void *k, const void *v,
                             void *o, float scale, int causal, sile_hip_stream stream);
 
+/* Flash-attention forward of a prompt over a sliding window, O = softmax(Q K^T *
+ * scale + mask) V: query i < q_len, at position p = q_start + i, sees the keys j <= p
+ * with j > p - window or j < sinks (the first tokens, which stay visible), j < kv_len.
+ * Q, O [batch][q_heads][q_len][head_dim], K, V [batch][kv_heads][kv_len][head_dim], all
+ * contiguous, f16 or bf16; query head h reads key head h / (q_heads / kv_heads).  With
+ * q_start > 0 the queries follow keys that are there already (a prompt in pieces); window
+ * >= q_start + q_len is plain causal attention.  A query that sees no key gives zeros;
+ * what lies in keys it does not see never reaches it, NaN and Inf included.  head_dim a
+ * multiple of 8 up to 256 with 16-byte aligned operands and scale > 0 runs on the matrix
+ * cores (the probabilities enter the second product in 16 bits; a row's rounding can depend on
+ * the shape of the call); others on a VALU kernel of one wave per query row.  A row
+ * whose result is not finite, or meets Inf or NaN in V of a masked key of its block, is
+ * taken again row by row: right, but slow.  q_start + q_len <= 2^29, and one head's
+ * K at most 2^31 - 1 bytes.  Its form for single tokens: sile_hip_paged_attn_decode.
+ * No reference counterpart, as sile_hip_flash_attn_fwd. */
+int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_heads,
+                                   int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                   int64_t head_dim, const void *q, const void *k, const void *v,
+                                   void *o, float scale, int64_t q_start, int64_t window,
+                                   int64_t sinks, sile_hip_stream stream);
+
 /* ---- a paged key-value cache, for programs that answer token by token -------
  * No counterpart in the reference: its DSL cannot index a page table.  A cache
  * is, all of it in the caller's device memory:

@@ -154,6 +154,8 @@ SIGNATURES = {
     "sile_hip_attention_f32_kt": [_I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _F32,
                                   _F32, _P],
     "sile_hip_matvec_f32": [_I64, _I64, _I64, _P, _I64, _P, _F32, _P, _P],
+    "sile_hip_flash_attn_window_fwd": [_I32, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _F32,
+                                       _I64, _I64, _I64, _P],
     "sile_hip_kv_append": [_I32, _I32, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64,
                            _I64, _I64, _P, _I64, _I64, _F32, _F32, _P],
     "sile_hip_kv_copy_pages": [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P],
@@ -500,6 +502,12 @@ def flash_attn_fwd(dtype, batch, heads, seq_len, head_dim, q, k, v, o, scale, ca
                    stream=None):
     call("sile_hip_flash_attn_fwd", dtype, batch, heads, seq_len, head_dim, q, k, v, o, scale,
          1 if causal else 0, _sh(stream))
+
+
+def flash_attn_window_fwd(dtype, batch, q_heads, kv_heads, q_len, kv_len, head_dim, q, k, v, o,
+                          scale, q_start, window, sinks=0, stream=None):
+    call("sile_hip_flash_attn_window_fwd", dtype, batch, q_heads, kv_heads, q_len, kv_len, head_dim,
+         q, k, v, o, scale, q_start, window, sinks, _sh(stream))
 
 
 def attention_f32_kt(n_q, n_k, head_dim, q, ldq, kt, ldkt, v, ldv, o, ldo, scale, m0,

@@ -29,7 +29,8 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
-KERNELS = ["dsl", "softmax", "gemm", "attention", "flash_attn", "paged_attn", "kv_cache"]
+KERNELS = ["dsl", "softmax", "gemm", "attention", "flash_attn", "flash_window", "paged_attn",
+           "kv_cache"]
 HOST_SOURCES = ["runtime.cpp", "ops.cpp", "paged.cpp", "llir.cpp", "tile_ir.cpp"]
 HIP_HOST_SOURCES = ["launch_noalloc.hip"]
 

@@ -235,6 +235,31 @@ FlashPlan flash_plan(int64_t bh, int64_t seq, int head_dim, bool causal) {
   return best;
 }
 
+// Key groups of the windowed kernel: the count with the least modelled time, as in
+// flash_plan, for query blocks that all take the keys of their window (of the last
+// query's length at most), their own and the sinks.
+int window_groups(int64_t heads, int64_t q_len, int64_t last_len, int64_t window, int64_t sinks,
+                  int head_dim) {
+  int cus = 0, best = 1;
+  if (head_dim > 128 || device_cus(&cus) != SILE_OK) return 1;
+  const int64_t key_block = head_dim <= 64 ? 64 : 32;
+  double best_t = 1e30;
+  for (int g : {1, 2, 4}) {
+    const double lo = g == 1 ? 0.72 : g == 2 ? 0.82 : 0.95, hi = g == 1 ? 0.95 : g == 2 ? 1.1 : 1.35;
+    const int64_t bq = 256 / g, wgs = heads * ((q_len + bq - 1) / bq);
+    const int64_t keys = std::min(last_len, window + std::min(bq, q_len) + key_block) + std::min(sinks, last_len);
+    const double iters = (double)(((keys + key_block * g - 1) / (key_block * g) + 1) / 2 * 2);
+    const double merge = g == 1 ? 0.0 : g == 2 ? 0.5 : 1.5;
+    const double tau = lo + (hi - lo) * std::min(1.0, (double)wgs / cus);
+    const double t = (double)((wgs + cus - 1) / cus) * (tau * iters + 5.0 + merge);
+    if (t < best_t) {
+      best_t = t;
+      best = g;
+    }
+  }
+  return best;
+}
+
 // Workgroups of one row a group of lanes from which on the sums of narrow rows are
 // taken four a group (bf16 65536 x 200, 8192 of them: 7.5 -> 6.5 us; 32768 x 200:
 // 3 % slower, and 16384 x 200 21 %).
@@ -1223,6 +1248,64 @@ int sile_hip_flash_attn_fwd(sile_dtype dtype, int64_t batch, int64_t heads, int6
   const char* name = dtype == SILE_F16 ? "sile_attn_fwd_rowwise_f16" : "sile_attn_fwd_rowwise_bf16";
   void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &bh, &seq_len, &head_dim, &scale, &causal};
   int rc = launch(Module::kAttention, name, dim3((unsigned)blocks), dim3(256), params, s);
+  return rc == SILE_OK ? ok() : rc;
+}
+
+int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_heads,
+                                   int64_t kv_heads, int64_t q_len, int64_t kv_len,
+                                   int64_t head_dim, const void* q, const void* k, const void* v,
+                                   void* o, float scale, int64_t q_start, int64_t window,
+                                   int64_t sinks, sile_hip_stream stream) {
+  if (dtype != SILE_F16 && dtype != SILE_BF16)
+    return fail(SILE_ERR_UNSUPPORTED_BACKEND, "attention over %s not supported", dtype_name(dtype));
+  if (batch < 0 || q_heads < 0 || kv_heads < 0 || q_len < 0 || kv_len < 0 || head_dim <= 0)
+    return fail(SILE_ERR_SHAPE, "invalid attention shape");
+  if (q_start < 0 || window <= 0 || sinks < 0)
+    return fail(SILE_ERR_SHAPE, "start %lld, window %lld, sinks %lld", (long long)q_start,
+                (long long)window, (long long)sinks);
+  if (batch == 0 || q_heads == 0 || q_len == 0) return ok();
+  if (kv_heads == 0 || q_heads % kv_heads != 0)
+    return fail(SILE_ERR_SHAPE, "%lld query heads over %lld key heads", (long long)q_heads, (long long)kv_heads);
+  if (!q || !o || (kv_len > 0 && (!k || !v))) return fail(SILE_ERR_SHAPE, "NULL operand");
+  if (head_dim > 256) return fail(SILE_ERR_UNSUPPORTED_BACKEND, "head_dim > 256 not supported");
+  // positions in 32 bits with room for the masks' differences; one head's K or V is
+  // one buffer resource (32-bit byte range)
+  constexpr int64_t kMost = 1ll << 29;
+  if (q_start > kMost || q_len > kMost - q_start || kv_len > kMost || kv_len * head_dim * 2 > 0x7fffffffLL)
+    return fail(SILE_ERR_SHAPE, "sequence too long for one head (%lld + %lld queries, %lld keys)",
+                (long long)q_start, (long long)q_len, (long long)kv_len);
+  if (batch > 0x7fffffffLL / q_heads || batch * q_heads > 0x7fffffffLL / q_len)
+    return fail(SILE_ERR_SHAPE, "attention too large");
+  const int64_t last_len = q_start + q_len;
+  // a window past the last query's position sees what one that long does
+  struct {
+    int64_t q_len, kv_len, start, window, sinks;
+    int32_t items, q_blocks, group, d;
+    float scale_log2;
+  } wa{q_len, kv_len, q_start, std::min(window, last_len), std::min(sinks, kv_len), 0, 0,
+       (int32_t)(q_heads / kv_heads), (int32_t)head_dim, scale * 1.4426950408889634f};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const char* dt = dtype == SILE_F16 ? "f16" : "bf16";
+  char name[64];
+  // the matrix kernel, as for sile_hip_flash_attn_fwd
+  if (head_dim % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && scale > 0.0f) {
+    const int dh = head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128
+                 : head_dim <= 192 ? 192 : 256;
+    const int groups = window_groups(batch * q_heads, q_len, last_len, wa.window, wa.sinks, dh);
+    const int waves = dh <= 128 ? 8 : 4;
+    const int64_t bq = 32 * waves / groups;
+    wa.q_blocks = (int32_t)((q_len + bq - 1) / bq);
+    wa.items = (int32_t)(batch * q_heads * wa.q_blocks);
+    snprintf(name, sizeof name, "sile_flash_window_%s_d%d_g%d", dt, dh, groups);
+    void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa};
+    const unsigned blocks = (unsigned)((wa.items + 7ll) / 8 * 8);
+    const int rc = launch(Module::kFlashWindow, name, dim3(blocks), dim3((unsigned)(64 * waves)), params, s);
+    return rc == SILE_OK ? ok() : rc;
+  }
+  int64_t rows = batch * q_heads * q_len;
+  snprintf(name, sizeof name, "sile_flash_window_rowwise_%s", dt);
+  void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa, &rows};
+  const int rc = launch(Module::kFlashWindow, name, dim3((unsigned)((rows + 3) / 4)), dim3(256), params, s);
   return rc == SILE_OK ? ok() : rc;
 }
 

@@ -43,6 +43,7 @@ SILE_EMBED(sile_co_attention, "attention.hsaco")
 SILE_EMBED(sile_co_flash_attn, "flash_attn.hsaco")
 SILE_EMBED(sile_co_paged_attn, "paged_attn.hsaco")
 SILE_EMBED(sile_co_kv_cache, "kv_cache.hsaco")
+SILE_EMBED(sile_co_flash_window, "flash_window.hsaco")
 
 namespace sile_rt {
 namespace {
@@ -61,6 +62,7 @@ const Image kImages[static_cast<int>(Module::kCount)] = {
     {sile_co_flash_attn_begin, sile_co_flash_attn_end, "flash_attn"},
     {sile_co_paged_attn_begin, sile_co_paged_attn_end, "paged_attn"},
     {sile_co_kv_cache_begin, sile_co_kv_cache_end, "kv_cache"},
+    {sile_co_flash_window_begin, sile_co_flash_window_end, "flash_window"},
 };
 
 struct DeviceState {

@@ -35,7 +35,8 @@ enum class Module : int {
   kFlashAttn = 4,
   kPagedAttn = 5,
   kKvCache = 6,
-  kCount = 7
+  kFlashWindow = 7,
+  kCount = 8
 };
 
 inline const char* dtype_name(int t) {

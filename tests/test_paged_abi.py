@@ -166,3 +166,24 @@ TABLES = 1 << 20
 ])
 def test_bookkeeping_refusals(name, args, code, needle):
     refused(name, args, code, needle)
+
+
+WINDOW = [F16, 2, 4, 2, 10, 20, 64, P, P, P, P, 0.125, 10, 5, 1, None]
+
+
+@pytest.mark.parametrize("at,value,code,needle", [
+    (0, F32, 2, "f32"), (1, -1, 5, "shape"), (3, 3, 5, "query heads"), (3, 0, 5, "query heads"), (4, -1, 5, "shape"),
+    (6, 0, 5, "shape"), (6, 257, 2, "head_dim"), (7, None, 5, "NULL"), (8, None, 5, "NULL"), (10, None, 5, "NULL"),
+    (12, -1, 5, "start"), (13, 0, 5, "window"), (14, -1, 5, "sinks"), (12, 2 ** 29, 5, "too long"), (5, 2 ** 24, 5, "too long"),
+    (1, 2 ** 31, 5, "too large")])
+def test_window_refusals(at, value, code, needle):
+    args = list(WINDOW)
+    args[at] = value
+    refused("sile_hip_flash_attn_window_fwd", args, code, needle)
+
+
+def test_window_without_queries_is_fine():
+    for at in (1, 2, 4):
+        args = list(WINDOW)
+        args[at] = 0
+        assert _abi.status("sile_hip_flash_attn_window_fwd", *args) == 0
