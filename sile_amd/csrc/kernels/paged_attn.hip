@@ -135,7 +135,7 @@ struct DealLds {
   int32_t row, before;
 };
 
-template <bool kBF16, bool kFp8, int kDp, bool kExact, int kQT>
+template <bool kBF16, bool kFp8, int kDp, bool kExact, bool kPage16, int kQT>
 __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, float* ml,
                                            DealLds* deal) {
   using Sh = Shape<kDp, kQT>;
@@ -173,7 +173,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
     if (w < wave) before += deal->wave_sum[w];
     rows_total += deal->wave_sum[w];
   }
-  const int32_t total = rows_total * heads;
+  const int32_t total = __builtin_amdgcn_readfirstlane(rows_total) * heads;
   const int32_t chunk = deal_chunk(total, a.grid);
   int32_t x = blockIdx.x * (int64_t)chunk < total ? blockIdx.x * chunk : total;
   const int32_t x1 = total - x < chunk ? total : x + chunk;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
   uint8_t* const vt = smem + wave * Sh::kWaveB;
 
   while (x < x1) {
-    const KeySpan span = key_span(a.lengths[row], a.capacity, a.window, a.sinks);
+    const KeySpan span = key_span(__builtin_amdgcn_readfirstlane(a.lengths[row]), a.capacity, a.window, a.sinks);
     if (span.tiles == 0 || x >= base + span.tiles * heads) {   // on to the next row
       base += span.tiles * heads;
       ++row;
@@ -212,15 +212,18 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
     const int head0 = kvh * a.group + hg * 16 * kQT;
     const int32_t* table = a.tables + (int64_t)row * a.ld_table;
 
+    int qlane = lane;
+    asm volatile("" : "+v"(qlane));   // (as at the end)
+    const int qg = qlane >> 4, ql = qlane & 15;
     // ---- Q^T fragments: query head l16 of tile qt, zeros past the heads and dims ----
     u32x4 qf[kQT][kKK];
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
-      const bool in = qt * 16 + l16 < rows;
-      const uint16_t* qr = a.q + (int64_t)row * a.ldq + (int64_t)(head0 + (in ? qt * 16 + l16 : 0)) * d;
+      const bool in = qt * 16 + ql < rows;
+      const uint16_t* qr = a.q + (int64_t)row * a.ldq + (int64_t)(head0 + (in ? qt * 16 + ql : 0)) * d;
 #pragma unroll
       for (int kk = 0; kk < kKK; ++kk) {
-        const int dim = kFp8 ? 64 * (kk / 2) + 16 * g + 8 * (kk & 1) : 32 * kk + 8 * g;
+        const int dim = kFp8 ? 64 * (kk / 2) + 16 * qg + 8 * (kk & 1) : 32 * kk + 8 * qg;
         u32x4 w = {0u, 0u, 0u, 0u};
         if (in && (kExact || dim < d)) w = *reinterpret_cast<const u32x4*>(qr + dim);
         qf[qt][kk] = w;
@@ -244,41 +247,92 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
       const int key = span_key(span, min(t, t1 - 1)) + (lane & 31);
       return table[min(key, span.len - 1) >> a.page_shift];
     };
+    // (defined by an empty asm: left undefined before a unit's first loads, they are kept
+    // in registers a second time, from the unit before)
     u32x4 kr[2][kKL], vr[kVL];
+#pragma unroll
+    for (int i = 0; i < kKL; ++i) asm volatile("" : "=v"(kr[0][i]), "=v"(kr[1][i]));
+#pragma unroll
+    for (int i = 0; i < kVL; ++i) asm volatile("" : "=v"(vr[i]));
     const int64_t head_off = (int64_t)kvh * d << a.page_shift;
-    // issues tile t's loads; returns the mask of its keys that are read
+    const int row_b = d * kEs;
+    // issues tile t's loads; returns the mask of its keys that are seen
     auto load_tile = [&](int t, int32_t id) -> uint32_t {
-      const int key0 = span_key(span, min(t, t1 - 1)) + (lane & 31);
-      const bool ok = t < t1 && span_sees(span, key0) && (uint32_t)id < (uint32_t)a.num_pages;
-      const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
-      if (seen == 0) return 0;
-      const int slot = key0 & ((1 << a.page_shift) - 1);
-      // keys that are not read take page 0's row of the same slot, which is there
-      const int64_t off = ((int64_t)(ok ? id : 0) * a.page_stride + head_off + (int64_t)slot * d) * kEs;
-      const int off_lo = (int)(uint32_t)off, off_hi = (int)(off >> 32);
-      auto row_off = [&](int key) {
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * key, off_lo);
-        const int32_t hi = __builtin_amdgcn_ds_bpermute(4 * key, off_hi);
-        return (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo);
-      };
+      if constexpr (kPage16) {
+        // 16 keys lie in one page: a buffer resource over their rows, which ends at
+        // the row's last key and is empty where the page does not exist, so
+        // that what lies past it is never read (it loads as zeros); all of it scalar
+        const int32_t ids[2] = {__builtin_amdgcn_readlane(id, 0), __builtin_amdgcn_readlane(id, 16)};
+        const int key0 = span_key(span, min(t, t1 - 1));
+        uint32_t seen = t < t1 ? span_bits(span, key0) : 0u;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const uint8_t* p = a.k + row_off(16 * s + l16);
+        for (int s = 0; s < 2; ++s)
+          if ((uint32_t)ids[s] >= (uint32_t)a.num_pages) seen &= s ? 0x0000ffffu : 0xffff0000u;
+        if (seen == 0) return 0;
+        const int slot = key0 & ((1 << a.page_shift) - 1);
 #pragma unroll
-        for (int i = 0; i < kKL; ++i) {
-          const int c = 4 * i + g;
-          u32x4 w = {0u, 0u, 0u, 0u};
-          if (kExact || c < chunks) w = *reinterpret_cast<const u32x4*>(p + 16 * c);
-          kr[s][i] = w;
+        for (int s = 0; s < 2; ++s) {
+          const bool ok = (uint32_t)ids[s] < (uint32_t)a.num_pages;
+          // (through readfirstlane: the clamp is a vector instruction, and a resource in
+          // vector registers costs a loop around every load)
+          const int rows_in =
+              __builtin_amdgcn_readfirstlane(ok ? min(max(span.len - key0 - 16 * s, 0), 16) : 0);
+          const int64_t at = (int64_t)(ok ? ids[s] : 0) * a.page_stride + head_off +
+                             (int64_t)((slot + 16 * s) & ((1 << a.page_shift) - 1)) * d;
+          const __amdgpu_buffer_rsrc_t kb = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(a.k + at * kEs), (short)0, rows_in * row_b, 0x00020000);
+          const __amdgpu_buffer_rsrc_t vb = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(a.v + at * kEs), (short)0, rows_in * row_b, 0x00020000);
+#pragma unroll
+          for (int i = 0; i < kKL; ++i) {
+            const int c = 4 * i + g;   // (a chunk past the dims: past the resource, zeros)
+            const int off = kExact || c < chunks ? l16 * row_b + 16 * c : 0x7fff0000;
+            kr[s][i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kb, off, 0, 0));
+          }
+#pragma unroll
+          for (int i = 0; i < kVL / 2; ++i) {
+            const int c = lane % kCh;
+            const int off = kExact || c < chunks ? (kVRows * i + lane / kCh) * row_b + 16 * c : 0x7fff0000;
+            vr[s * (kVL / 2) + i] =
+                __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vb, off, 0, 0));
+          }
         }
-      }
+        return seen;
+      } else {
+        // pages of 1 to 8 keys: every lane works out its own key's row, the lanes that
+        // load it ask that lane
+        const int key = span_key(span, min(t, t1 - 1)) + (lane & 31);
+        const bool ok = t < t1 && span_sees(span, key) && (uint32_t)id < (uint32_t)a.num_pages;
+        const uint32_t seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+        if (seen == 0) return 0;
+        const int slot = key & ((1 << a.page_shift) - 1);
+        // keys that are not seen take page 0's row of the same slot, which is there
+        const int64_t off = ((int64_t)(ok ? id : 0) * a.page_stride + head_off + (int64_t)slot * d) * kEs;
+        const int off_lo = (int)(uint32_t)off, off_hi = (int)(off >> 32);
+        auto row_off = [&](int k) {
+          const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(4 * k, off_lo);
+          const int32_t hi = __builtin_amdgcn_ds_bpermute(4 * k, off_hi);
+          return (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo);
+        };
 #pragma unroll
-      for (int i = 0; i < kVL; ++i) {
-        const int c = lane % kCh;   // a chunk past the dims reads chunk 0 (its O^T rows are not kept)
-        const uint8_t* p = a.v + row_off(kVRows * i + lane / kCh);
-        vr[i] = *reinterpret_cast<const u32x4*>(p + 16 * (kExact || c < chunks ? c : 0));
+        for (int s = 0; s < 2; ++s) {
+          const uint8_t* p = a.k + row_off(16 * s + l16);
+#pragma unroll
+          for (int i = 0; i < kKL; ++i) {
+            const int c = 4 * i + g;
+            u32x4 w = {0u, 0u, 0u, 0u};
+            if (kExact || c < chunks) w = *reinterpret_cast<const u32x4*>(p + 16 * c);
+            kr[s][i] = w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kVL; ++i) {
+          const int c = lane % kCh;   // a chunk past the dims reads chunk 0 (its O^T rows are not kept)
+          const uint8_t* p = a.v + row_off(kVRows * i + lane / kCh);
+          vr[i] = *reinterpret_cast<const u32x4*>(p + 16 * (kExact || c < chunks ? c : 0));
+        }
+        return seen;
       }
-      return seen;
     };
     auto vswz = [](int r) { return (kDp == 64 ? 2 : 4) * (r & 3); };
 
@@ -341,16 +395,15 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
 #pragma unroll
       for (int qt = 0; qt < kQT; ++qt) {
         float sc[8];
-        float mx = -__builtin_inff();
+        float mx = kLowest;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float v = sacc[qt][i >> 2][i & 3] * a.scale_log2;
-          const bool in = (bits >> i) & 1;
-          sc[i] = in ? v : -__builtin_inff();
-          mx = __builtin_fmaxf(mx, in ? __builtin_fmaxf(v, kLowest) : -__builtin_inff());
+          sc[i] = sacc[qt][i >> 2][i & 3] * a.scale_log2;
+          if (now != 0xffffffffu) sc[i] = (bits >> i) & 1 ? sc[i] : -__builtin_inff();
+          mx = __builtin_fmaxf(mx, sc[i]);
         }
-        const float m_new = __builtin_fmaxf(m_run[qt], quad_max(mx));
-        const float alpha = exp2_fast(m_run[qt] - m_new);   // (m_new > -inf: a key is seen)
+        const float m_new = __builtin_fmaxf(m_run[qt], quad_max(mx));   // (> -inf: a key is seen)
+        const float alpha = exp2_fast(m_run[qt] - m_new);
         m_run[qt] = m_new;
         float rs = 0.0f;
 #pragma unroll
@@ -395,20 +448,25 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
     }
 
     // ---- the four waves' (m, l, O) added up ----
+    // (the thread number through an empty asm: addresses worked out here are not
+    // kept in registers through the rounds)
+    int et = tid;
+    asm volatile("" : "+v"(et));
+    const int eg = (et & 63) >> 4, el = et & 15;
     const bool whole = t0 == 0 && t1 == span.tiles;
     const int slot = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
 #pragma unroll
     for (int qt = 0; qt < kQT; ++qt) {
       const float l = quad_sum(l_run[qt]);
-      if (g == 0) {
-        ml[(wave * 16 + l16) * 2] = m_run[qt];
-        ml[(wave * 16 + l16) * 2 + 1] = l;
+      if (eg == 0) {
+        ml[(wave * 16 + el) * 2] = m_run[qt];
+        ml[(wave * 16 + el) * 2 + 1] = l;
       }
-      float* ot = reinterpret_cast<float*>(vt) + l16 * Sh::kPitch + 4 * g;
+      float* ot = reinterpret_cast<float*>(vt) + el * Sh::kPitch + 4 * eg;
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<f32x4*>(ot + 16 * dt) = oacc[qt][dt];
       __syncthreads();
-      const int r = tid >> 4, head = qt * 16 + r;
+      const int r = et >> 4, head = qt * 16 + r;
       float w[4], m = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) m = __builtin_fmaxf(m, ml[(i * 16 + r) * 2]);
@@ -422,7 +480,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
         // a row without keys gives zeros; scores that are all -inf give 0 / 0
         const float f = whole ? (m == -__builtin_inff() ? 0.0f : a.v_scale / sum) : 1.0f;
         const int64_t at = (int64_t)slot * 16 * kQT + head;
-        for (int c = 4 * (tid & 15); c < d; c += 64) {
+        for (int c = 4 * (et & 15); c < d; c += 64) {
           f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -438,7 +496,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
             *reinterpret_cast<f32x4*>(a.part_o + at * d + c) = acc;
           }
         }
-        if (!whole && (tid & 15) == 0) {
+        if (!whole && (et & 15) == 0) {
           a.part_ml[at * 2] = m;
           a.part_ml[at * 2 + 1] = sum;
         }
@@ -448,43 +506,89 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
   }
 }
 
-// Joins a unit's parts (row, key head, head group: blockIdx.x; four query heads a
-// workgroup, a wave each: blockIdx.y), or writes the zeros of a row without keys.
+// Joins the parts of a unit (row, key head, head group: blockIdx.x), or writes the zeros
+// of a row without keys.  A part is a few hundred bytes and there are two or three of
+// it, or, where a long row is all there is, one a workgroup: `split` (1, 2, 4 or 8) of a
+// workgroup's eight waves take a query head's parts in turn, each lane up to four dims, eight
+// parts' loads in flight, and the waves' sums are added up through LDS in their order;
+// the waves left over take the next query heads (blockIdx.y: groups of 8 / split).
+constexpr int kJoinWaves = 8;
 template <bool kBF16, int kQT>
-__device__ __forceinline__ void paged_join(const PagedArgs& a) {
+__device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float* lds) {
   const int heads = a.kv_heads * a.head_groups;
   const int row = blockIdx.x / heads, unit = blockIdx.x - row * heads;
   const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
-  const int rows = min(16 * kQT, a.group - hg * 16 * kQT);
-  const int lane = threadIdx.x & 63;
-  const int r = 4 * blockIdx.y + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const KeySpan span = key_span(a.lengths[row], a.capacity, a.window, a.sinks);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int part0 = wave % split, r = blockIdx.y * (kJoinWaves / split) + wave / split;
+  const bool in = r < min(16 * kQT, a.group - hg * 16 * kQT);
+  const int32_t length = a.lengths[row], before = a.plan[row], chunk = a.plan[a.batch];
+  const KeySpan span = key_span(length, a.capacity, a.window, a.sinks);
   uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)(kvh * a.group + hg * 16 * kQT + r) * a.d;
   if (span.tiles == 0) {
-    for (int c = lane; c < a.d; c += 64) o[c] = 0;
+    if (in && part0 == 0)
+      for (int c = lane; c < a.d; c += 64) o[c] = 0;
     return;
   }
-  const int32_t chunk = a.plan[a.batch];
-  const int32_t x0 = a.plan[row] * heads + unit * span.tiles;
+  const int32_t x0 = before * heads + unit * span.tiles;
   const int32_t g0 = x0 / chunk, g1 = (x0 + span.tiles - 1) / chunk;
   if (g0 == g1) return;   // one workgroup had it whole
   auto at = [&](int32_t w) { return ((int64_t)(2 * w + (w == g0 ? 1 : 0)) * 16 * kQT + r); };
-  float m = -__builtin_inff();
-  for (int32_t w = g0 + lane; w <= g1; w += 64) m = __builtin_fmaxf(m, a.part_ml[at(w) * 2]);
-  m = wave_max(m);
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-#pragma unroll 4
-  for (int32_t w = g0; w <= g1; ++w) {
-    const float mi = a.part_ml[at(w) * 2];
-    const float f = mi == -__builtin_inff() ? 0.0f : exp2_fast(mi - m);
-    sum += f * a.part_ml[at(w) * 2 + 1];
-    const float* p = a.part_o + at(w) * a.d;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f, m = -__builtin_inff();
+  for (int32_t w0 = g0 + part0; in && w0 <= g1; w0 += 8 * split) {
+    float mi[8], li[8], v[8][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 64 * i < a.d) acc[i] += f * p[lane + 64 * i];
+    for (int u = 0; u < 8; ++u) {
+      const int32_t w = w0 + u * split;
+      mi[u] = -__builtin_inff();
+      li[u] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[u][i] = 0.0f;
+      if (w <= g1) {
+        mi[u] = a.part_ml[at(w) * 2];
+        li[u] = a.part_ml[at(w) * 2 + 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (lane + 64 * i < a.d) v[u][i] = a.part_o[at(w) * a.d + lane + 64 * i];
+      }
+    }
+    float m_new = m;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m_new = __builtin_fmaxf(m_new, mi[u]);
+    if (m_new == -__builtin_inff()) continue;   // no key seen so far
+    const float alpha = exp2_fast(m - m_new);
+    m = m_new;
+    sum *= alpha;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] *= alpha;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float f = exp2_fast(mi[u] - m);   // (a part without keys: m_i = -inf, 0)
+      sum += f * li[u];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += f * v[u][i];
+    }
   }
-  const float f = m == -__builtin_inff() ? 0.0f : a.v_scale / sum;
+  float top = m, all = sum;
+  if (split > 1) {
+    if (lane == 0) {
+      lds[2 * wave] = m;
+      lds[2 * wave + 1] = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[2 * kJoinWaves + 256 * wave + 64 * i + lane] = acc[i];
+    __syncthreads();
+    if (part0 != 0) return;
+    for (int w = wave; w < wave + split; ++w) top = __builtin_fmaxf(top, lds[2 * w]);
+    all = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+    for (int w = wave; w < wave + split; ++w) {
+      const float f = lds[2 * w] == -__builtin_inff() ? 0.0f : exp2_fast(lds[2 * w] - top);
+      all += f * lds[2 * w + 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] += f * lds[2 * kJoinWaves + 256 * w + 64 * i + lane];
+    }
+  }
+  if (!in) return;
+  const float f = top == -__builtin_inff() ? 0.0f : a.v_scale / all;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (lane + 64 * i < a.d)
@@ -493,30 +597,35 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a) {
 
 }  // namespace
 
-#define SILE_PAGED_KERNEL(NAME, BF, F8, DP, EX, QT, EU)                                   \
+#define SILE_PAGED_KERNEL(NAME, BF, F8, DP, EX, P16, QT, EU)                              \
   extern "C" __global__ __launch_bounds__(256, EU) void NAME(PagedArgs a) {               \
     __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * Shape<DP, QT>::kWaveB];    \
     __shared__ float ml[4 * 16 * 2];                                                      \
     __shared__ DealLds deal;                                                              \
-    paged_attn<BF, F8, DP, EX, QT>(a, smem, ml, &deal);                                   \
+    paged_attn<BF, F8, DP, EX, P16, QT>(a, smem, ml, &deal);                              \
   }
-// d<D>: that head dimension; p<D>: any smaller one.  q<N>: N tiles of 16 query heads.
-#define SILE_PAGED_TYPES(SUFFIX, DP, EX, QT, EU)                                  \
-  SILE_PAGED_KERNEL(sile_paged_attn_f16_##SUFFIX, false, false, DP, EX, QT, EU)   \
-  SILE_PAGED_KERNEL(sile_paged_attn_bf16_##SUFFIX, true, false, DP, EX, QT, EU)   \
-  SILE_PAGED_KERNEL(sile_paged_attn_f16_fp8_##SUFFIX, false, true, DP, EX, QT, EU) \
-  SILE_PAGED_KERNEL(sile_paged_attn_bf16_fp8_##SUFFIX, true, true, DP, EX, QT, EU)
-#define SILE_PAGED_DIM(DP, QT, EU)                \
-  SILE_PAGED_TYPES(d##DP##_q##QT, DP, true, QT, EU)  \
-  SILE_PAGED_TYPES(p##DP##_q##QT, DP, false, QT, EU)
+// d<D>: that head dimension; p<D>: any smaller one; s<D>: any up to it, pages below 16
+// keys.  q<N>: N tiles of 16 query heads.
+#define SILE_PAGED_TYPES(SUFFIX, DP, EX, P16, QT, EU)                                  \
+  SILE_PAGED_KERNEL(sile_paged_attn_f16_##SUFFIX, false, false, DP, EX, P16, QT, EU)   \
+  SILE_PAGED_KERNEL(sile_paged_attn_bf16_##SUFFIX, true, false, DP, EX, P16, QT, EU)   \
+  SILE_PAGED_KERNEL(sile_paged_attn_f16_fp8_##SUFFIX, false, true, DP, EX, P16, QT, EU) \
+  SILE_PAGED_KERNEL(sile_paged_attn_bf16_fp8_##SUFFIX, true, true, DP, EX, P16, QT, EU)
+#define SILE_PAGED_DIM(DP, QT, EU)                         \
+  SILE_PAGED_TYPES(d##DP##_q##QT, DP, true, true, QT, EU)  \
+  SILE_PAGED_TYPES(p##DP##_q##QT, DP, false, true, QT, EU) \
+  SILE_PAGED_TYPES(s##DP##_q##QT, DP, false, false, QT, EU)
 SILE_PAGED_DIM(64, 1, 2)
 SILE_PAGED_DIM(64, 2, 2)
 SILE_PAGED_DIM(128, 1, 2)
 SILE_PAGED_DIM(128, 2, 1)
 SILE_PAGED_DIM(256, 1, 1)
 
-#define SILE_PAGED_JOIN(NAME, BF, QT) \
-  extern "C" __global__ __launch_bounds__(256) void NAME(PagedArgs a) { paged_join<BF, QT>(a); }
+#define SILE_PAGED_JOIN(NAME, BF, QT)                                             \
+  extern "C" __global__ __launch_bounds__(64 * kJoinWaves) void NAME(PagedArgs a, int split) { \
+    __shared__ float lds[(2 + 256) * kJoinWaves];                                 \
+    paged_join<BF, QT>(a, split, lds);                                            \
+  }
 SILE_PAGED_JOIN(sile_paged_attn_join_f16_q1, false, 1)
 SILE_PAGED_JOIN(sile_paged_attn_join_bf16_q1, true, 1)
 SILE_PAGED_JOIN(sile_paged_attn_join_f16_q2, false, 2)

@@ -52,6 +52,19 @@ SILE_HD bool span_sees(const KeySpan& s, int32_t key) {
   return key >= 0 && key < s.len && (key >= s.first || key < s.sink_end);
 }
 
+// The seen keys among the 32 from key0 on (a tile's first, below len), bit i key0 + i.
+SILE_HD uint32_t span_bits(const KeySpan& s, int32_t key0) {
+  const int32_t left = s.len - key0;
+  uint32_t m = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+  if (key0 < s.first) {
+    const int32_t w = s.first - key0, e = s.sink_end - key0;
+    const uint32_t in_window = w >= 32 ? 0u : 0xffffffffu << w;
+    const uint32_t in_sinks = e <= 0 ? 0u : e >= 32 ? 0xffffffffu : (1u << e) - 1u;
+    m &= in_window | in_sinks;
+  }
+  return m;
+}
+
 // Tiles a workgroup takes: an equal share of all tiles, at least one round of
 // its waves, in whole rounds.
 SILE_HD int32_t deal_chunk(int32_t total, int32_t workgroups) {

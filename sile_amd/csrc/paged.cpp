@@ -163,11 +163,11 @@ struct PagedPlan {
   int dp, q_tiles, per_cu, cus;
   int64_t head_groups, grid, plan_ints, slots, bytes;
 };
-int paged_plan(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, PagedPlan* p) {
+int paged_plan(bool fp8, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, PagedPlan* p) {
   const int64_t group = q_heads / kv_heads;
   p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
   p->q_tiles = group > 16 && p->dp < 256 ? 2 : 1;
-  p->per_cu = p->dp == 64 || (p->dp == 128 && p->q_tiles == 1) ? 2 : 1;
+  p->per_cu = p->dp == 64 ? (p->q_tiles == 1 ? 4 : 2) : p->dp == 128 && p->q_tiles == 1 ? (fp8 ? 3 : 2) : 1;
   const int rc = device_cus(&p->cus);
   if (rc != SILE_OK) return rc;
   p->head_groups = (group + 16 * p->q_tiles - 1) / (16 * p->q_tiles);
@@ -397,7 +397,8 @@ int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_hea
   int rc = check_heads(batch, q_heads, kv_heads, head_dim);
   if (rc != SILE_OK) return rc;
   PagedPlan plan;
-  if ((rc = paged_plan(batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
+  // (the 8-bit cache's grid is the larger one, where they differ)
+  if ((rc = paged_plan(true, batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
   *bytes = (size_t)plan.bytes;
   return ok();
 }
@@ -426,7 +427,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
     return fail(SILE_ERR_SHAPE, "q, o and the pages have to be 16-byte aligned");
   if (ldq > (1ll << 40) || ldo > (1ll << 40)) return fail(SILE_ERR_SHAPE, "leading dimension too large");
   PagedPlan plan;
-  if ((rc = paged_plan(batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
+  if ((rc = paged_plan(es == 1, batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, plan.bytes)) != SILE_OK) return rc;
   // without a page every row is empty
   const int64_t capacity = num_pages > 0 ? std::min<int64_t>(ld_table * page_size, kIntMax) : 0;
@@ -469,14 +470,20 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   const char* dt = dtype == SILE_F16 ? "f16" : "bf16";
   char name[64];
   snprintf(name, sizeof name, "sile_paged_attn_%s%s_%c%d_q%d", dt, cache_type == dtype ? "" : "_fp8",
-           head_dim == plan.dp ? 'd' : 'p', plan.dp, plan.q_tiles);
+           page_size < 16 ? 's' : head_dim == plan.dp ? 'd' : 'p', plan.dp, plan.q_tiles);
   void* params[] = {&a};
   rc = launch(Module::kPagedAttn, name, dim3((unsigned)plan.grid), dim3(256), params, s);
   if (rc != SILE_OK) return rc;
+  // a unit has about grid / units parts (and one or two more): up to 16 for one wave,
+  // two rounds of eight, then more waves
   const int64_t units = batch * kv_heads * plan.head_groups;
   const int64_t heads = std::min<int64_t>(a.group, 16 * plan.q_tiles);
+  const int64_t parts = plan.grid / units + 2;
+  int split = parts <= 16 ? 1 : parts <= 32 ? 2 : parts <= 64 ? 4 : 8;
+  const int64_t groups = (heads * split + 7) / 8;
   snprintf(name, sizeof name, "sile_paged_attn_join_%s_q%d", dt, plan.q_tiles);
-  rc = launch(Module::kPagedAttn, name, dim3((unsigned)units, (unsigned)((heads + 3) / 4)), dim3(256), params, s);
+  void* join[] = {&a, &split};
+  rc = launch(Module::kPagedAttn, name, dim3((unsigned)units, (unsigned)groups), dim3(512), join, s);
   return rc == SILE_OK ? ok() : rc;
 }
 

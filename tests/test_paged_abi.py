@@ -24,7 +24,9 @@ void cover(int32_t len, int64_t cap, int64_t window, int64_t sinks, int32_t n, i
   for (int32_t t = 0; t < s.tiles; ++t)
     for (int32_t i = 0; i < sile::kTileKeys; ++i) {
       const int32_t key = sile::span_key(s, t) + i;
-      if (sile::span_sees(s, key) && key < n) ++out[key];
+      const bool bit = (sile::span_bits(s, sile::span_key(s, t)) >> i) & 1;
+      if (bit != sile::span_sees(s, key)) out[0] = -1000;
+      if (bit && key < n) ++out[key];
     }
 }
 int32_t chunk(int32_t total, int32_t groups) { return sile::deal_chunk(total, groups); }
