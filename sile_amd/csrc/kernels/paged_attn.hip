@@ -25,7 +25,7 @@
 //    numbers of the one after.
 //
 // The tiles of all rows and key heads are one flat list, dealt in equal shares to
-// a fixed grid of workgroups (deal_chunk): a long row is spread over many
+// a fixed grid of workgroups (make_deal): a long row is spread over many
 // workgroups and a batch of mixed lengths has no straggler, with the lengths
 // known only on the device.  A workgroup whose share covers a row's key head
 // whole writes its output; the others leave (O, m, l) in fp32 in the workspace, at
@@ -56,11 +56,11 @@ struct PagedArgs {
   uint16_t* o;
   const int32_t* tables;
   const int32_t* lengths;
-  int32_t* plan;        // workspace: tiles of the rows before each row, then the total and the chunk
+  int32_t* plan;        // workspace: tiles of the rows before each row, then of all rows
   float* part_ml;       // workspace: [slots][rows][2]
   float* part_o;        // workspace: [slots][rows][d]
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
-  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, grid;
+  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups;
   float scale_log2, v_scale;
 };
 
@@ -158,7 +158,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
   const int per = (a.batch + 255) / 256;
   int32_t mine = 0;
   for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r)
-    mine += key_span(a.lengths[r], a.capacity, a.window, a.sinks).tiles;
+    mine += unit_size(key_span(a.lengths[r], a.capacity, a.window, a.sinks));
   int32_t incl = mine;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
@@ -174,13 +174,13 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
     rows_total += deal->wave_sum[w];
   }
   const int32_t total = __builtin_amdgcn_readfirstlane(rows_total) * heads;
-  const int32_t chunk = deal_chunk(total, a.grid);
-  int32_t x = blockIdx.x * (int64_t)chunk < total ? blockIdx.x * chunk : total;
-  const int32_t x1 = total - x < chunk ? total : x + chunk;
+  const Deal shares = make_deal(total, a.groups);
+  int32_t x = deal_start(shares, blockIdx.x);
+  const int32_t x1 = deal_start(shares, blockIdx.x + 1);
   if (blockIdx.x == 0 || x < x1) {
     int32_t at = before;
     for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r) {
-      const int32_t t = key_span(a.lengths[r], a.capacity, a.window, a.sinks).tiles;
+      const int32_t t = unit_size(key_span(a.lengths[r], a.capacity, a.window, a.sinks));
       if (blockIdx.x == 0) a.plan[r] = at;
       if (x < x1 && x / heads >= at && x / heads < at + t) {
         deal->row = r;
@@ -188,7 +188,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
       }
       at += t;
     }
-    if (blockIdx.x == 0 && tid == 0) a.plan[a.batch] = chunk;
+    if (blockIdx.x == 0 && tid == 0) a.plan[a.batch] = rows_total;
   }
   if (x >= x1) return;
   __syncthreads();
@@ -198,15 +198,17 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
 
   while (x < x1) {
     const KeySpan span = key_span(__builtin_amdgcn_readfirstlane(a.lengths[row]), a.capacity, a.window, a.sinks);
-    if (span.tiles == 0 || x >= base + span.tiles * heads) {   // on to the next row
-      base += span.tiles * heads;
+    const int32_t size = unit_size(span);
+    if (x >= base + size * heads) {   // on to the next row
+      base += size * heads;
       ++row;
       continue;
     }
-    const int unit = (x - base) / span.tiles;
-    const int t0 = x - base - unit * span.tiles;
-    const int t1 = min(span.tiles, t0 + (x1 - x));
-    x += t1 - t0;
+    const int unit = (x - base) / size;
+    const int u0 = x - base - unit * size, u1 = min(size, u0 + (x1 - x));
+    x += u1 - u0;
+    const int t0 = max(u0 - kUnitTiles, 0), t1 = u1 - kUnitTiles;
+    if (t1 <= t0) continue;   // of this unit only what it counts extra
     const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
     const int rows = min(16 * kQT, a.group - hg * 16 * kQT);   // query heads of this unit
     const int head0 = kvh * a.group + hg * 16 * kQT;
@@ -521,7 +523,7 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float*
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int part0 = wave % split, r = blockIdx.y * (kJoinWaves / split) + wave / split;
   const bool in = r < min(16 * kQT, a.group - hg * 16 * kQT);
-  const int32_t length = a.lengths[row], before = a.plan[row], chunk = a.plan[a.batch];
+  const int32_t length = a.lengths[row], before = a.plan[row], all_rows = a.plan[a.batch];
   const KeySpan span = key_span(length, a.capacity, a.window, a.sinks);
   uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)(kvh * a.group + hg * 16 * kQT + r) * a.d;
   if (span.tiles == 0) {
@@ -529,8 +531,9 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float*
       for (int c = lane; c < a.d; c += 64) o[c] = 0;
     return;
   }
-  const int32_t x0 = before * heads + unit * span.tiles;
-  const int32_t g0 = x0 / chunk, g1 = (x0 + span.tiles - 1) / chunk;
+  const Deal shares = make_deal(all_rows * heads, a.groups);
+  const int32_t x0 = before * heads + unit * unit_size(span) + kUnitTiles;
+  const int32_t g0 = deal_workgroup(shares, x0), g1 = deal_workgroup(shares, x0 + span.tiles - 1);
   if (g0 == g1) return;   // one workgroup had it whole
   auto at = [&](int32_t w) { return ((int64_t)(2 * w + (w == g0 ? 1 : 0)) * 16 * kQT + r); };
   float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f, m = -__builtin_inff();

@@ -49,7 +49,7 @@ struct PagedArgs {
   int32_t* plan;
   float *part_ml, *part_o;
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
-  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, grid;
+  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups;
   float scale_log2, v_scale;
 };
 
@@ -161,7 +161,7 @@ int copy_ints(const int32_t* from, int32_t* to, int64_t n, hipStream_t s) {
 // 16 query heads (two where a key head has more than 16), workgroups a CU holds.
 struct PagedPlan {
   int dp, q_tiles, per_cu, cus;
-  int64_t head_groups, grid, plan_ints, slots, bytes;
+  int64_t head_groups, groups, plan_ints, slots, bytes;
 };
 int paged_plan(bool fp8, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, PagedPlan* p) {
   const int64_t group = q_heads / kv_heads;
@@ -171,9 +171,9 @@ int paged_plan(bool fp8, int64_t batch, int64_t q_heads, int64_t kv_heads, int64
   const int rc = device_cus(&p->cus);
   if (rc != SILE_OK) return rc;
   p->head_groups = (group + 16 * p->q_tiles - 1) / (16 * p->q_tiles);
-  p->grid = (int64_t)p->per_cu * p->cus;
+  p->groups = (int64_t)p->per_cu * p->cus;
   p->plan_ints = ints16(batch + 1);
-  p->slots = 2 * p->grid * 16 * p->q_tiles;
+  p->slots = 2 * p->groups * 16 * p->q_tiles;   // two a workgroup
   p->bytes = 4 * (p->plan_ints + p->slots * (2 + head_dim));
   return SILE_OK;
 }
@@ -435,7 +435,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   const int64_t seen = window > 0 ? std::min<int64_t>(capacity, std::min<int64_t>(window, kIntMax) +
                                                                     std::min<int64_t>(sinks, kIntMax))
                                   : capacity;
-  const int64_t row_tiles = (seen / sile::kTileKeys + 3) * kv_heads * plan.head_groups;
+  const int64_t row_tiles = (seen / sile::kTileKeys + 3 + sile::kUnitTiles) * kv_heads * plan.head_groups;
   if (batch > (kIntMax - (1 << 20)) / row_tiles)
     return fail(SILE_ERR_SHAPE, "%lld rows of up to %lld keys: too many for one call", (long long)batch,
                 (long long)seen);
@@ -463,7 +463,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   a.d = (int32_t)head_dim;
   a.num_pages = (int32_t)num_pages;
   a.page_shift = page_shift_of(page_size);
-  a.grid = (int32_t)plan.grid;
+  a.groups = (int32_t)plan.groups;
   a.scale_log2 = scale * k_scale * 1.4426950408889634f;
   a.v_scale = v_scale;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -472,13 +472,14 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   snprintf(name, sizeof name, "sile_paged_attn_%s%s_%c%d_q%d", dt, cache_type == dtype ? "" : "_fp8",
            page_size < 16 ? 's' : head_dim == plan.dp ? 'd' : 'p', plan.dp, plan.q_tiles);
   void* params[] = {&a};
-  rc = launch(Module::kPagedAttn, name, dim3((unsigned)plan.grid), dim3(256), params, s);
+  const int32_t grid = sile::deal_workgroups(batch * row_tiles, a.groups);
+  rc = launch(Module::kPagedAttn, name, dim3((unsigned)grid), dim3(256), params, s);
   if (rc != SILE_OK) return rc;
-  // a unit has about grid / units parts (and one or two more): up to 16 for one wave,
+  // a unit has at most about grid / units parts (and one or two more): up to 16 for one wave,
   // two rounds of eight, then more waves
   const int64_t units = batch * kv_heads * plan.head_groups;
   const int64_t heads = std::min<int64_t>(a.group, 16 * plan.q_tiles);
-  const int64_t parts = plan.grid / units + 2;
+  const int64_t parts = grid / units + 2;
   int split = parts <= 16 ? 1 : parts <= 32 ? 2 : parts <= 64 ? 4 : 8;
   const int64_t groups = (heads * split + 7) / 8;
   snprintf(name, sizeof name, "sile_paged_attn_join_%s_q%d", dt, plan.q_tiles);

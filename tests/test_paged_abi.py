@@ -12,7 +12,7 @@ from sile_amd import _abi
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SOURCE = r"""
-#include "%s"
+#include "PLAN_H"
 extern "C" {
 void span(int32_t len, int64_t cap, int64_t window, int64_t sinks, int32_t* out) {
   const sile::KeySpan s = sile::key_span(len, cap, window, sinks);
@@ -29,7 +29,24 @@ void cover(int32_t len, int64_t cap, int64_t window, int64_t sinks, int32_t n, i
       if (bit && key < n) ++out[key];
     }
 }
-int32_t chunk(int32_t total, int32_t groups) { return sile::deal_chunk(total, groups); }
+// the shares of a list; returns the workgroups that have one, -1 if a share's tiles do not name it
+int32_t deal(int32_t total, int32_t groups) {
+  const sile::Deal d = sile::make_deal(total, groups);
+  const int32_t n = sile::deal_workgroups(total, groups);
+  int32_t at = 0, used = 0;
+  for (int32_t w = 0; w < n; ++w) {
+    const int32_t x0 = sile::deal_start(d, w), x1 = sile::deal_start(d, w + 1);
+    if (x0 != at || x1 < x0) return -1;
+    if (x1 > x0) {
+      ++used;
+      if (sile::deal_workgroup(d, x0) != w || sile::deal_workgroup(d, x1 - 1) != w) return -1;
+      if ((x1 - x0) % sile::kTileWaves && x1 != total) return -1;
+    }
+    at = x1;
+  }
+  return at == total ? used : -1;
+}
+int32_t workgroups(int64_t total, int32_t groups) { return sile::deal_workgroups(total, groups); }
 }
 """
 
@@ -38,14 +55,15 @@ int32_t chunk(int32_t total, int32_t groups) { return sile::deal_chunk(total, gr
 def plan(tmp_path_factory):
     d = tmp_path_factory.mktemp("plan")
     src = d / "plan.cpp"
-    src.write_text(SOURCE % os.path.join(ROOT, "sile_amd", "csrc", "kernels", "paged_plan.h"))
+    src.write_text(SOURCE.replace("PLAN_H", os.path.join(ROOT, "sile_amd", "csrc", "kernels", "paged_plan.h")))
     subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-shared", "-fPIC",
                     "-o", str(d / "plan.so"), str(src)], check=True)
     lib = ctypes.CDLL(str(d / "plan.so"))
     i32, i64 = ctypes.c_int32, ctypes.c_int64
     lib.span.argtypes = [i32, i64, i64, i64, ctypes.c_void_p]
     lib.cover.argtypes = [i32, i64, i64, i64, i32, ctypes.c_void_p]
-    lib.chunk.argtypes, lib.chunk.restype = [i32, i32], i32
+    lib.deal.argtypes, lib.deal.restype = [i32, i32], i32
+    lib.workgroups.argtypes, lib.workgroups.restype = [i64, i32], i32
     return lib
 
 
@@ -73,10 +91,18 @@ def test_lengths_are_held_to_the_table(plan):
 
 
 def test_shares_cover_the_tiles(plan):
-    for groups in (1, 256, 512):
-        for total in (0, 1, 3, 4, 5, 511, 512, 513, 2048, 2049, 99999, 2 ** 30):
-            c = plan.chunk(total, groups)
-            assert c % 4 == 0 and c >= 4 and c * groups >= total
+    """Every tile in one share, the shares in order; never more workgroups than a larger
+    list needs (the grid is sized for the largest)."""
+    r = np.random.default_rng(1)
+    for groups in (1, 3, 256, 512, 1024):
+        totals = [0, 1, 3, 4, 5, groups * 4, groups * 4 + 1, groups * 47, groups * 48 - 1, groups * 48, groups * 48 + 1,
+                  99999, 2 ** 30, 2 ** 31 - 2 ** 20] + [int(x) for x in r.integers(0, groups * 200, 50)]
+        most = 0
+        for total in sorted(totals):
+            used = plan.deal(total, groups)
+            assert 0 <= used <= plan.workgroups(total, groups) <= groups, (groups, total)
+            assert plan.workgroups(total, groups) >= most
+            most = plan.workgroups(total, groups)
 
 
 P = 4096   # an aligned address that nothing reads
