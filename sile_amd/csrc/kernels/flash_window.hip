@@ -6,7 +6,7 @@
 //
 // The matrix cores bound it: 4 D flop for each seen pair, and the keys of a window are
 // read again for every block of queries, out of the L2.  The pipeline is that of the
-// causal kernel (flash_attn.hip): a workgroup of 8 waves (4 past D = 128) takes 32 queries a wave;
+// causal kernel (flash_attn.hip): a workgroup of 4 waves, two of them a CU up to D = 128, takes 32 queries a wave;
 // K and V blocks go from memory to LDS by LDS-DMA, two stages of each; iteration j
 // issues S_{j+1} = K_{j+1} Q^T and O^T += V_{j-1}^T P_{j-1} on the matrix cores beside
 // the online softmax of S_j, whose accumulator holds one query a lane; V^T is read
@@ -17,14 +17,21 @@
 //    every query of the workgroup sees whole skip the mask.
 //  * A wave passes over an iteration whose three blocks none of its queries sees
 //    (at both ends of the window); its P is then zero.
+//  * The waves of a workgroup take up to four query heads of one key head (the K and V tiles
+//    are theirs alike) before further queries: 32 queries of four heads need 34 blocks of
+//    32 keys for a window of 1024, 128 queries of one 37.
 //  * Workgroups that read the same keys run together: an XCD takes a contiguous run of
-//    (batch x key head, query block, query head of that key head), so that a window's keys
+//    (batch x key head, query block, query heads of that key head), so that a window's keys
 //    are read from its L2 by all of them.
 //  * A row whose result is not finite (Inf or NaN in a masked key's V makes it so: 0 times
 //    it), or that sees no key, is taken again by one wave that reads its seen keys only.
 //
+// Two workgroups of 4 waves a CU and not one of 8: the first loads and the stores of one run beside
+// the other's products, and a block's window ends sooner (8192 queries, 32 heads of 128, window
+// 1024: 201 us with one, 172 with two; of 64: 150, 107).
+//
 // Key groups (kG = 2, 4): few query blocks leave CUs idle, so the blocks of the list can be
-// dealt to groups of the workgroup's waves, which join their (m, l, O) at the end.
+// dealt to groups of the waves of a workgroup of 8, which join their (m, l, O) at the end.
 //
 // The head dimension is rounded up to kDh (32, 64, 96, 128, 192 or 256): the chunks of a
 // row past D are loaded as zeros and its O^T rows past D are not stored.
@@ -77,8 +84,9 @@ SILE_DEV float pair_sum(uint32_t pk, float acc) {
 
 struct WindowArgs {
   int64_t q_len, kv_len, start, window, sinks;   // each below 2^31
-  int32_t items;        // batch * kv_heads * q_blocks * group
+  int32_t items;        // batch * kv_heads * q_blocks * group / heads
   int32_t q_blocks, group, d;
+  int32_t heads;        // query heads of one key head that a workgroup takes: 1, 2 or 4, a divisor of group
   float scale_log2;     // softmax scale * log2(e)
 };
 
@@ -179,14 +187,17 @@ __device__ __forceinline__ void window_fwd(const uint16_t* __restrict__ Q, const
   const int per_xcd = (a.items + 7) / 8;
   const int item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per_xcd || item >= a.items) return;
-  const int kvh = item / (a.q_blocks * a.group);
-  const int rest = item - kvh * (a.q_blocks * a.group);
-  const int qb = a.q_blocks - 1 - rest / a.group;   // the longest windows first
-  const int64_t head = (int64_t)kvh * a.group + rest % a.group;
+  const int head_sets = a.group / a.heads;
+  const int kvh = item / (a.q_blocks * head_sets);
+  const int rest = item - kvh * (a.q_blocks * head_sets);
+  const int qb = a.q_blocks - 1 - rest / head_sets;   // the longest windows first
+  // wave w: query head w % heads of the set, 32 queries w / heads of the block
+  const int64_t head = (int64_t)kvh * a.group + rest % head_sets * a.heads + wave % a.heads;
   const int64_t S = a.q_len;
   const int64_t q_off = head * S * d, kv_off = (int64_t)kvh * a.kv_len * d;
-  const int q0 = qb * kBQ;
-  const int wq0 = q0 + wave * 32;
+  const int bq = kBQ / a.heads;           // queries of the block
+  const int q0 = qb * bq;
+  const int wq0 = q0 + wave / a.heads * 32;
   auto kswz = [](int r) { return kChunks == 8 ? ((r >> 1) & 7) : (r & 15); };
   auto vswz = [](int r) { return (kChunks == 8 ? 2 : 4) * (r & 3); };
 
@@ -205,7 +216,7 @@ __device__ __forceinline__ void window_fwd(const uint16_t* __restrict__ Q, const
   // ---- the list of key blocks ----
   const int kv_last = (int)a.kv_len - 1;
   const int win = (int)a.window;
-  const int p0 = (int)(a.start + q0), p1 = (int)(a.start + min((int64_t)q0 + kBQ, S) - 1);
+  const int p0 = (int)(a.start + q0), p1 = (int)(a.start + min((int64_t)q0 + bq, S) - 1);
   const int lo0 = max(p0 - win + 1, 0);                // first key of the first query's window
   const int end = min(p1, kv_last);                    // last key of the last query
   const int blk0 = lo0 / kNK;
@@ -528,26 +539,26 @@ __device__ __forceinline__ void window_fwd(const uint16_t* __restrict__ Q, const
 
 }  // namespace
 
-#define SILE_FW_KERNEL(NAME, BF, W, NK, DH, DP, G)                                      \
-  extern "C" __global__ __launch_bounds__(W * 64, 1) void NAME(                         \
+#define SILE_FW_KERNEL(NAME, BF, W, EU, NK, DH, DP, G)                                  \
+  extern "C" __global__ __launch_bounds__(W * 64, EU) void NAME(                        \
       const uint16_t* Q, const uint16_t* K, const uint16_t* V, uint16_t* O, WindowArgs a) { \
     __shared__ __attribute__((aligned(1024))) uint8_t smem[lds_bytes<NK, DH, DP, W, G>()]; \
     window_fwd<BF, W, NK, DH, DP, G>(Q, K, V, O, a, smem);                              \
   }
 // d<D>: head dimensions up to D; g<N>: key groups
-#define SILE_FW_DTYPES(W, NK, DH, DP, G)                                              \
-  SILE_FW_KERNEL(sile_flash_window_f16_d##DH##_g##G, false, W, NK, DH, DP, G)         \
-  SILE_FW_KERNEL(sile_flash_window_bf16_d##DH##_g##G, true, W, NK, DH, DP, G)
+#define SILE_FW_DTYPES(W, EU, NK, DH, DP, G)                                          \
+  SILE_FW_KERNEL(sile_flash_window_f16_d##DH##_g##G, false, W, EU, NK, DH, DP, G)     \
+  SILE_FW_KERNEL(sile_flash_window_bf16_d##DH##_g##G, true, W, EU, NK, DH, DP, G)
 #define SILE_FW_GROUPS(NK, DH, DP) \
-  SILE_FW_DTYPES(8, NK, DH, DP, 1) \
-  SILE_FW_DTYPES(8, NK, DH, DP, 2) \
-  SILE_FW_DTYPES(8, NK, DH, DP, 4)
+  SILE_FW_DTYPES(4, 2, NK, DH, DP, 1) \
+  SILE_FW_DTYPES(8, 2, NK, DH, DP, 2) \
+  SILE_FW_DTYPES(8, 2, NK, DH, DP, 4)
 SILE_FW_GROUPS(64, 32, 64)
 SILE_FW_GROUPS(64, 64, 64)
 SILE_FW_GROUPS(32, 96, 128)
 SILE_FW_GROUPS(32, 128, 128)
-SILE_FW_DTYPES(4, 32, 192, 256, 1)
-SILE_FW_DTYPES(4, 32, 256, 256, 1)
+SILE_FW_DTYPES(4, 1, 32, 192, 256, 1)
+SILE_FW_DTYPES(4, 1, 32, 256, 256, 1)
 
 // Any head dimension up to 256, alignment and scale: a wave a query row.
 template <bool kBF16>

@@ -235,26 +235,44 @@ FlashPlan flash_plan(int64_t bh, int64_t seq, int head_dim, bool causal) {
   return best;
 }
 
-// Key groups of the windowed kernel: the count with the least modelled time, as in
-// flash_plan, for query blocks that all take the keys of their window (of the last
-// query's length at most), their own and the sinks.
-int window_groups(int64_t heads, int64_t q_len, int64_t last_len, int64_t window, int64_t sinks,
-                  int head_dim) {
-  int cus = 0, best = 1;
-  if (head_dim > 128 || device_cus(&cus) != SILE_OK) return 1;
+// How the windowed kernel's work is laid out: key groups (1: workgroups of 4 waves, two
+// a CU; 2 and 4: of 8 waves), waves that take queries, and the query heads of one key head among them.
+struct WindowPlan {
+  int groups, waves, q_waves, heads;
+};
+
+// The layout with the least modelled time.  A query block takes the keys of its window
+// (of the last query's length at most), its own and the sinks, in `iters` rounds of a key
+// block (32 keys; 64 up to head_dim 64) a group, each tau us, and 5 us of start and end.  tau
+// as in flash_plan for 8 waves; for 4 waves, 0.5 us alone on a CU to 0.85 beside another.
+// Measured, us a call with 1, 2, 4 groups: see the kernel's comment and the cases of its test.
+WindowPlan window_plan(int64_t batch_kv, int group, int64_t q_len, int64_t last_len, int64_t window,
+                       int64_t sinks, int head_dim) {
+  auto heads_of = [&](int q_waves) {
+    int h = 1;
+    while (2 * h <= std::min(q_waves, 4) && group % (2 * h) == 0) h *= 2;
+    return h;
+  };
+  WindowPlan best{1, 4, 4, heads_of(4)};
+  int cus = 0;
+  if (head_dim > 128 || device_cus(&cus) != SILE_OK) return best;
   const int64_t key_block = head_dim <= 64 ? 64 : 32;
   double best_t = 1e30;
   for (int g : {1, 2, 4}) {
-    const double lo = g == 1 ? 0.72 : g == 2 ? 0.82 : 0.95, hi = g == 1 ? 0.95 : g == 2 ? 1.1 : 1.35;
-    const int64_t bq = 256 / g, wgs = heads * ((q_len + bq - 1) / bq);
+    const int waves = g == 1 ? 4 : 8, q_waves = waves / g, heads = heads_of(q_waves);
+    const int64_t bq = 32 * q_waves / heads;
+    const int64_t wgs = batch_kv * (group / heads) * ((q_len + bq - 1) / bq);
     const int64_t keys = std::min(last_len, window + std::min(bq, q_len) + key_block) + std::min(sinks, last_len);
     const double iters = (double)(((keys + key_block * g - 1) / (key_block * g) + 1) / 2 * 2);
+    const int per_cu = g == 1 ? 2 : 1;
+    const double lo = g == 1 ? 0.5 : g == 2 ? 0.82 : 0.95, hi = g == 1 ? 0.85 : g == 2 ? 1.1 : 1.35;
+    const double busy = std::min(1.0, (double)wgs / (per_cu * cus));
     const double merge = g == 1 ? 0.0 : g == 2 ? 0.5 : 1.5;
-    const double tau = lo + (hi - lo) * std::min(1.0, (double)wgs / cus);
-    const double t = (double)((wgs + cus - 1) / cus) * (tau * iters + 5.0 + merge);
+    const double rounds = (double)((wgs + per_cu * cus - 1) / (per_cu * cus));
+    const double t = rounds * ((lo + (hi - lo) * busy) * iters + 5.0 + merge);
     if (t < best_t) {
       best_t = t;
-      best = g;
+      best = {g, waves, q_waves, heads};
     }
   }
   return best;
@@ -1280,10 +1298,10 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
   // a window past the last query's position sees what one that long does
   struct {
     int64_t q_len, kv_len, start, window, sinks;
-    int32_t items, q_blocks, group, d;
+    int32_t items, q_blocks, group, d, heads;
     float scale_log2;
   } wa{q_len, kv_len, q_start, std::min(window, last_len), std::min(sinks, kv_len), 0, 0,
-       (int32_t)(q_heads / kv_heads), (int32_t)head_dim, scale * 1.4426950408889634f};
+       (int32_t)(q_heads / kv_heads), (int32_t)head_dim, 1, scale * 1.4426950408889634f};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const char* dt = dtype == SILE_F16 ? "f16" : "bf16";
   char name[64];
@@ -1291,15 +1309,15 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
   if (head_dim % 8 == 0 && aligned16(q) && aligned16(k) && aligned16(v) && aligned16(o) && scale > 0.0f) {
     const int dh = head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : head_dim <= 96 ? 96 : head_dim <= 128 ? 128
                  : head_dim <= 192 ? 192 : 256;
-    const int groups = window_groups(batch * q_heads, q_len, last_len, wa.window, wa.sinks, dh);
-    const int waves = dh <= 128 ? 8 : 4;
-    const int64_t bq = 32 * waves / groups;
+    const WindowPlan plan = window_plan(batch * kv_heads, wa.group, q_len, last_len, wa.window, wa.sinks, dh);
+    const int64_t bq = 32 * plan.q_waves / plan.heads;
+    wa.heads = plan.heads;
     wa.q_blocks = (int32_t)((q_len + bq - 1) / bq);
-    wa.items = (int32_t)(batch * q_heads * wa.q_blocks);
-    snprintf(name, sizeof name, "sile_flash_window_%s_d%d_g%d", dt, dh, groups);
+    wa.items = (int32_t)(batch * kv_heads * (wa.group / plan.heads) * wa.q_blocks);
+    snprintf(name, sizeof name, "sile_flash_window_%s_d%d_g%d", dt, dh, plan.groups);
     void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa};
     const unsigned blocks = (unsigned)((wa.items + 7ll) / 8 * 8);
-    const int rc = launch(Module::kFlashWindow, name, dim3(blocks), dim3((unsigned)(64 * waves)), params, s);
+    const int rc = launch(Module::kFlashWindow, name, dim3(blocks), dim3((unsigned)(64 * plan.waves)), params, s);
     return rc == SILE_OK ? ok() : rc;
   }
   int64_t rows = batch * q_heads * q_len;
