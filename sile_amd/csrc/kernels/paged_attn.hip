@@ -29,7 +29,8 @@
 // workgroups and a batch of mixed lengths has no straggler, with the lengths
 // known only on the device.  A workgroup whose share covers a row's key head
 // whole writes its output; the others leave (O, m, l) in fp32 in the workspace, at
-// most two a workgroup, and a second launch joins them.
+// most two a workgroup, and a second launch joins them.  Where the host knows that
+// every row is short, a workgroup takes one unit instead, and there is nothing to join.
 //
 // An 8-bit cache (e4m3) is widened in registers, exactly: K into the operand, V on
 // its way into LDS; the scales go into the score's and the output's factor.
@@ -61,6 +62,7 @@ struct PagedArgs {
   float* part_o;        // workspace: [slots][rows][d]
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
   int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups;
+  int32_t direct;       // 1: a workgroup a unit, no list and no parts
   float scale_log2, v_scale;
 };
 
@@ -154,46 +156,66 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
   const int d = kExact ? kDp : a.d;
   const int chunks = d * kEs / 16;
 
-  // ---- deal ----
-  const int per = (a.batch + 255) / 256;
-  int32_t mine = 0;
-  for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r)
-    mine += unit_size(key_span(a.lengths[r], a.capacity, a.window, a.sinks));
-  int32_t incl = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int32_t up = __shfl_up(incl, off);
-    if (lane >= off) incl += up;
-  }
-  if (lane == 63) deal->wave_sum[wave] = incl;
-  __syncthreads();
-  int32_t before = incl - mine, rows_total = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) before += deal->wave_sum[w];
-    rows_total += deal->wave_sum[w];
-  }
-  const int32_t total = __builtin_amdgcn_readfirstlane(rows_total) * heads;
-  const Deal shares = make_deal(total, a.groups);
-  int32_t x = deal_start(shares, blockIdx.x);
-  const int32_t x1 = deal_start(shares, blockIdx.x + 1);
-  if (blockIdx.x == 0 || x < x1) {
-    int32_t at = before;
-    for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r) {
-      const int32_t t = unit_size(key_span(a.lengths[r], a.capacity, a.window, a.sinks));
-      if (blockIdx.x == 0) a.plan[r] = at;
-      if (x < x1 && x / heads >= at && x / heads < at + t) {
-        deal->row = r;
-        deal->before = at;
-      }
-      at += t;
+  int row;
+  int32_t x, x1, base;   // the list's tiles x .. x1 - 1 are this workgroup's; row `row` begins at base
+  if (a.direct) {
+    // ---- a unit a workgroup ----
+    row = blockIdx.x / heads;
+    const int unit = blockIdx.x - row * heads;
+    const int32_t size = unit_size(
+        key_span(__builtin_amdgcn_readfirstlane(a.lengths[row]), a.capacity, a.window, a.sinks));
+    base = 0;
+    x = unit * size;
+    x1 = x + size;
+    if (size == 0) {   // a row without keys
+      const int kvh = unit / a.head_groups, h0 = (unit - kvh * a.head_groups) * 16 * kQT;
+      const int n = min(16 * kQT, a.group - h0) * d;
+      uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)(kvh * a.group + h0) * d;
+      for (int c = tid; c < n; c += 256) o[c] = 0;
+      return;
     }
-    if (blockIdx.x == 0 && tid == 0) a.plan[a.batch] = rows_total;
+  } else {
+    // ---- deal ----
+    const int per = (a.batch + 255) / 256;
+    int32_t mine = 0;
+    for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r)
+      mine += unit_size(key_span(a.lengths[r], a.capacity, a.window, a.sinks));
+    int32_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int32_t up = __shfl_up(incl, off);
+      if (lane >= off) incl += up;
+    }
+    if (lane == 63) deal->wave_sum[wave] = incl;
+    __syncthreads();
+    int32_t before = incl - mine, rows_total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += deal->wave_sum[w];
+      rows_total += deal->wave_sum[w];
+    }
+    const int32_t total = __builtin_amdgcn_readfirstlane(rows_total) * heads;
+    const Deal shares = make_deal(total, a.groups);
+    x = deal_start(shares, blockIdx.x);
+    x1 = deal_start(shares, blockIdx.x + 1);
+    if (blockIdx.x == 0 || x < x1) {
+      int32_t at = before;
+      for (int r = tid * per; r < min((tid + 1) * per, a.batch); ++r) {
+        const int32_t t = unit_size(key_span(a.lengths[r], a.capacity, a.window, a.sinks));
+        if (blockIdx.x == 0) a.plan[r] = at;
+        if (x < x1 && x / heads >= at && x / heads < at + t) {
+          deal->row = r;
+          deal->before = at;
+        }
+        at += t;
+      }
+      if (blockIdx.x == 0 && tid == 0) a.plan[a.batch] = rows_total;
+    }
+    if (x >= x1) return;
+    __syncthreads();
+    row = __builtin_amdgcn_readfirstlane(deal->row);
+    base = __builtin_amdgcn_readfirstlane(deal->before) * heads;
   }
-  if (x >= x1) return;
-  __syncthreads();
-  int row = __builtin_amdgcn_readfirstlane(deal->row);
-  int32_t base = __builtin_amdgcn_readfirstlane(deal->before) * heads;
   uint8_t* const vt = smem + wave * Sh::kWaveB;
 
   while (x < x1) {

@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -25,7 +26,7 @@ struct AppendArgs {
   void *k_pages, *v_pages;
   int64_t tokens, ldk, ldv, page_stride, ld_table, capacity;
   int32_t heads, d, num_pages, page_shift, n_rows, per_group;
-  float k_scale, v_scale;
+  float k_scale, v_scale, k_rcp, v_rcp;
 };
 constexpr int kMaxPools = 128;
 constexpr int64_t kSegB = 16384;
@@ -49,9 +50,15 @@ struct PagedArgs {
   int32_t* plan;
   float *part_ml, *part_o;
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
-  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups;
+  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups, direct;
   float scale_log2, v_scale;
 };
+
+// 1 / scale, or 0 where the kernel is to divide
+float reciprocal(float scale) {
+  const float x = std::fabs(scale);
+  return x >= 0x1p-60f && x <= 0x1p60f ? 1.0f / scale : 0.0f;
+}
 
 // log2 of a power of two up to 65536, or -1
 int page_shift_of(int64_t page_size) {
@@ -212,7 +219,8 @@ int sile_hip_kv_append(sile_dtype dtype, sile_dtype cache_type, int64_t n_tokens
   const int64_t each = 2 * kv_heads * head_dim / (fp8 ? 16 : 8);   // chunks of a token
   AppendArgs a{k, v, rows, positions, tables, k_pages, v_pages, n_tokens, ldk, ldv, page_stride,
                ld_table, ld_table * page_size, (int32_t)kv_heads, (int32_t)head_dim, (int32_t)num_pages,
-               page_shift_of(page_size), (int32_t)n_rows, 1, k_scale, v_scale};
+               page_shift_of(page_size), (int32_t)n_rows, 1, k_scale, v_scale, reciprocal(k_scale),
+               reciprocal(v_scale)};
   // two chunks a thread where a token has few
   a.per_group = (int32_t)std::max<int64_t>(1, 512 / each);
   const int64_t blocks = (n_tokens + a.per_group - 1) / a.per_group;
@@ -472,12 +480,19 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   snprintf(name, sizeof name, "sile_paged_attn_%s%s_%c%d_q%d", dt, cache_type == dtype ? "" : "_fp8",
            page_size < 16 ? 's' : head_dim == plan.dp ? 'd' : 'p', plan.dp, plan.q_tiles);
   void* params[] = {&a};
-  const int32_t grid = sile::deal_workgroups(batch * row_tiles, a.groups);
+  const int64_t units = batch * kv_heads * plan.head_groups;
+  // A workgroup a unit, in one launch, where a unit is short (what the table's width or the
+  // window allows, as the lengths stand on the device): up to 512 keys in any case, up to 2048 where
+  // the units fill half the device.  Us a call, dealt and so, 8 key heads of 128: 1 x 256 keys 9.9,
+  // 7.3; 1 x 512 10.2, 9.1; 1 x 1024 10.7, 13.3; 32 x 1024 35, 27; 128 x 1024 99, 94; 32 x 2048 58,
+  // 49; 8 x 2048 21.3, 22.9; past that a single long row among short ones would keep its
+  // workgroups alone for long.
+  a.direct = (seen <= 512 || (seen <= 2048 && 2 * units >= plan.groups)) && units <= kIntMax;
+  const int32_t grid = a.direct ? (int32_t)units : sile::deal_workgroups(batch * row_tiles, a.groups);
   rc = launch(Module::kPagedAttn, name, dim3((unsigned)grid), dim3(256), params, s);
-  if (rc != SILE_OK) return rc;
+  if (rc != SILE_OK || a.direct) return rc == SILE_OK ? ok() : rc;
   // a unit has at most about grid / units parts (and one or two more): up to 16 for one wave,
   // two rounds of eight, then more waves
-  const int64_t units = batch * kv_heads * plan.head_groups;
   const int64_t heads = std::min<int64_t>(a.group, 16 * plan.q_tiles);
   const int64_t parts = grid / units + 2;
   int split = parts <= 16 ? 1 : parts <= 32 ? 2 : parts <= 64 ? 4 : 8;

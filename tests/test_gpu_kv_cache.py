@@ -254,6 +254,30 @@ def test_append(hip, dtype, fp8, tokens, hkv, d, page):
         assert (got == want).all(), (which, np.argwhere(got != want)[:5], got[got != want][:5], want[got != want][:5])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("scale", [1.0, 0.1, 1 / 3, 0.007, 2.0 ** -126, 1e-40, 3e38, -0.3, 1.9999999, 0.0])
+def test_append_e4m3_every_value(hip, dtype, scale):
+    """Every 16-bit value over a scale: the correctly rounded quotient's nearest code."""
+    say(f"kv append {dtype} every value / {scale}")
+    bits = np.arange(65536, dtype=np.uint16).reshape(64, 1024)
+    x = bits.view(np.float16).astype(np.float32) if dtype == "f16" else cpuref.f32_from_bf16(bits)
+    dx, dt = hip.DeviceBuffer.from_array(bits), ints(hip, [[0]])
+    dr_, dp = ints(hip, np.zeros(64)), ints(hip, np.arange(64))
+    pools = [hip.DeviceBuffer(65536) for _ in "kv"]
+    t = hip.F16 if dtype == "f16" else hip.BF16
+    hip.kv_append(t, hip.F8E4M3, 64, 4, 256, dx.ptr, 1024, dx.ptr, 1024, dr_.ptr, dp.ptr, pools[0].ptr, pools[1].ptr,
+                  1, 64, 65536, dt.ptr, 1, 1, scale, 1.0)
+    hip.synchronize()
+    for buf, s in zip(pools, (scale, 1.0)):
+        got = buf.download(np.uint8, (4, 64, 256)).transpose(1, 0, 2).reshape(64, 1024)
+        with np.errstate(all="ignore"):
+            y = np.clip(x / np.float32(s), -448, 448)   # (NaN stays)
+        want = cpuref.e4m3_encode(y, 1.0)
+        nan = np.isnan(y)
+        assert ((got & 0x7F)[nan] == 0x7F).all()
+        assert (got[~nan] == want[~nan]).all(), (s, x[~nan][got[~nan] != want[~nan]][:5])
+
+
 def test_serving_run(hip):
     """Steps of a serving program, captured where they repeat: prompts stored, a token a
     step, beams forked and dropped, pages made writable, the pool closed up; after each
