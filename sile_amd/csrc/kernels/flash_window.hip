@@ -188,16 +188,20 @@ __device__ __forceinline__ void window_fwd(const uint16_t* __restrict__ Q, const
   const int item = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per_xcd || item >= a.items) return;
   const int head_sets = a.group / a.heads;
-  const int kvh = item / (a.q_blocks * head_sets);
+  // (through readfirstlane: the divisions are vector instructions, and a buffer resource
+  // in vector registers costs a loop around its loads)
+  const int kvh = __builtin_amdgcn_readfirstlane(item / (a.q_blocks * head_sets));
   const int rest = item - kvh * (a.q_blocks * head_sets);
-  const int qb = a.q_blocks - 1 - rest / head_sets;   // the longest windows first
+  const int qb = a.q_blocks - 1 - __builtin_amdgcn_readfirstlane(rest / head_sets);   // the longest windows first
   // wave w: query head w % heads of the set, 32 queries w / heads of the block
-  const int64_t head = (int64_t)kvh * a.group + rest % head_sets * a.heads + wave % a.heads;
+  const int64_t head = (int64_t)kvh * a.group +
+                       __builtin_amdgcn_readfirstlane(rest % head_sets * a.heads + (wave & (a.heads - 1)));
   const int64_t S = a.q_len;
   const int64_t q_off = head * S * d, kv_off = (int64_t)kvh * a.kv_len * d;
-  const int bq = kBQ / a.heads;           // queries of the block
+  const int heads_log2 = __builtin_ctz(a.heads);
+  const int bq = kBQ >> heads_log2;       // queries of the block
   const int q0 = qb * bq;
-  const int wq0 = q0 + wave / a.heads * 32;
+  const int wq0 = q0 + (wave >> heads_log2) * 32;
   auto kswz = [](int r) { return kChunks == 8 ? ((r >> 1) & 7) : (r & 15); };
   auto vswz = [](int r) { return (kChunks == 8 ? 2 : 4) * (r & 3); };
 
