@@ -355,6 +355,27 @@ __device__ __forceinline__ void window_fwd(const uint16_t* __restrict__ Q, const
     s_block(0, sa);
     __syncthreads();
 
+    // The order of a region: fragment reads some steps ahead of the products that take
+    // them, and the softmax spread between the products.  Up to head_dim 96 (4096 queries x 64
+    // heads of 96, window 256: 66 -> 59 us); at 128, where it frees 40 registers, the compiler's own
+    // order is 3 % faster.
+    auto spread = [] {
+      constexpr int kMfmas = 2 * kKK * kST, kReads = 3 * kKK * kST, kAhead = 3;
+      constexpr int kValu = (48 * kST + kMfmas - 1) / kMfmas;
+      __builtin_amdgcn_sched_group_barrier(sched::kDsRead, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < kMfmas; ++i) {
+        __builtin_amdgcn_sched_group_barrier(sched::kMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(sched::kValu, kValu, 0);
+        if (kAhead + 3 * i / 2 < kReads) {
+          if (i & 1)
+            __builtin_amdgcn_sched_group_barrier(sched::kDsRead, 2, 0);
+          else
+            __builtin_amdgcn_sched_group_barrier(sched::kDsRead, 1, 0);
+        }
+      }
+    };
+
     auto softmax_block = [&](int j, auto masked, f32x16 (&s)[kST], u32x4 (&pnew)[kPN]) {
       constexpr bool kMasked = decltype(masked)::value;
       if constexpr (kMasked) {
@@ -394,6 +415,7 @@ __device__ __forceinline__ void window_fwd(const uint16_t* __restrict__ Q, const
         return rs;
       };
       float rs = probs(m_run * c - kLift<kBF16>);
+      if constexpr (kDh <= 96) spread();
       if (__builtin_amdgcn_ballot_w64(!(rs <= kBlockSumLimit<kBF16>)) != 0) {
 #pragma unroll
         for (int st = 0; st < kST; ++st) asm volatile("" : "+v"(s[st]));
