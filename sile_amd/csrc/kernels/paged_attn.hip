@@ -218,7 +218,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
   }
   uint8_t* const vt = smem + wave * Sh::kWaveB;
 
-  while (x < x1) {
+  while (x < x1 && row < a.batch) {
     const KeySpan span = key_span(__builtin_amdgcn_readfirstlane(a.lengths[row]), a.capacity, a.window, a.sinks);
     const int32_t size = unit_size(span);
     if (x >= base + size * heads) {   // on to the next row

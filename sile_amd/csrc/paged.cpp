@@ -87,7 +87,9 @@ int check_cache(sile_dtype dtype, sile_dtype cache_type, int64_t kv_heads, int64
   if (num_pages > 0 && (page_stride < kv_heads * page_size * head_dim || page_stride * *es % 16 != 0))
     return fail(SILE_ERR_SHAPE, "page_stride %lld: a page has %lld elements, in steps of 16 bytes",
                 (long long)page_stride, (long long)(kv_heads * page_size * head_dim));
-  if (page_stride > (1ll << 40)) return fail(SILE_ERR_SHAPE, "page_stride too large");
+  if (num_pages > 0 && page_stride > (1ll << 47) / num_pages)
+    return fail(SILE_ERR_SHAPE, "page_stride %lld too large for %lld pages", (long long)page_stride,
+                (long long)num_pages);
   return SILE_OK;
 }
 
@@ -110,15 +112,16 @@ int check_in_out(const int32_t* in, const int32_t* out, int64_t n, const char* w
   return SILE_OK;
 }
 
-int check_pools(void* const* pools, int64_t n_pools, int64_t page_bytes, int64_t page_stride, Pools* out) {
+int check_pools(void* const* pools, int64_t n_pools, int64_t page_bytes, int64_t page_stride,
+                int64_t num_pages, Pools* out) {
   memset(out, 0, sizeof *out);
   if (n_pools < 0 || n_pools > kMaxPools)
     return fail(SILE_ERR_SHAPE, "%lld pools (0 to %d)", (long long)n_pools, kMaxPools);
   if (n_pools == 0) return SILE_OK;
   if (!pools) return fail(SILE_ERR_SHAPE, "NULL pools");
   if (page_bytes <= 0 || page_bytes % 16 != 0 || page_stride % 16 != 0 || page_stride < page_bytes ||
-      page_bytes > (1ll << 40) || page_stride > (1ll << 44))
-    return fail(SILE_ERR_SHAPE, "pages of %lld bytes every %lld: multiples of 16, apart",
+      page_bytes > (1ll << 32) || page_stride > (1ll << 48) / std::max<int64_t>(num_pages, 1))
+    return fail(SILE_ERR_SHAPE, "pages of %lld bytes every %lld: multiples of 16, apart, at most 4 GiB each",
                 (long long)page_bytes, (long long)page_stride);
   for (int64_t i = 0; i < n_pools; ++i) {
     if (!pools[i]) return fail(SILE_ERR_SHAPE, "pool %lld is NULL", (long long)i);
@@ -235,11 +238,11 @@ int sile_hip_kv_append(sile_dtype dtype, sile_dtype cache_type, int64_t n_tokens
 int sile_hip_kv_copy_pages(void* const* pools, int64_t n_pools, int64_t page_bytes,
                            int64_t page_stride_bytes, int64_t num_pages, int64_t n,
                            const int32_t* src, const int32_t* dst, sile_hip_stream stream) {
-  Pools p;
-  int rc = check_pools(pools, n_pools, page_bytes, page_stride_bytes, &p);
-  if (rc != SILE_OK) return rc;
   if (n < 0 || num_pages < 0 || n > kIntMax || num_pages > kIntMax)
     return fail(SILE_ERR_SHAPE, "%lld copies in a pool of %lld pages", (long long)n, (long long)num_pages);
+  Pools p;
+  int rc = check_pools(pools, n_pools, page_bytes, page_stride_bytes, num_pages, &p);
+  if (rc != SILE_OK) return rc;
   if (n == 0 || n_pools == 0 || num_pages == 0) return ok();
   if (!src || !dst) return fail(SILE_ERR_SHAPE, "NULL operand");
   int64_t groups = 0;
@@ -324,7 +327,7 @@ int sile_hip_kv_reserve(int64_t n_rows, int64_t ld_table, int64_t page_size, con
     return fail(SILE_ERR_SHAPE, "page_size %lld is no power of two up to 65536", (long long)page_size);
   if (num_pages < 0 || num_pages > kIntMax) return fail(SILE_ERR_SHAPE, "invalid page count");
   Pools p;
-  if ((rc = check_pools(pools, n_pools, page_bytes, page_stride_bytes, &p)) != SILE_OK) return rc;
+  if ((rc = check_pools(pools, n_pools, page_bytes, page_stride_bytes, num_pages, &p)) != SILE_OK) return rc;
   if (num_pages > 0 && (!refs_in || !refs_out)) return fail(SILE_ERR_SHAPE, "NULL operand");
   if (n_rows > 0 && (!lengths || !need || !granted || (ld_table > 0 && (!tables_in || !tables_out))))
     return fail(SILE_ERR_SHAPE, "NULL operand");
@@ -372,7 +375,7 @@ int sile_hip_kv_compact(int64_t n_rows, int64_t ld_table, const int32_t* tables_
   if (rc != SILE_OK) return rc;
   if (num_pages < 0 || num_pages > kIntMax) return fail(SILE_ERR_SHAPE, "invalid page count");
   Pools p;
-  if ((rc = check_pools(pools, n_pools, page_bytes, page_stride_bytes, &p)) != SILE_OK) return rc;
+  if ((rc = check_pools(pools, n_pools, page_bytes, page_stride_bytes, num_pages, &p)) != SILE_OK) return rc;
   if (!used || (num_pages > 0 && (!refs_in || !refs_out)) ||
       (n_rows * ld_table > 0 && (!tables_in || !tables_out)))
     return fail(SILE_ERR_SHAPE, "NULL operand");

@@ -123,7 +123,7 @@ APPEND = [F16, F16, 3, 2, 64, P, 128, P, 128, None, P, P, P, 10, 16, 2048, P, 4,
     (5, None, 5, "NULL"), (5, P + 8, 5, "aligned"), (6, 120, 5, "leading dimension"), (6, 132, 5, "aligned"),
     (8, 127, 5, "leading dimension"), (10, None, 5, "NULL"), (11, P + 4, 5, "aligned"), (13, -1, 5, "cache shape"),
     (14, 24, 5, "power of two"), (14, 0, 5, "power of two"), (14, 131072, 5, "power of two"), (15, 2047, 5, "page_stride"),
-    (15, 2052, 5, "page_stride"), (17, -1, 5, "negative"), (18, -1, 5, "negative"), (17, 2 ** 31, 5, "too large"),
+    (15, 2052, 5, "page_stride"), (15, 2 ** 46, 5, "too large for"), (17, -1, 5, "negative"), (18, -1, 5, "negative"), (17, 2 ** 31, 5, "too large"),
     (18, 2 ** 30, 5, "too large")])
 def test_append_refusals(at, value, code, needle):
     args = list(APPEND)
@@ -171,6 +171,8 @@ TABLES = 1 << 20
     ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 129, 16, 16, 4, 1, P, P, None], 5, "pools"),
     ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 8, 16, 4, 1, P, P, None], 5, "multiples of 16"),
     ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 32, 16, 4, 1, P, P, None], 5, "multiples of 16"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 16, 1 << 40, 1 << 20, 1, P, P, None], 5, "4 GiB"),
+    ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 1 << 33, 1 << 33, 4, 1, P, P, None], 5, "4 GiB"),
     ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P + 8), 1, 16, 16, 4, 1, P, P, None], 5, "aligned"),
     ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 16, 16, 4, 1, None, P, None], 5, "NULL"),
     ("sile_hip_kv_copy_pages", [(ctypes.c_void_p * 1)(P), 1, 16, 16, 4, -1, P, P, None], 5, "copies"),
