@@ -9,7 +9,10 @@
 // first), and no page is read and written by one launch.
 //
 // All of it is bound by memory, or, at a serving step's few rows, by the launches:
-// each entry point is one to three of them, and a thread moves 16 bytes a load.
+// each entry point is one to three of them, and a thread moves 16 bytes a load.  Tokens and
+// pages are stored past the caches (non-temporal): 16000 tokens of 8 heads of 128 into a 16-bit
+// cache take 33 us with plain stores and 24 so (5.5 TB/s), closing up a pool of 4700 pages
+// 39 and 31; loads that way are slower (24 us, 32).
 #include "common.h"
 
 using namespace sile;
@@ -37,7 +40,7 @@ struct AppendArgs {
 // correctly rounded: one correction of x * rcp by its remainder is then the quotient
 // (Markstein), wherever it is neither past the range, where it saturates in any case,
 // nor so small that it rounds to zero, and scale is no extreme; else (rcp = 0) the division
-// (a third of the kernel's instructions: 16382 tokens of 8 heads of 128 take 24 us with it, 22 so).
+// (a third of the kernel's instructions: 16382 tokens of 8 heads of 128 take 31 us with it, 26 so, before the stores' change).
 SILE_DEV float e4m3_in(float x, float scale, float rcp) {
   float y;
   if (rcp == 0.0f) {
@@ -77,7 +80,7 @@ SILE_DEV void append(const AppendArgs& a) {
     u32x4_t out;
     if constexpr (kIn == 0) {
       out = *reinterpret_cast<const u32x4_t*>(src);
-      *reinterpret_cast<u32x4_t*>((is_v ? a.v_pages : a.k_pages) + 2 * at) = out;
+      __builtin_nontemporal_store(out, reinterpret_cast<u32x4_t*>((is_v ? a.v_pages : a.k_pages) + 2 * at));
     } else {
       const float scale = is_v ? a.v_scale : a.k_scale, rcp = is_v ? a.v_rcp : a.k_rcp;
 #pragma unroll
@@ -96,7 +99,7 @@ SILE_DEV void append(const AppendArgs& a) {
           out[2 * h + j] = (uint32_t)code;
         }
       }
-      *reinterpret_cast<u32x4_t*>((is_v ? a.v_pages : a.k_pages) + at) = out;
+      __builtin_nontemporal_store(out, reinterpret_cast<u32x4_t*>((is_v ? a.v_pages : a.k_pages) + at));
     }
   }
 }
@@ -124,7 +127,8 @@ SILE_DEV void copy_segment(const Pools& p, int pool, int seg, int32_t src, int32
     if (at + 4096 * i < p.page_bytes) w[i] = *reinterpret_cast<const u32x4_t*>(from + at + 4096 * i);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (at + 4096 * i < p.page_bytes) *reinterpret_cast<u32x4_t*>(to + at + 4096 * i) = w[i];
+    if (at + 4096 * i < p.page_bytes)
+      __builtin_nontemporal_store(w[i], reinterpret_cast<u32x4_t*>(to + at + 4096 * i));
 }
 
 // pairs (src[i], dst[i]), i < n, workgroup `first` of `groups`
