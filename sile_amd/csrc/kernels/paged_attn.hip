@@ -44,6 +44,10 @@ typedef unsigned int u32x2v __attribute__((ext_vector_type(2)));
 namespace {
 
 constexpr float kLowest = -3.402823466e38f;
+// V's rows are loaded whole by one instruction and non-temporal; K's by several, of 64 bytes a
+// row each, which the caches have to bring together (32 rows up to 8192 keys of 128: 107 us,
+// V so 97, K too 94; but 128 rows up to 1000: 30, 26, 30, and 32 rows up to 2000 of 256: 65, 58, 77).
+constexpr int kNonTemporal = 2;
 // The probabilities of a row carry a factor 2^kLift, its maximum's being exactly
 // that: f16 has no exponent below 2^-24, and a long row has many keys far below
 // its maximum.  l and O carry it too, so it drops out of O / l.
@@ -318,7 +322,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
             const int c = lane % kCh;
             const int off = kExact || c < chunks ? (kVRows * i + lane / kCh) * row_b + 16 * c : 0x7fff0000;
             vr[s * (kVL / 2) + i] =
-                __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vb, off, 0, 0));
+                __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vb, off, 0, kNonTemporal));
           }
         }
         return seen;
@@ -353,7 +357,8 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
         for (int i = 0; i < kVL; ++i) {
           const int c = lane % kCh;   // a chunk past the dims reads chunk 0 (its O^T rows are not kept)
           const uint8_t* p = a.v + row_off(kVRows * i + lane / kCh);
-          vr[i] = *reinterpret_cast<const u32x4*>(p + 16 * (kExact || c < chunks ? c : 0));
+          vr[i] = __builtin_nontemporal_load(
+              reinterpret_cast<const u32x4*>(p + 16 * (kExact || c < chunks ? c : 0)));
         }
         return seen;
       }
