@@ -485,12 +485,13 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   void* params[] = {&a};
   const int64_t units = batch * kv_heads * plan.head_groups;
   // A workgroup a unit, in one launch, where a unit is short (what the table's width or the
-  // window allows, as the lengths stand on the device): up to 512 keys in any case, up to 2048 where
-  // the units fill half the device.  Us a call, dealt and so, 8 key heads of 128: 1 x 256 keys 9.9,
-  // 7.3; 1 x 512 10.2, 9.1; 1 x 1024 10.7, 13.3; 32 x 1024 35, 27; 128 x 1024 99, 94; 32 x 2048 58,
-  // 49; 8 x 2048 21.3, 22.9; past that a single long row among short ones would keep its
-  // workgroups alone for long.
-  a.direct = (seen <= 512 || (seen <= 2048 && 2 * units >= plan.groups)) && units <= kIntMax;
+  // window allows, as the lengths stand on the device): up to 512 keys in any case, up to 2048
+  // (1024 of 256 16-bit dims) where there is a unit for every CU.  Us a call, dealt and so, 8
+  // key heads of 128: 1 x 256 keys 9.9, 7.3; 1 x 512 10.2, 9.1; 1 x 1024 10.7, 13.3; 32 x 1024
+  // 35, 27; 128 x 1024 99, 94; 32 x 2048 58, 49; 8 x 2048 21.3, 22.9; 4 of 256, 64 x 2000 56,
+  // 71.  Past that a single long row among short ones would keep its workgroups alone for long.
+  a.direct = (seen <= 512 || (seen <= 2048 && seen * head_dim * es <= (1 << 19) && units >= plan.cus)) &&
+             units <= kIntMax;
   const int32_t grid = a.direct ? (int32_t)units : sile::deal_workgroups(batch * row_tiles, a.groups);
   rc = launch(Module::kPagedAttn, name, dim3((unsigned)grid), dim3(256), params, s);
   if (rc != SILE_OK || a.direct) return rc == SILE_OK ? ok() : rc;
