@@ -369,6 +369,73 @@ def test_serving_run(hip):
     st.close()
 
 
+@pytest.mark.parametrize("window,sinks", [(1000, 0), (50, 3)])
+def test_prompt_then_tokens(hip, window, sinks):
+    """A prompt's attention, its tokens stored, then token by token over the cache: one
+    sequence's attention, row for row, in one graph per step."""
+    say(f"kv prompt then tokens window={window}")
+    r = rng(9)
+    n, steps, hq, hkv, d, page, width = 90, 12, 4, 2, 64, 16, 8
+    total, stride = n + steps, hkv * page * d
+    qb, q = f16_round(r.normal(size=(total, hq, d)))
+    kb, k = f16_round(r.normal(size=(total, hkv, d)))
+    vb, v = f16_round(r.normal(size=(total, hkv, d)))
+    st = hip.Stream()
+    up = hip.DeviceBuffer.from_array
+    heads = lambda x: up(np.ascontiguousarray(x[:n].transpose(1, 0, 2)))  # noqa: E731
+    hq_, hk, hv, ho = heads(qb), heads(kb), heads(vb), hip.DeviceBuffer(n * hq * d * 2)
+    hip.flash_attn_window_fwd(hip.F16, 1, hq, hkv, n, n, d, hq_.ptr, hk.ptr, hv.ptr, ho.ptr, d ** -0.5, 0, window, sinks, st)
+    dq, dk, dv = up(qb), up(kb), up(vb)
+    pk, pv = (up(np.full((width, stride), 0x7E00, np.uint16)) for _ in "kv")
+    table, refs = ints(hip, np.full((1, width), -1)), ints(hip, np.zeros(width))
+    length, need, pos, granted = ints(hip, [0]), ints(hip, [n]), ints(hip, np.arange(n)), ints(hip, [0])
+    rows = ints(hip, np.zeros(n))
+    ws, wa = hip.DeviceBuffer(hip.kv_workspace(1, width)), hip.DeviceBuffer(hip.paged_attn_workspace(1, hq, hkv, d))
+    out = hip.DeviceBuffer(hq * d * 2)
+    pools = ([pk.ptr, pv.ptr], 2 * stride, 2 * stride)
+
+    def reserve():
+        hip.kv_reserve(1, width, page, length.ptr, need.ptr, table.ptr, table.ptr, width, refs.ptr, refs.ptr, granted.ptr,
+                       *pools, ws.ptr, ws.nbytes, st)
+
+    reserve()
+    hip.kv_append(hip.F16, hip.F16, n, hkv, d, dk.ptr, hkv * d, dv.ptr, hkv * d, rows.ptr, pos.ptr, pk.ptr, pv.ptr, width,
+                  page, stride, table.ptr, 1, width, stream=st)
+    st.synchronize()
+    got = [x for x in ho.download(np.float16, (hq, n, d)).transpose(1, 0, 2)]
+    # a step: the newest token at fixed places, so that one graph serves all steps
+    tq, tk, tv = (hip.DeviceBuffer(x.nbytes // total) for x in (qb, kb, vb))
+    need.upload(np.array([1], np.int32))
+    before = ints(hip, [0])
+    with hip.Graph(st) as graph:
+        hip.kv_reserve(1, width, page, before.ptr, need.ptr, table.ptr, table.ptr, width, refs.ptr, refs.ptr, granted.ptr,
+                       *pools, ws.ptr, ws.nbytes, st)
+        hip.kv_append(hip.F16, hip.F16, 1, hkv, d, tk.ptr, hkv * d, tv.ptr, hkv * d, None, before.ptr, pk.ptr, pv.ptr, width,
+                      page, stride, table.ptr, 1, width, stream=st)
+        hip.paged_attn_decode(hip.F16, hip.F16, 1, hq, hkv, d, tq.ptr, hq * d, pk.ptr, pv.ptr, width, page, stride,
+                              table.ptr, width, length.ptr, out.ptr, hq * d, d ** -0.5, window=window, sinks=sinks,
+                              workspace=wa.ptr, workspace_bytes=wa.nbytes, stream=st)
+    for i in range(n, total):
+        for buf, x in ((tq, qb), (tk, kb), (tv, vb)):
+            buf.upload(x[i])
+        before.upload(np.array([i], np.int32))
+        length.upload(np.array([i + 1], np.int32))
+        hip.synchronize()
+        graph.launch()
+        st.synchronize()
+        assert down(granted, 1)[0] == 1
+        got.append(out.download(np.float16, (hq, d)))
+    for i in range(total):
+        at = paged_ref.seen_keys(i + 1, window, sinks)
+        for h in range(hq):
+            ref, spread, size = paged_ref.attention(q[i, h], k[at, h // 2], v[at, h // 2], d ** -0.5)
+            p_error = 2.0 ** -11 if i < n else 2.0 ** -21
+            bound = paged_ref.error_bound(ref, spread, size, "f16", d, len(at), p_error)
+            assert (np.abs(got[i][h].astype(np.float64) - ref) <= bound).all(), (i, h)
+    graph.close()
+    st.close()
+
+
 def test_graph_of_a_step(hip):
     """free, fork, reserve and compact captured once: each replay on its own state gives
     what the eager calls give, with eager work in between."""

@@ -156,6 +156,31 @@ def test_window_and_sinks(hip, window, sinks, page):
              f"paged attn window={window} sinks={sinks} page={page}")
 
 
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (16, 1), (17, 1), (33, 1), (40, 2)])
+@pytest.mark.parametrize("d,page,fp8", [(64, 16, False), (64, 4, True), (80, 64, False), (128, 32, True), (128, 8, False),
+                                        (104, 2, False), (256, 16, False), (176, 128, True)])
+def test_rows_split_over_workgroups(hip, hq, hkv, d, page, fp8):
+    """Every instance with rows long enough to be dealt out and joined: each page size's
+    addressing, one and two query tiles, head groups past them."""
+    run_case(hip, Case(20, "bf16", [1500, 0, 3, 700, 129], hq, hkv, d, page, fp8=fp8),
+             f"paged attn split {hq}/{hkv} d={d} page={page} fp8={fp8}")
+
+
+@pytest.mark.parametrize("window,sinks", [(600, 0), (600, 70), (1000, 1), (513, 2000), (2000, 33)])
+def test_windows_dealt_out(hip, window, sinks):
+    run_case(hip, Case(21, "f16", [0, 5, 599, 600, 601, 700, 1500, 4000], 6, 2, 72, 16, window, sinks),
+             f"paged attn dealt window={window} sinks={sinks}")
+
+
+@pytest.mark.parametrize("batch", [1, 64, 200, 257, 520])
+def test_short_rows_a_workgroup_each(hip, batch):
+    """A table of 512 keys at most (a workgroup a unit), and one past it."""
+    lengths = [int(n) for n in rng(22).integers(0, 300, batch)]
+    run_case(hip, Case(22, "f16", lengths, 2, 1, 64, 32), f"paged attn {batch} short rows")
+    lengths[batch // 2] = 1100
+    run_case(hip, Case(23, "f16", lengths, 2, 1, 64, 32), f"paged attn {batch} rows, one of 1100")
+
+
 def test_many_rows_and_one_long_one(hip):
     """More rows than a workgroup has threads, most of them short or empty."""
     lengths = [int(n) for n in rng(6).integers(0, 40, 700)]
