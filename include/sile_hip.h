@@ -478,6 +478,7 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
  *   refs     int32 [num_pages] table entries that hold the page; <= 0: free
  * Page numbers, lengths and positions are looked at on the device only: one
  * outside its range names nothing, and nothing is read or written for it.
+ * At most 2^22 rows; the entries of a table and the pages each below 2^31.
  * All calls only enqueue, on the current device, and can be captured into a
  * graph (they are plain kernel launches); the same workspace serves calls
  * that run one after another, never two that may run side by side. */
@@ -515,8 +516,8 @@ int sile_hip_kv_free(int64_t n_rows, int64_t ld_table, const int32_t *drop,
 
 /* Forks rows: row i < n_out of the new table and lengths is row src[i] of the old ones
  * (n_in rows), empty where src[i] is outside [0, n_in).  The pages are shared, not copied:
- * a page's count changes by how many rows took its row, less one, so a row that none
- * took is freed and a row that two took is forked (beam search's reordering is one call).
+ * a page's count changes by how many rows took its row, less one, so that a row that none
+ * took is freed and one that two took is forked (beam search's reordering is one call).
  * Old and new tables and lengths must not overlap; the counts may be one array. */
 int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_t *src,
                      const int32_t *tables_in, int32_t *tables_out, const int32_t *lengths_in,
@@ -553,7 +554,8 @@ int sile_hip_kv_compact(int64_t n_rows, int64_t ld_table, const int32_t *tables_
                         int64_t page_bytes, int64_t page_stride_bytes, void *workspace,
                         size_t workspace_bytes, sile_hip_stream stream);
 
-/* Workspace bytes that sile_hip_paged_attn_decode needs (for any lengths). */
+/* Workspace bytes that sile_hip_paged_attn_decode needs on the current device (for any
+ * lengths). */
 int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                   int64_t head_dim, size_t *bytes);
 

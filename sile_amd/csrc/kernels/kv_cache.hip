@@ -148,16 +148,6 @@ SILE_DEV void copy_ints(const int32_t* from, int32_t* to, int64_t n, int64_t fir
   for (int64_t i = first * 256 + threadIdx.x; i < n; i += groups * 256) to[i] = from[i];
 }
 
-SILE_DEV int block_sum(int v, int* lds) {   // 256 threads
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = lds[0] + lds[1] + lds[2] + lds[3];
-  __syncthreads();
-  return v;
-}
-
 // exclusive sum over 1024 threads; *all: the whole sum
 SILE_DEV int scan_1024(int v, int* lds, int* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -240,30 +230,28 @@ extern "C" __global__ __launch_bounds__(256) void sile_kv_free(
 }
 
 // Row i of the new table is row src[i] of the old one (empty where src[i] names
-// none): workgroups 0 .. n_out - 1; a page's count changes by how often its old
-// row was taken, less one: a workgroup an old row behind them.
+// none), and each of its pages counts once more: workgroups 0 .. n_out - 1.  Each page of
+// an old row counts once less: a workgroup an old row behind them.
 extern "C" __global__ __launch_bounds__(256) void sile_kv_fork(
     int32_t n_in, int32_t n_out, int64_t ld_table, const int32_t* src, const int32_t* tables_in,
     int32_t* tables_out, const int32_t* lengths_in, int32_t* lengths_out, int32_t num_pages,
     int32_t* refs_out) {
-  __shared__ int lds[4];
   if ((int64_t)blockIdx.x < n_out) {
     const int64_t i = blockIdx.x;
     const int32_t s = src[i];
     const bool in = s >= 0 && s < n_in;
-    for (int64_t e = threadIdx.x; e < ld_table; e += 256)
-      tables_out[i * ld_table + e] = in ? tables_in[s * ld_table + e] : -1;
+    for (int64_t e = threadIdx.x; e < ld_table; e += 256) {
+      const int32_t id = in ? tables_in[s * ld_table + e] : -1;
+      if ((uint32_t)id < (uint32_t)num_pages) atomicAdd(&refs_out[id], 1);
+      tables_out[i * ld_table + e] = id;
+    }
     if (threadIdx.x == 0) lengths_out[i] = in ? lengths_in[s] : 0;
     return;
   }
   const int64_t row = (int64_t)blockIdx.x - n_out;
-  int n = 0;
-  for (int32_t i = threadIdx.x; i < n_out; i += 256) n += src[i] == row;
-  n = block_sum(n, lds);
-  if (n == 1) return;
   for (int64_t e = threadIdx.x; e < ld_table; e += 256) {
     const int32_t id = tables_in[row * ld_table + e];
-    if ((uint32_t)id < (uint32_t)num_pages) atomicAdd(&refs_out[id], n - 1);
+    if ((uint32_t)id < (uint32_t)num_pages) atomicSub(&refs_out[id], 1);
   }
 }
 

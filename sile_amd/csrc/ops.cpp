@@ -1314,6 +1314,8 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
     wa.heads = plan.heads;
     wa.q_blocks = (int32_t)((q_len + bq - 1) / bq);
     wa.items = (int32_t)(batch * kv_heads * (wa.group / plan.heads) * wa.q_blocks);
+    // (a launch has less than 2^32 threads)
+    if (wa.items > (1 << 22)) return fail(SILE_ERR_SHAPE, "attention too large (%d blocks)", wa.items);
     snprintf(name, sizeof name, "sile_flash_window_%s_d%d_g%d", dt, dh, plan.groups);
     void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa};
     const unsigned blocks = (unsigned)((wa.items + 7ll) / 8 * 8);
@@ -1321,6 +1323,7 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
     return rc == SILE_OK ? ok() : rc;
   }
   int64_t rows = batch * q_heads * q_len;
+  if (rows > (1 << 24)) return fail(SILE_ERR_SHAPE, "attention too large (%lld rows)", (long long)rows);
   snprintf(name, sizeof name, "sile_flash_window_rowwise_%s", dt);
   void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa, &rows};
   const int rc = launch(Module::kFlashWindow, name, dim3((unsigned)((rows + 3) / 4)), dim3(256), params, s);

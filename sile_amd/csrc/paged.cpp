@@ -18,6 +18,8 @@ using namespace sile_rt;
 namespace {
 
 constexpr int64_t kIntMax = 0x7fffffff;
+// rows of a table, and units of an attention call: a launch has less than 2^32 threads
+constexpr int64_t kMaxRows = 1 << 22;
 
 // Kernel argument blocks; layouts match the structs in kernels/*.hip.
 struct AppendArgs {
@@ -83,7 +85,7 @@ int check_cache(sile_dtype dtype, sile_dtype cache_type, int64_t kv_heads, int64
                 dtype_name(cache_type), (long long)head_dim, (long long)(16 / *es));
   if (page_shift_of(page_size) < 0)
     return fail(SILE_ERR_SHAPE, "page_size %lld is no power of two up to 65536", (long long)page_size);
-  if (kv_heads > (1 << 16) || num_pages > kIntMax) return fail(SILE_ERR_SHAPE, "cache too large");
+  if (kv_heads > (1 << 15) || num_pages > kIntMax) return fail(SILE_ERR_SHAPE, "cache too large");
   if (num_pages > 0 && (page_stride < kv_heads * page_size * head_dim || page_stride * *es % 16 != 0))
     return fail(SILE_ERR_SHAPE, "page_stride %lld: a page has %lld elements, in steps of 16 bytes",
                 (long long)page_stride, (long long)(kv_heads * page_size * head_dim));
@@ -95,7 +97,7 @@ int check_cache(sile_dtype dtype, sile_dtype cache_type, int64_t kv_heads, int64
 
 int check_table(int64_t rows, int64_t ld_table) {
   if (rows < 0 || ld_table < 0) return fail(SILE_ERR_SHAPE, "negative table extent");
-  if (rows > kIntMax || (rows > 0 && ld_table > kIntMax / rows))
+  if (rows > kMaxRows || (rows > 0 && ld_table > kIntMax / rows))
     return fail(SILE_ERR_SHAPE, "page table of %lld x %lld entries too large", (long long)rows,
                 (long long)ld_table);
   return SILE_OK;
@@ -211,7 +213,8 @@ int sile_hip_kv_append(sile_dtype dtype, sile_dtype cache_type, int64_t n_tokens
   int rc = check_cache(dtype, cache_type, kv_heads, head_dim, num_pages, page_size, page_stride, &es);
   if (rc != SILE_OK) return rc;
   if ((rc = check_table(n_rows, ld_table)) != SILE_OK) return rc;
-  if (n_tokens < 0) return fail(SILE_ERR_SHAPE, "negative token count");
+  if (n_tokens < 0 || n_tokens > kIntMax)
+    return fail(SILE_ERR_SHAPE, "%lld tokens: negative or too many", (long long)n_tokens);
   if (n_tokens == 0 || n_rows == 0 || ld_table == 0 || num_pages == 0) return ok();
   if (!k || !v || !positions || !k_pages || !v_pages || !tables) return fail(SILE_ERR_SHAPE, "NULL operand");
   if (ldk < kv_heads * head_dim || ldv < kv_heads * head_dim)
@@ -224,10 +227,9 @@ int sile_hip_kv_append(sile_dtype dtype, sile_dtype cache_type, int64_t n_tokens
                ld_table, ld_table * page_size, (int32_t)kv_heads, (int32_t)head_dim, (int32_t)num_pages,
                page_shift_of(page_size), (int32_t)n_rows, 1, k_scale, v_scale, reciprocal(k_scale),
                reciprocal(v_scale)};
-  // two chunks a thread where a token has few
-  a.per_group = (int32_t)std::max<int64_t>(1, 512 / each);
+  // two chunks a thread where a token has few; at most 2^22 workgroups
+  a.per_group = (int32_t)std::max<int64_t>({1, 512 / each, (n_tokens >> 22) + 1});
   const int64_t blocks = (n_tokens + a.per_group - 1) / a.per_group;
-  if (blocks > kIntMax) return fail(SILE_ERR_SHAPE, "too many tokens");
   void* params[] = {&a};
   rc = launch(Module::kKvCache, !fp8 ? "sile_kv_append" : dtype == SILE_F16 ? "sile_kv_append_f16_fp8"
                                                                             : "sile_kv_append_bf16_fp8",
@@ -297,7 +299,6 @@ int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = copy_ints(refs_in, refs_out, num_pages, s)) != SILE_OK) return rc;
   if (n_in + n_out == 0) return ok();
-  if (n_in + n_out > kIntMax) return fail(SILE_ERR_SHAPE, "too many rows");
   int32_t in = (int32_t)n_in, out = (int32_t)n_out, pages = (int32_t)num_pages;
   void* params[] = {&in, &out, &ld_table, (void*)&src, (void*)&tables_in, &tables_out,
                     (void*)&lengths_in, &lengths_out, &pages, &refs_out};
@@ -308,7 +309,7 @@ int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_
 int sile_hip_kv_workspace(int64_t n_rows, int64_t num_pages, size_t* bytes) {
   if (!bytes) return fail(SILE_ERR_SHAPE, "bytes is NULL");
   *bytes = 0;
-  if (n_rows < 0 || num_pages < 0 || n_rows > kIntMax || num_pages > kIntMax)
+  if (n_rows < 0 || num_pages < 0 || n_rows > kMaxRows || num_pages > kIntMax)
     return fail(SILE_ERR_SHAPE, "%lld rows over %lld pages", (long long)n_rows, (long long)num_pages);
   *bytes = (size_t)(4 * kv_ints(n_rows, num_pages));
   return ok();
@@ -447,7 +448,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
                                                                     std::min<int64_t>(sinks, kIntMax))
                                   : capacity;
   const int64_t row_tiles = (seen / sile::kTileKeys + 3 + sile::kUnitTiles) * kv_heads * plan.head_groups;
-  if (batch > (kIntMax - (1 << 20)) / row_tiles)
+  if (batch > (kIntMax - (1 << 20)) / row_tiles || batch * kv_heads * plan.head_groups > kMaxRows)
     return fail(SILE_ERR_SHAPE, "%lld rows of up to %lld keys: too many for one call", (long long)batch,
                 (long long)seen);
   PagedArgs a{};
@@ -490,8 +491,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   // key heads of 128: 1 x 256 keys 9.9, 7.3; 1 x 512 10.2, 9.1; 1 x 1024 10.7, 13.3; 32 x 1024
   // 35, 27; 128 x 1024 99, 94; 32 x 2048 58, 49; 8 x 2048 21.3, 22.9; 4 of 256, 64 x 2000 56,
   // 71.  Past that a single long row among short ones would keep its workgroups alone for long.
-  a.direct = (seen <= 512 || (seen <= 2048 && seen * head_dim * es <= (1 << 19) && units >= plan.cus)) &&
-             units <= kIntMax;
+  a.direct = (seen <= 512 || (seen <= 2048 && seen * head_dim * es <= (1 << 19) && units >= plan.cus));
   const int32_t grid = a.direct ? (int32_t)units : sile::deal_workgroups(batch * row_tiles, a.groups);
   rc = launch(Module::kPagedAttn, name, dim3((unsigned)grid), dim3(256), params, s);
   if (rc != SILE_OK || a.direct) return rc == SILE_OK ? ok() : rc;

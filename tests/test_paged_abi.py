@@ -119,7 +119,7 @@ APPEND = [F16, F16, 3, 2, 64, P, 128, P, 128, None, P, P, P, 10, 16, 2048, P, 4,
 
 @pytest.mark.parametrize("at,value,code,needle", [
     (0, F32, 2, "tokens of f32"), (1, BF16, 2, "under f16"), (1, F32, 2, "under f16"), (2, -1, 5, "negative"),
-    (3, 0, 5, "cache shape"), (4, 0, 5, "cache shape"), (4, 264, 2, "head_dim > 256"), (4, 60, 2, "no multiple"),
+    (2, 2 ** 31, 5, "too many"), (3, 2 ** 15 + 1, 5, "too large"), (3, 0, 5, "cache shape"), (4, 0, 5, "cache shape"), (4, 264, 2, "head_dim > 256"), (4, 60, 2, "no multiple"),
     (5, None, 5, "NULL"), (5, P + 8, 5, "aligned"), (6, 120, 5, "leading dimension"), (6, 132, 5, "aligned"),
     (8, 127, 5, "leading dimension"), (10, None, 5, "NULL"), (11, P + 4, 5, "aligned"), (13, -1, 5, "cache shape"),
     (14, 24, 5, "power of two"), (14, 0, 5, "power of two"), (14, 131072, 5, "power of two"), (15, 2047, 5, "page_stride"),
@@ -182,6 +182,8 @@ TABLES = 1 << 20
     ("sile_hip_kv_free", [4, 4, None, P, P, P, P, 9, P, P, None], 5, "NULL"),
     ("sile_hip_kv_fork", [4, 4, 4, P, P, P, TABLES, 2 * TABLES, 9, P, P, None], 5, "must not overlap"),
     ("sile_hip_kv_fork", [4, 4, 4, P, TABLES, 2 * TABLES, P, P, 9, P, P, None], 5, "must not overlap"),
+    ("sile_hip_kv_fork", [4, 2 ** 22 + 1, 1, P, TABLES, 2 * TABLES, P, P, 9, P, P, None], 5, "too large"),
+    ("sile_hip_kv_workspace", [2 ** 22 + 1, 4, ctypes.byref(ctypes.c_size_t())], 5, "rows"),
     ("sile_hip_kv_fork", [-1, 4, 4, P, TABLES, 2 * TABLES, P, P, 9, P, P, None], 5, "negative"),
     ("sile_hip_kv_reserve", [4, 4, 3, P, P, P, P, 9, P, P, P, None, 0, 0, 0, P, 1 << 20, None], 5, "power of two"),
     ("sile_hip_kv_reserve", [4, 4, 16, P, P, P, P, 9, P, P, P, None, 0, 0, 0, None, 0, None], 5, "workspace"),
