@@ -245,7 +245,9 @@ struct WindowPlan {
 // (of the last query's length at most), its own and the sinks, in `iters` rounds of a key
 // block (32 keys; 64 up to head_dim 64) a group, each tau us, and 5 us of start and end.  tau
 // as in flash_plan for 8 waves; for 4 waves, 0.5 us alone on a CU to 0.85 beside another.
-// Measured, us a call with 1, 2, 4 groups: see the kernel's comment and the cases of its test.
+// Measured, us a call with 1, 2, 4 groups: 8192 queries x 32 heads (8 key heads) of 128, window 1024:
+// 154, 194, 283; 2 x 512 queries x 16 heads behind 7680 keys, window 4096: 71, 57, 45; 2 x 777
+// queries x 6 heads of 72, window 100: 15, 13.4, 9.2.
 WindowPlan window_plan(int64_t batch_kv, int group, int64_t q_len, int64_t last_len, int64_t window,
                        int64_t sinks, int head_dim) {
   auto heads_of = [&](int q_waves) {

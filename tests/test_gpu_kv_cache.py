@@ -278,6 +278,38 @@ def test_append_e4m3_every_value(hip, dtype, scale):
         assert (got[~nan] == want[~nan]).all(), (s, x[~nan][got[~nan] != want[~nan]][:5])
 
 
+def test_pages_past_32_bits(hip):
+    """Pages 2^30 bytes apart in a pool of 6 GiB: tokens stored into and pages copied between
+    its ends."""
+    say("kv pages past 4 GiB")
+    r = rng(10)
+    num, far, hkv, d, page = 6, 1 << 30, 2, 64, 16
+    size = hkv * page * d * 2
+    pool = hip.DeviceBuffer((num - 1) * far + 2 * size)
+    one = r.integers(0, 65536, size // 2, dtype=np.uint16)
+    pages = [one + np.uint16(i) for i in range(num)]
+    for i, x in enumerate(pages):
+        hip.call("sile_hip_memcpy_htod", pool.ptr + i * far, x.ctypes.data, size)
+    bits = f16_round(r.normal(size=(3, 2, hkv, d)))[0]
+    dx, table, pos = hip.DeviceBuffer.from_array(bits), ints(hip, [[5, 0, 4]]), ints(hip, [3, 16, 47])
+    rows = ints(hip, [0, 0, 0])
+    # (V's pages lie behind K's in the same records)
+    hip.kv_append(hip.F16, hip.F16, 3, hkv, d, dx.ptr, 2 * hkv * d, dx.ptr + 2 * hkv * d, 2 * hkv * d, rows.ptr, pos.ptr,
+                  pool.ptr, pool.ptr + size, num, page, far // 2, table.ptr, 1, 3)
+    src, dst = ints(hip, [5, 0]), ints(hip, [1, 3])
+    hip.kv_copy_pages([pool.ptr], size, far, num, 2, src.ptr, dst.ptr)
+    hip.synchronize()
+    want = [x.reshape(hkv, page, d).copy() for x in pages]
+    for t, (p, slot) in enumerate(((5, 3), (0, 0), (4, 15))):
+        want[p][:, slot] = bits[t, 0]
+    want[1], want[3] = want[5], want[0]
+    got = np.empty(size // 2, np.uint16)
+    for i in range(num):
+        hip.call("sile_hip_memcpy_dtoh", got.ctypes.data, pool.ptr + i * far, size)
+        assert (got == want[i].ravel()).all(), i
+    pool.close()
+
+
 def test_serving_run(hip):
     """Steps of a serving program, captured where they repeat: prompts stored, a token a
     step, beams forked and dropped, pages made writable, the pool closed up; after each
