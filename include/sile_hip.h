@@ -508,7 +508,7 @@ int sile_hip_kv_copy_pages(void *const *pools, int64_t n_pools, int64_t page_byt
 
 /* Frees the rows with drop[r] != 0: each of their entries gives its page's count
  * back and becomes -1, their length 0.  The other rows stay.  Old and new tables,
- * lengths and counts are each the same array or separate ones. */
+ * lengths and counts are each the same array or separate ones; drop is one of its own. */
 int sile_hip_kv_free(int64_t n_rows, int64_t ld_table, const int32_t *drop,
                      const int32_t *tables_in, int32_t *tables_out, const int32_t *lengths_in,
                      int32_t *lengths_out, int64_t num_pages, const int32_t *refs_in,
@@ -518,7 +518,7 @@ int sile_hip_kv_free(int64_t n_rows, int64_t ld_table, const int32_t *drop,
  * (n_in rows), empty where src[i] is outside [0, n_in).  The pages are shared, not copied:
  * a page's count changes by how many rows took its row, less one, so that a row that none
  * took is freed and one that two took is forked (beam search's reordering is one call).
- * Old and new tables and lengths must not overlap; the counts may be one array. */
+ * src, old and new tables and lengths must not overlap; the counts may be one array. */
 int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_t *src,
                      const int32_t *tables_in, int32_t *tables_out, const int32_t *lengths_in,
                      int32_t *lengths_out, int64_t num_pages, const int32_t *refs_in,
@@ -536,7 +536,7 @@ int sile_hip_kv_workspace(int64_t n_rows, int64_t num_pages, size_t *bytes);
  * first, to the rows in order.  granted[r] is 1, or 0 for a row that its table cannot
  * hold and for the first row that the free pages do not cover and every later one that
  * needs any: those stay as they are.  lengths stay.  Old and new tables and counts are
- * each the same array or separate ones. */
+ * each the same array or separate ones; granted is one of its own. */
 int sile_hip_kv_reserve(int64_t n_rows, int64_t ld_table, int64_t page_size,
                         const int32_t *lengths, const int32_t *need, const int32_t *tables_in,
                         int32_t *tables_out, int64_t num_pages, const int32_t *refs_in,

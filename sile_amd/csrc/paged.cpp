@@ -270,6 +270,8 @@ int sile_hip_kv_free(int64_t n_rows, int64_t ld_table, const int32_t* drop, cons
       (rc = check_in_out(lengths_in, lengths_out, n_rows, "lengths")) != SILE_OK ||
       (rc = check_in_out(refs_in, refs_out, num_pages, "counts")) != SILE_OK)
     return rc;
+  if (overlap(drop, n_rows, lengths_out, n_rows) || overlap(drop, n_rows, tables_out, n_rows * ld_table))
+    return fail(SILE_ERR_SHAPE, "drop overlaps what is written");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = copy_ints(refs_in, refs_out, num_pages, s)) != SILE_OK) return rc;
   if (n_rows == 0) return ok();
@@ -293,8 +295,9 @@ int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_
       (n_in > 0 && (!lengths_in || (ld_table > 0 && !tables_in))))
     return fail(SILE_ERR_SHAPE, "NULL operand");
   if (overlap(tables_in, n_in * ld_table, tables_out, n_out * ld_table) ||
-      overlap(lengths_in, n_in, lengths_out, n_out))
-    return fail(SILE_ERR_SHAPE, "a fork's old and new tables and lengths must not overlap");
+      overlap(lengths_in, n_in, lengths_out, n_out) || overlap(src, n_out, lengths_out, n_out) ||
+      overlap(src, n_out, tables_out, n_out * ld_table))
+    return fail(SILE_ERR_SHAPE, "a fork's src, old and new tables and lengths must not overlap");
   if ((rc = check_in_out(refs_in, refs_out, num_pages, "counts")) != SILE_OK) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = copy_ints(refs_in, refs_out, num_pages, s)) != SILE_OK) return rc;
@@ -336,6 +339,8 @@ int sile_hip_kv_reserve(int64_t n_rows, int64_t ld_table, int64_t page_size, con
       (rc = check_in_out(refs_in, refs_out, num_pages, "counts")) != SILE_OK)
     return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, 4 * kv_ints(n_rows, num_pages))) != SILE_OK) return rc;
+  if (overlap(granted, n_rows, need, n_rows) || overlap(granted, n_rows, lengths, n_rows))
+    return fail(SILE_ERR_SHAPE, "granted overlaps need or lengths");
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (n_rows == 0) {
     rc = copy_ints(refs_in, refs_out, num_pages, s);

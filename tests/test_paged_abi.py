@@ -200,6 +200,24 @@ def test_bookkeeping_refusals(name, args, code, needle):
     refused(name, args, code, needle)
 
 
+APART = 1 << 24
+
+
+@pytest.mark.parametrize("name,args,needle", [
+    ("sile_hip_kv_free", [4, 4, P, APART, APART, P, P, 9, P, P, None], "drop overlaps"),
+    ("sile_hip_kv_free", [4, 4, P + 60, P, P, APART, APART, 9, P, P, None], "drop overlaps"),
+    ("sile_hip_kv_fork", [4, 4, 4, P, TABLES, 2 * TABLES, APART, P + 8, 9, P, P, None], "must not overlap"),
+    ("sile_hip_kv_fork", [4, 4, 4, 2 * TABLES + 16, TABLES, 2 * TABLES, APART, P, 9, P, P, None],
+     "must not overlap"),
+    ("sile_hip_kv_reserve", [4, 4, 16, P, APART, P, P, 9, P, P, APART, None, 0, 0, 0, P, 1 << 20, None],
+     "granted overlaps"),
+    ("sile_hip_kv_reserve", [4, 4, 16, P, APART, P, P, 9, P, P, P + 4, None, 0, 0, 0, P, 1 << 20, None],
+     "granted overlaps"),
+])
+def test_arrays_of_their_own_are_refused_when_they_overlap(name, args, needle):
+    refused(name, args, 5, needle)
+
+
 WINDOW = [F16, 2, 4, 2, 10, 20, 64, P, P, P, P, 0.125, 10, 5, 1, None]
 
 
