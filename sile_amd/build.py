@@ -4,9 +4,9 @@
    sile_amd/_build/<name>.hsaco (hipcc --genco --no-gpu-bundle-output).
 2. The host runtime (runtime.cpp, ops.cpp, paged.cpp, llir.cpp,
    tile_ir.cpp) is compiled with g++ against the HIP runtime headers;
-   runtime.cpp assembles the code objects into the library image with .incbin.  launch_noalloc.hip
-   (host code plus the device array its entry point uses) is compiled by
-   hipcc for the host and gfx950.
+   runtime.cpp assembles the code objects into the library image with
+   .incbin.  launch_noalloc.hip (host code plus the device array its entry
+   point uses) is compiled by hipcc for the host and gfx950.
 3. The objects are linked into sile_amd/libsile_hip.so against libamdhip64.
 
 Run: python -m sile_amd.build

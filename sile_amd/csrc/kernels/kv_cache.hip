@@ -40,7 +40,8 @@ struct AppendArgs {
 // correctly rounded: one correction of x * rcp by its remainder is then the quotient
 // (Markstein), wherever it is neither past the range, where it saturates in any case,
 // nor so small that it rounds to zero, and scale is no extreme; else (rcp = 0) the division
-// (a third of the kernel's instructions: 16382 tokens of 8 heads of 128 take 31 us with it, 26 so, before the stores' change).
+// (a third of the kernel's instructions: with plain stores, 16382 tokens of 8 heads of 128
+// take 31 us with it and 26 so).
 SILE_DEV float e4m3_in(float x, float scale, float rcp) {
   float y;
   if (rcp == 0.0f) {

@@ -32,14 +32,16 @@
 // most two a workgroup, and a second launch joins them.  Where the host knows that
 // every row is short, a workgroup takes one unit instead, and there is nothing to join.
 //
+// Measured: 32 rows of up to 8192 keys, 8 key heads of 128 in 16 bits, 97 us (5.7 TB/s of K and V;
+// a copy reaches 5.3), one row of 131071 91 (5.9); 64 rows of up to 4000 in e4m3 61 (4.3); 100 rows
+// under a window of 1000, 4 key heads of 80, 26 (4.8); one row of 300 keys 6.1.
+//
 // An 8-bit cache (e4m3) is widened in registers, exactly: K into the operand, V on
 // its way into LDS; the scales go into the score's and the output's factor.
 #include "common.h"
 #include "paged_plan.h"
 
 using namespace sile;
-
-typedef unsigned int u32x2v __attribute__((ext_vector_type(2)));
 
 namespace {
 
@@ -70,7 +72,6 @@ struct PagedArgs {
   float scale_log2, v_scale;
 };
 
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
 
@@ -123,7 +124,7 @@ SILE_DEV float quad_max(float v) {
 }
 SILE_DEV float quad_sum(float v) { return pair32_sum(v + swizzle_xor16(v)); }
 
-template <int kDp, int kQT>
+template <int kDp>
 struct Shape {
   static constexpr int kRow = 2 * kDp;                        // bytes of a V row in LDS
   static constexpr int kPitch = kDp + 4;                      // floats of an O row in LDS
@@ -132,10 +133,10 @@ struct Shape {
   static constexpr int kWaveB = kTileB > kMergeB ? kTileB : kMergeB;
 };
 
-// The row that holds flat tile x0: the tiles of the rows before row b number
-// before(b), H times each (H key heads' worth).  Every thread adds up a run of
-// rows, a scan over the 256 threads follows.  Workgroup 0 keeps the sums for the
-// join.
+// Dealing: which row holds a workgroup's first tile of the flat list.  Every thread adds
+// up the unit sizes of a run of rows, a scan over the 256 threads follows, and the thread
+// whose run holds the row leaves it here, with the sizes before it (a row stands in the
+// list once a unit).  Workgroup 0 keeps the sums for the join.
 struct DealLds {
   int32_t wave_sum[4];
   int32_t row, before;
@@ -144,7 +145,7 @@ struct DealLds {
 template <bool kBF16, bool kFp8, int kDp, bool kExact, bool kPage16, int kQT>
 __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, float* ml,
                                            DealLds* deal) {
-  using Sh = Shape<kDp, kQT>;
+  using Sh = Shape<kDp>;
   constexpr int kKK = kDp / 32;                      // d-steps of S^T
   constexpr int kDT = kDp / 16;                      // 16-dim tiles of O^T
   constexpr int kEs = kFp8 ? 1 : 2;                  // bytes of a cache element
@@ -629,7 +630,7 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float*
 
 #define SILE_PAGED_KERNEL(NAME, BF, F8, DP, EX, P16, QT, EU)                              \
   extern "C" __global__ __launch_bounds__(256, EU) void NAME(PagedArgs a) {               \
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * Shape<DP, QT>::kWaveB];    \
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * Shape<DP>::kWaveB];        \
     __shared__ float ml[4 * 16 * 2];                                                      \
     __shared__ DealLds deal;                                                              \
     paged_attn<BF, F8, DP, EX, P16, QT>(a, smem, ml, &deal);                              \
