@@ -568,7 +568,9 @@ int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_hea
  * sile_hip_kv_append; an f8e4m3 one holds k / k_scale and v / v_scale (1 otherwise).  A key whose page does not
  * exist counts as unseen; a row without any seen key gives zeros; what lies in
  * unseen slots never reaches a result, NaN and Inf included.  fp32 throughout
- * but for the products' operands, where the probabilities are two 16-bit parts.
+ * but for the products' operands, where the probabilities are two 16-bit parts; a query
+ * head that meets Inf or NaN in V of a key it sees is taken again with fp32 ones by one
+ * wave: as the formula says, but slow.
  * A row's keys may be split over workgroups, by the lengths of all rows, so its
  * rounding can depend on the batch; the same call gives the same bits. */
 int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t batch,

@@ -20,7 +20,8 @@
 //    another until the end of its keys.
 //  * P enters the product as two 16-bit parts, value and rest (16 bits of it in
 //    bf16, 22 in f16): the matrix cores have the room, and the result is then as exact
-//    as an fp32 P's.
+//    as an fp32 P's.  But an Inf of V times a part that is zero, or has the other sign, is not
+//    what the formula says: a result that is not finite is taken again with one fp32 p.
 //  * while a tile is computed the next one's loads are in flight, and the page
 //    numbers of the one after.
 //
@@ -69,6 +70,7 @@ struct PagedArgs {
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
   int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups;
   int32_t direct;       // 1: a workgroup a unit, no list and no parts
+  int32_t e4m3;         // 1: an 8-bit cache
   float scale_log2, v_scale;
 };
 
@@ -140,7 +142,114 @@ struct Shape {
 struct DealLds {
   int32_t wave_sum[4];
   int32_t row, before;
+  int32_t x, x1, first_row, base;   // the workgroup's share, for paged_again
+  int32_t again;                    // 1: it has rows to be taken again
 };
+
+// Whether l is a sum of probabilities that are numbers (scores of NaN, or all -inf, make a whole
+// row NaN, and it stays so).
+SILE_DEV bool finite_sum(float l) { return l > 0.0f && l < __builtin_inff(); }
+
+// A query head of a row by a wave, with p as one fp32 value, for a cache of 16 bits: where V has
+// an Inf in a seen key, the second part of P (zero, or of a sign of its own) makes a NaN of it
+// on the matrix cores.  64 keys at a time: a lane works out a key's score, then the lanes
+// take dims, with eight keys' loads in flight.
+template <bool kBF16>
+SILE_DEV void paged_row(const PagedArgs& a, int row, int kvh, int head, const KeySpan& span) {
+  const int lane = threadIdx.x & 63, d = a.d;
+  auto f32_of = [](uint32_t b) { return kBF16 ? bf16_to_f32((uint16_t)b) : f16_to_f32((uint16_t)b); };
+  const uint16_t* q = a.q + (int64_t)row * a.ldq + (int64_t)head * d;
+  const uint16_t* const k = reinterpret_cast<const uint16_t*>(a.k);
+  const uint16_t* const v = reinterpret_cast<const uint16_t*>(a.v);
+  const int32_t* table = a.tables + (int64_t)row * a.ld_table;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = kLowest, l = 0.0f;
+  const int64_t n = (int64_t)span.sink_end + span.len - span.first;
+  for (int64_t i0 = 0; i0 < n; i0 += 64) {
+    const int64_t i = min(i0 + lane, n - 1);
+    const int key = (int)(i < span.sink_end ? i : i - span.sink_end + span.first);
+    const int32_t id = table[key >> a.page_shift];
+    const bool ok = i0 + lane < n && (uint32_t)id < (uint32_t)a.num_pages;
+    // (a key that is not seen: page 0's row of its slot, which is there)
+    const int64_t off = (int64_t)(ok ? id : 0) * a.page_stride +
+                        (((int64_t)kvh << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * d;
+    float s = 0.0f;
+    for (int c = 0; c < d; c += 8) {
+      const u32x4 qw = *reinterpret_cast<const u32x4*>(q + c), kw = *reinterpret_cast<const u32x4*>(k + off + c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        s += f32_of(qw[j >> 1] >> (16 * (j & 1))) * f32_of(kw[j >> 1] >> (16 * (j & 1)));
+    }
+    s *= a.scale_log2;
+    const float m_new = __builtin_fmaxf(m, wave_max(ok && s == s ? s : kLowest));
+    const float alpha = exp2_fast(m - m_new), p = ok ? exp2_fast(s - m_new) : 0.0f;
+    m = m_new;
+    l = l * alpha + wave_sum(p);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[t] *= alpha;
+    const uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
+    const int off_lo = (int)(uint32_t)off, off_hi = (int)(off >> 32);
+    for (int k0 = 0; k0 < 64; k0 += 8) {
+      uint16_t w[8][4];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane(off_lo, k0 + u);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane(off_hi, k0 + u);
+        const uint16_t* vr = v + (int64_t)((uint64_t)hi << 32 | lo);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[u][t] = lane + 64 * t < d ? vr[lane + 64 * t] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float pu = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(p), k0 + u));
+        if ((seen >> (k0 + u)) & 1)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[t] += pu * f32_of(w[u][t]);
+      }
+    }
+  }
+  const float f = a.v_scale / l;
+  uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)head * d;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    if (lane + 64 * t < d) o[lane + 64 * t] = kBF16 ? bf16_rne(acc[t] * f) : f16_rne(acc[t] * f);
+}
+
+// The query heads of this workgroup's whole units whose results are not finite, again.  Behind
+// the rounds and from what stands in LDS, so that they keep nothing for it (called where a unit
+// ends, it took 28 scalar registers of theirs: 32 rows of 1024 keys 23.4 -> 23.8 us, group 24 40 -> 43;
+// so 23.6 and 40.8).
+template <bool kBF16, int kQT>
+SILE_DEV void paged_again(const PagedArgs& a, const DealLds* deal) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int heads = a.kv_heads * a.head_groups;
+  int32_t x = __builtin_amdgcn_readfirstlane(deal->x), row = __builtin_amdgcn_readfirstlane(deal->first_row);
+  int32_t base = __builtin_amdgcn_readfirstlane(deal->base);
+  const int32_t x1 = __builtin_amdgcn_readfirstlane(deal->x1);
+  while (x < x1 && row < a.batch) {   // as in paged_attn
+    const KeySpan span = key_span(__builtin_amdgcn_readfirstlane(a.lengths[row]), a.capacity, a.window, a.sinks);
+    const int32_t size = unit_size(span);
+    if (x >= base + size * heads) {
+      base += size * heads;
+      ++row;
+      continue;
+    }
+    const int unit = (x - base) / size;
+    const int u0 = x - base - unit * size, u1 = min(size, u0 + (x1 - x));
+    x += u1 - u0;
+    if (u0 > kUnitTiles || u1 < size) continue;   // in parts: the join's
+    const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
+    const int rows = min(16 * kQT, a.group - hg * 16 * kQT);
+    for (int r = 0; r < rows; ++r) {
+      if (((r >> 2) & 3) != wave) continue;   // (the wave that stored it)
+      const int head = kvh * a.group + hg * 16 * kQT + r;
+      const uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)head * a.d;
+      constexpr uint16_t kExp = kBF16 ? 0x7f80 : 0x7c00;
+      bool bad = false;
+      for (int c = lane; c < a.d; c += 64) bad |= (o[c] & kExp) == kExp;
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) paged_row<kBF16>(a, row, kvh, head, span);
+    }
+  }
+}
 
 template <bool kBF16, bool kFp8, int kDp, bool kExact, bool kPage16, int kQT>
 __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, float* ml,
@@ -222,6 +331,13 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
     base = __builtin_amdgcn_readfirstlane(deal->before) * heads;
   }
   uint8_t* const vt = smem + wave * Sh::kWaveB;
+  if (!kFp8 && tid == 0) {
+    deal->x = x;
+    deal->x1 = x1;
+    deal->first_row = row;
+    deal->base = base;
+    deal->again = 0;
+  }
 
   while (x < x1 && row < a.batch) {
     const KeySpan span = key_span(__builtin_amdgcn_readfirstlane(a.lengths[row]), a.capacity, a.window, a.sinks);
@@ -510,6 +626,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
         // a row without keys gives zeros; scores that are all -inf give 0 / 0
         const float f = whole ? (m == -__builtin_inff() ? 0.0f : a.v_scale / sum) : 1.0f;
         const int64_t at = (int64_t)slot * 16 * kQT + head;
+        float z = 0.0f;
         for (int c = 4 * (et & 15); c < d; c += 64) {
           f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -519,6 +636,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
             acc += v * w[i];
           }
           acc *= f;
+          if constexpr (!kFp8) z = __builtin_fmaf((acc[0] + acc[1]) + (acc[2] + acc[3]), 0.0f, z);
           if (whole) {
             const u32x2 out = {pack2<kBF16>(acc[0], acc[1]), pack2<kBF16>(acc[2], acc[3])};
             *reinterpret_cast<u32x2*>(a.o + (int64_t)row * a.ldo + (int64_t)(head0 + head) * d + c) = out;
@@ -526,6 +644,8 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
             *reinterpret_cast<f32x4*>(a.part_o + at * d + c) = acc;
           }
         }
+        // (codes of e4m3 have no Inf)
+        if (!kFp8 && whole && !(z == 0.0f) && finite_sum(sum)) deal->again = 1;
         if (!whole && (et & 15) == 0) {
           a.part_ml[at * 2] = m;
           a.part_ml[at * 2 + 1] = sum;
@@ -533,6 +653,10 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
       }
       __syncthreads();
     }
+  }
+  if constexpr (!kFp8) {
+    __syncthreads();   // (a share may have no round and so no barrier since the flag was cleared)
+    if (__builtin_amdgcn_readfirstlane(deal->again) != 0) paged_again<kBF16, kQT>(a, deal);
   }
 }
 
@@ -620,6 +744,13 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float*
   }
   if (!in) return;
   const float f = top == -__builtin_inff() ? 0.0f : a.v_scale / all;
+  float z = 0.0f;   // (dims past the head's: zeros)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[i] * f, 0.0f, z);
+  if (!a.e4m3 && finite_sum(all) && __builtin_amdgcn_ballot_w64(!(z == 0.0f)) != 0) {
+    paged_row<kBF16>(a, row, kvh, kvh * a.group + hg * 16 * kQT + r, span);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (lane + 64 * i < a.d)

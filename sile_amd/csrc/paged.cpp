@@ -52,7 +52,7 @@ struct PagedArgs {
   int32_t* plan;
   float *part_ml, *part_o;
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
-  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups, direct;
+  int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups, direct, e4m3;
   float scale_log2, v_scale;
 };
 
@@ -481,6 +481,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   a.num_pages = (int32_t)num_pages;
   a.page_shift = page_shift_of(page_size);
   a.groups = (int32_t)plan.groups;
+  a.e4m3 = es == 1;
   a.scale_log2 = scale * k_scale * 1.4426950408889634f;
   a.v_scale = v_scale;
   hipStream_t s = static_cast<hipStream_t>(stream);

@@ -344,3 +344,45 @@ def test_refusals(hip):
             case.run(hip, **over)
     hip.synchronize()
     assert (case.do.download(np.uint16, (2, case.ldo)) == 0x5A5A).all()
+
+
+INF16 = {"f16": 0x7C00, "bf16": 0x7F80}
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("lengths,hq,hkv,d,page,window,sinks", [
+    ([1, 2, 40, 0, 300], 4, 2, 64, 16, 0, 0), ([1, 77], 3, 1, 128, 8, 0, 0), ([1, 200, 33], 20, 1, 80, 32, 0, 0),
+    ([500, 65], 6, 2, 256, 16, 60, 3), ([700, 1, 5000, 64], 4, 2, 128, 16, 0, 0), ([3000, 1], 40, 2, 64, 4, 0, 0),
+    ([20001], 4, 1, 72, 64, 0, 0), ([4000, 900, 5], 17, 1, 104, 16, 700, 40), ([1500, 2500], 5, 1, 256, 128, 0, 0)])
+def test_values_that_are_not_finite(hip, dtype, lengths, hq, hkv, d, page, window, sinks):
+    """Inf and NaN in V of keys that the token sees, in rows of one workgroup and in rows
+    dealt out and joined: in their own dimension the result is what the formula gives
+    (Inf of a sign, or NaN where Inf meets -Inf or NaN is there), and the others are as
+    without them."""
+    case = Case(24, dtype, lengths, hq, hkv, d, page, window, sinks)
+    view = case.pools[1].reshape(case.num, hkv, page, d)
+    inf, nan, neg = INF16[dtype], NAN16[dtype], 0x8000
+    for i, n in enumerate(lengths):
+        at = paged_ref.seen_keys(n, window, sinks)
+        if len(at) == 0:
+            continue
+        mid = at[len(at) // 2]
+        for h in range(hkv):
+            for j, dim, bits in ((at[0], 3, inf), (at[-1], 5, inf | neg), (mid, 2, inf), (mid, 7, nan),
+                                 (at[0], d - 1, inf), (at[-1], d - 1, inf | neg)):
+                if h and dim == 3:
+                    continue   # another key head: other dimensions
+                view[case.tables[i, j // page], h, j % page, dim] = bits
+                case.kv[i][1][h, j, dim] = as_f32(np.array([bits], np.uint16), dtype)[0]
+    say(f"paged attn Inf in V {dtype} {lengths} {hq}/{hkv} d={d} page={page} window={window}")
+    case.upload(hip)
+    case.run(hip)
+    got = as_f32(case.result(hip), dtype).astype(np.float64)
+    for i in range(case.b):
+        for h in range(hq):
+            with np.errstate(invalid="ignore"):
+                ref, bound = case.reference(i, h)
+                err = np.abs(got[i, h] - ref)
+            same = (got[i, h] == ref) | (np.isnan(got[i, h]) & np.isnan(ref))
+            assert (same | (np.isfinite(ref) & (err <= bound))).all(), (i, h, got[i, h][:8], ref[:8])
+            assert lengths[i] == 0 or np.isinf(ref).any()
