@@ -224,3 +224,18 @@ def test_stream_and_graph(hip):
         c.run(hip)
     graph.close()
     st.close()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 72, 128])
+@pytest.mark.parametrize("hq,hkv,n,window", [
+    (48, 16, 700, 100), (32, 16, 1100, 100), (16, 4, 2100, 100),    # one key group; 1, 2 and 4 query heads a workgroup
+    (8, 8, 2100, 300), (8, 4, 2100, 300), (8, 2, 2100, 300),        # two
+    (2, 2, 777, 500), (4, 2, 500, 400), (3, 1, 900, 700)])          # four; 1, 2 and 1 query heads
+def test_every_layout(hip, dtype, d, hq, hkv, n, window):
+    """What window_plan chooses on 256 CUs: every number of key groups, with every number
+    of query heads a workgroup takes, in each width up to 128; rows at the edges of
+    blocks and of the window, in every head."""
+    c = Case(15, dtype, 1, hq, hkv, n, d, window, 4)
+    at = {0, 1, 31, 32, 33, 63, 64, 65, 127, 128, window - 1, window, window + 1, n // 2, n - 65, n - 33, n - 32, n - 2, n - 1}
+    c.check(c.run(hip), rows=sorted(at))
