@@ -520,3 +520,36 @@ def test_graph_of_a_step(hip):
             assert (a == b).all()
     graph.close()
     st.close()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_large_pools(hip, in_place):
+    """A pool of 100000 pages: the one workgroup that ranks free pages and plans the
+    closing up goes on past what it holds in registers."""
+    say(f"kv 100000 pages in_place={in_place}")
+    s = State(11, 300, 400, 16, 40000, page_bytes=16, pools=1, extra=5).upload(hip)
+    assert s.num > 90000, s.num
+    need = s.r.integers(0, 3000, 300).astype(np.int32)
+    dn, dg, used = ints(hip, need), ints(hip, np.full(300, 9)), ints(hip, [-1])
+    t, f = (s.dt, s.dr) if in_place else (ints(hip, s.tables * 0), ints(hip, s.refs * 0))
+    hip.kv_reserve(300, 400, 16, s.dl.ptr, dn.ptr, s.dt.ptr, t.ptr, s.num, s.dr.ptr, f.ptr, dg.ptr, *s.pool_args(),
+                   s.ws.ptr, s.ws.nbytes)
+    hip.synchronize()
+    tables, refs, granted, copies = paged_ref.reserve(16, s.num, s.lengths.tolist(), need.tolist(), s.tables.tolist(),
+                                                      s.refs.tolist())
+    assert 0 < sum(granted) < 300 and (down(dg, 300) == granted).all()
+    assert (down(t, s.tables.shape) == tables).all() and (down(f, s.num) == refs).all()
+    s.check_pools(copies, "copies")
+    # every 20th row goes; what stays is closed up
+    s.tables, s.refs = np.array(tables, np.int32), np.array(refs, np.int32)
+    s.pools = [p.download(np.uint8, x.shape) for p, x in zip(s.dp, s.pools)]
+    s.refs -= counts_of(s.tables[::20], s.num, np.zeros(s.num)).astype(np.int32)
+    s.tables[::20] = -1
+    dt, dr = ints(hip, s.tables), ints(hip, s.refs)
+    t, f = (dt, dr) if in_place else (t, f)
+    hip.kv_compact(300, 400, dt.ptr, t.ptr, s.num, dr.ptr, f.ptr, used.ptr, *s.pool_args(), s.ws.ptr, s.ws.nbytes)
+    hip.synchronize()
+    tables, refs, u, moves = paged_ref.compact(s.num, s.tables.tolist(), s.refs.tolist())
+    assert down(used, 1)[0] == u and len(moves) > 1000 and max(moves) > 65536
+    assert (down(t, s.tables.shape) == tables).all() and (down(f, s.num) == refs).all()
+    s.check_pools(list(moves.items()), "moves")
