@@ -455,8 +455,9 @@ int sile_hip_flash_attn_fwd(sile_dtype dtype, int64_t batch, int64_t heads, int6
  * cores (the probabilities enter the second product in 16 bits; a row's rounding can depend on
  * the shape of the call); others on a VALU kernel of one wave per query row.  A row
  * whose result is not finite, or meets Inf or NaN in V of a masked key of its block, is
- * taken again row by row: right, but slow.  q_start + q_len <= 2^29, and one head's
- * K at most 2^31 - 1 bytes.  Its form for single tokens: sile_hip_paged_attn_decode.
+ * taken again row by row: right, but slow.  q_start + q_len and kv_len <= 2^29, one head's
+ * K at most 2^31 - 1 bytes, batch * q_heads * q_len < 2^31 (on the matrix cores some 2^24 blocks
+ * of 32 to 128 query rows of one key head; more key heads take more launches).  Its form for single tokens: sile_hip_paged_attn_decode.
  * No reference counterpart, as sile_hip_flash_attn_fwd. */
 int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_heads,
                                    int64_t kv_heads, int64_t q_len, int64_t kv_len,

@@ -591,16 +591,16 @@ SILE_FW_GROUPS(32, 128, 128)
 SILE_FW_DTYPES(4, 1, 32, 192, 256, 1)
 SILE_FW_DTYPES(4, 1, 32, 256, 256, 1)
 
-// Any head dimension up to 256, alignment and scale: a wave a query row.
+// Any head dimension up to 256, alignment and scale: a wave a query row, and the next past the grid.
 template <bool kBF16>
 SILE_DEV void window_rowwise(const uint16_t* Q, const uint16_t* K, const uint16_t* V, uint16_t* O,
                              const WindowArgs& a, int64_t rows) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int64_t head = r / a.q_len, i = r - head * a.q_len, kv = head / a.group * a.kv_len * a.d;
-  int64_t sink_end, first, last;
-  seen_range(a, a.start + i, &sink_end, &first, &last);
-  window_row<kBF16>(Q + r * a.d, K + kv, V + kv, O + r * a.d, sink_end, first, last, a.d, a.scale_log2);
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+    const int64_t head = r / a.q_len, i = r - head * a.q_len, kv = head / a.group * a.kv_len * a.d;
+    int64_t sink_end, first, last;
+    seen_range(a, a.start + i, &sink_end, &first, &last);
+    window_row<kBF16>(Q + r * a.d, K + kv, V + kv, O + r * a.d, sink_end, first, last, a.d, a.scale_log2);
+  }
 }
 extern "C" __global__ __launch_bounds__(256) void sile_flash_window_rowwise_f16(
     const uint16_t* Q, const uint16_t* K, const uint16_t* V, uint16_t* O, WindowArgs a, int64_t rows) {

@@ -1315,20 +1315,29 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
     const int64_t bq = 32 * plan.q_waves / plan.heads;
     wa.heads = plan.heads;
     wa.q_blocks = (int32_t)((q_len + bq - 1) / bq);
-    wa.items = (int32_t)(batch * kv_heads * (wa.group / plan.heads) * wa.q_blocks);
-    // (a launch has less than 2^32 threads)
-    if (wa.items > (1 << 22)) return fail(SILE_ERR_SHAPE, "attention too large (%d blocks)", wa.items);
+    // a launch has less than 2^32 threads; past that the key heads in several launches
+    const int64_t each = (int64_t)(wa.group / plan.heads) * wa.q_blocks, most = 0xffffffffll / (64 * plan.waves) / 8 * 8;
+    if (each > most) return fail(SILE_ERR_SHAPE, "attention too large (%lld blocks of one key head)", (long long)each);
     snprintf(name, sizeof name, "sile_flash_window_%s_d%d_g%d", dt, dh, plan.groups);
-    void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa};
-    const unsigned blocks = (unsigned)((wa.items + 7ll) / 8 * 8);
-    const int rc = launch(Module::kFlashWindow, name, dim3(blocks), dim3((unsigned)(64 * plan.waves)), params, s);
-    return rc == SILE_OK ? ok() : rc;
+    const int64_t kv_all = batch * kv_heads, step = most / each;
+    for (int64_t kv0 = 0; kv0 < kv_all; kv0 += step) {
+      wa.items = (int32_t)(std::min(step, kv_all - kv0) * each);
+      const int64_t at_q = kv0 * wa.group * q_len * head_dim, at_kv = kv0 * kv_len * head_dim;
+      const uint16_t* qs = static_cast<const uint16_t*>(q) + at_q;
+      const uint16_t* ks = static_cast<const uint16_t*>(k) + at_kv;
+      const uint16_t* vs = static_cast<const uint16_t*>(v) + at_kv;
+      uint16_t* os = static_cast<uint16_t*>(o) + at_q;
+      void* params[] = {&qs, &ks, &vs, &os, &wa};
+      const unsigned blocks = (unsigned)((wa.items + 7ll) / 8 * 8);
+      const int rc = launch(Module::kFlashWindow, name, dim3(blocks), dim3((unsigned)(64 * plan.waves)), params, s);
+      if (rc != SILE_OK) return rc;
+    }
+    return ok();
   }
-  int64_t rows = batch * q_heads * q_len;
-  if (rows > (1 << 24)) return fail(SILE_ERR_SHAPE, "attention too large (%lld rows)", (long long)rows);
+  int64_t rows = batch * q_heads * q_len;   // (a wave takes several past 2^25)
   snprintf(name, sizeof name, "sile_flash_window_rowwise_%s", dt);
   void* params[] = {(void*)&q, (void*)&k, (void*)&v, &o, &wa, &rows};
-  const int rc = launch(Module::kFlashWindow, name, dim3((unsigned)((rows + 3) / 4)), dim3(256), params, s);
+  const int rc = launch(Module::kFlashWindow, name, dim3((unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 23)), dim3(256), params, s);
   return rc == SILE_OK ? ok() : rc;
 }
 

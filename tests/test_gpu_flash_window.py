@@ -239,3 +239,39 @@ def test_every_layout(hip, dtype, d, hq, hkv, n, window):
     c = Case(15, dtype, 1, hq, hkv, n, d, window, 4)
     at = {0, 1, 31, 32, 33, 63, 64, 65, 127, 128, window - 1, window, window + 1, n // 2, n - 65, n - 33, n - 32, n - 2, n - 1}
     c.check(c.run(hip), rows=sorted(at))
+
+
+def test_more_rows_than_a_launch_takes(hip):
+    """Query rows past 2^25 on the row kernel (an odd head dimension) and past 2^24 blocks on
+    the matrix cores: the calls an aligned or a smaller one takes, and every row written."""
+    r = rng(16)
+    n, d = (1 << 25) + 77, 3
+    q = r.integers(-8, 8, (n, d), dtype=np.int16).astype(np.float16)
+    say(f"window f16 1x1 q={n} d={d} w=2")
+    buf = hip.DeviceBuffer.from_array(q.view(np.uint16))
+    o = hip.DeviceBuffer(q.nbytes)
+    o.fill_bytes(0xFF)
+    hip.flash_attn_window_fwd(hip.F16, 1, 1, 1, n, n, d, buf.ptr, buf.ptr, buf.ptr, o.ptr, 0.25, 0, 2)
+    hip.synchronize()
+    got = o.download(np.float16, (n, d))
+    assert np.isfinite(got).all()
+    for i in (0, 1, 2, (1 << 24) - 1, 1 << 24, (1 << 25) - 1, 1 << 25, n - 2, n - 1):
+        x = q[max(0, i - 1):i + 1].astype(np.float64)
+        ref, spread, size = paged_ref.attention(x[-1], x, x, 0.25)
+        assert (np.abs(got[i] - ref) <= paged_ref.error_bound(ref, spread, size, "f16", d, 2, 0.0)).all(), i
+    buf.close()
+    o.close()
+    # one query and one key a head: the result is V's row
+    b, d = (1 << 24) + 5, 8
+    say(f"window f16 {b}x1 q=1 d={d}")
+    bits = r.integers(0, 0x7C00, (1 << 20) * d, dtype=np.uint16)
+    v = np.resize(bits, b * d)
+    dv, o = hip.DeviceBuffer.from_array(v), hip.DeviceBuffer(v.nbytes)
+    o.fill_bytes(0xFF)
+    hip.flash_attn_window_fwd(hip.F16, b, 1, 1, 1, 1, d, dv.ptr, dv.ptr, dv.ptr, o.ptr, 1e-4, 0, 1)
+    hip.synchronize()
+    got = o.download(np.float16, v.shape).astype(np.float32)
+    want = v.view(np.float16).astype(np.float32)
+    assert (np.abs(got - want) <= 2.0 ** -11 * want + 2.0 ** -25).all()
+    dv.close()
+    o.close()

@@ -237,3 +237,13 @@ def test_window_without_queries_is_fine():
         args = list(WINDOW)
         args[at] = 0
         assert _abi.status("sile_hip_flash_attn_window_fwd", *args) == 0
+
+
+@pytest.mark.parametrize("over,needle", [
+    ({1: 1, 2: 64, 3: 1, 4: 2 ** 25 - 1}, "blocks of one key head"), ({2: 2 ** 15, 3: 2 ** 15, 4: 2 ** 16}, "too large"),
+    ({4: 2 ** 29, 12: 1}, "too long"), ({5: 2 ** 29 + 1, 6: 1}, "too long")])
+def test_window_limits(over, needle):
+    args = list(WINDOW)
+    for at, value in over.items():
+        args[at] = value
+    refused("sile_hip_flash_attn_window_fwd", args, 5, needle)
