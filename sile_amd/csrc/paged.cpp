@@ -175,14 +175,17 @@ struct PagedPlan {
   int dp, q_tiles, per_cu, cus;
   int64_t head_groups, groups, plan_ints, slots, bytes;
 };
-int paged_plan(bool fp8, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, PagedPlan* p) {
+void paged_shape(int64_t q_heads, int64_t kv_heads, int64_t head_dim, PagedPlan* p) {
   const int64_t group = q_heads / kv_heads;
   p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
   p->q_tiles = group > 16 && p->dp < 256 ? 2 : 1;
+  p->head_groups = (group + 16 * p->q_tiles - 1) / (16 * p->q_tiles);
+}
+int paged_plan(bool fp8, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim, PagedPlan* p) {
+  paged_shape(q_heads, kv_heads, head_dim, p);
   p->per_cu = p->dp == 64 ? (p->q_tiles == 1 ? 4 : 2) : p->dp == 128 && p->q_tiles == 1 ? (fp8 ? 3 : 2) : 1;
   const int rc = device_cus(&p->cus);
   if (rc != SILE_OK) return rc;
-  p->head_groups = (group + 16 * p->q_tiles - 1) / (16 * p->q_tiles);
   p->groups = (int64_t)p->per_cu * p->cus;
   p->plan_ints = ints16(batch + 1);
   p->slots = 2 * p->groups * 16 * p->q_tiles;   // two a workgroup
@@ -444,8 +447,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
     return fail(SILE_ERR_SHAPE, "q, o and the pages have to be 16-byte aligned");
   if (ldq > (1ll << 40) || ldo > (1ll << 40)) return fail(SILE_ERR_SHAPE, "leading dimension too large");
   PagedPlan plan;
-  if ((rc = paged_plan(es == 1, batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
-  if ((rc = check_workspace(workspace, workspace_bytes, plan.bytes)) != SILE_OK) return rc;
+  paged_shape(q_heads, kv_heads, head_dim, &plan);
   // without a page every row is empty
   const int64_t capacity = num_pages > 0 ? std::min<int64_t>(ld_table * page_size, kIntMax) : 0;
   // tiles are numbered in 32 bits, over all rows and key heads
@@ -456,6 +458,8 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   if (batch > (kIntMax - (1 << 20)) / row_tiles || batch * kv_heads * plan.head_groups > kMaxRows)
     return fail(SILE_ERR_SHAPE, "%lld rows of up to %lld keys: too many for one call", (long long)batch,
                 (long long)seen);
+  if ((rc = paged_plan(es == 1, batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
+  if ((rc = check_workspace(workspace, workspace_bytes, plan.bytes)) != SILE_OK) return rc;
   PagedArgs a{};
   a.q = q;
   a.k = k_pages;

@@ -247,3 +247,14 @@ def test_window_limits(over, needle):
     for at, value in over.items():
         args[at] = value
     refused("sile_hip_flash_attn_window_fwd", args, 5, needle)
+
+
+@pytest.mark.parametrize("over", [
+    {2: 2 ** 21, 3: 8, 4: 4, 7: 512, 12: 4096, 17: 512},               # units: rows x key heads
+    {2: 2 ** 21, 3: 129, 4: 1, 7: 129 * 64, 17: 129 * 64, 12: 1024},   # and groups of query heads
+    {2: 2 ** 14, 14: 2 ** 16, 11: 64, 12: 8192}])                      # tiles of rows of 2^22 keys
+def test_decode_limits(over):
+    args = list(DECODE)
+    for at, value in over.items():
+        args[at] = value
+    refused("sile_hip_paged_attn_decode", args, 5, "too many for one call")
