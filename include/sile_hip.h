@@ -482,7 +482,9 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
  * At most 2^22 rows; the entries of a table and the pages each below 2^31.
  * All calls only enqueue, on the current device, and can be captured into a
  * graph (they are plain kernel launches); the same workspace serves calls
- * that run one after another, never two that may run side by side. */
+ * that run one after another, never two that may run side by side.  An int32 array
+ * that a call writes, and a workspace, shares nothing with another array of the call
+ * but its own old form, where that may be the same: refused otherwise. */
 
 /* Stores n_tokens new tokens: K's rows k + t * ldk and V's v + t * ldv, each
  * [kv_heads][head_dim] (so both may point into one fused projection), at position

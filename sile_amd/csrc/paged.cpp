@@ -9,6 +9,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 
 #include "kernels/paged_plan.h"
 #include "runtime_internal.h"
@@ -105,7 +106,22 @@ int check_table(int64_t rows, int64_t ld_table) {
 
 // whether [x, x + nx) and [y, y + ny) share an element
 bool overlap(const int32_t* x, int64_t nx, const int32_t* y, int64_t ny) {
-  return x && y && x < y + ny && y < x + nx;
+  return x && y && nx > 0 && ny > 0 && x < y + ny && y < x + nx;
+}
+// The arrays of a call: one that it writes shares nothing with another, but for the old and the
+// new form of the same thing (check_in_out).
+struct Span {
+  const char* name;
+  const int32_t* p;
+  int64_t n;
+  bool written;
+};
+int check_apart(std::initializer_list<Span> all) {
+  for (const Span& x : all)
+    for (const Span& y : all)
+      if (x.written && strcmp(x.name, y.name) != 0 && overlap(x.p, x.n, y.p, y.n))
+        return fail(SILE_ERR_SHAPE, "%s overlaps %s", x.name, y.name);
+  return SILE_OK;
 }
 // a call in place or out of place, nothing in between
 int check_in_out(const int32_t* in, const int32_t* out, int64_t n, const char* what) {
@@ -275,6 +291,12 @@ int sile_hip_kv_free(int64_t n_rows, int64_t ld_table, const int32_t* drop, cons
     return rc;
   if (overlap(drop, n_rows, lengths_out, n_rows) || overlap(drop, n_rows, tables_out, n_rows * ld_table))
     return fail(SILE_ERR_SHAPE, "drop overlaps what is written");
+  const int64_t entries = n_rows * ld_table;
+  if ((rc = check_apart({{"drop", drop, n_rows, false}, {"tables", tables_in, entries, false},
+                         {"tables", tables_out, entries, true}, {"lengths", lengths_in, n_rows, false},
+                         {"lengths", lengths_out, n_rows, true}, {"counts", refs_in, num_pages, false},
+                         {"counts", refs_out, num_pages, true}})) != SILE_OK)
+    return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = copy_ints(refs_in, refs_out, num_pages, s)) != SILE_OK) return rc;
   if (n_rows == 0) return ok();
@@ -302,6 +324,11 @@ int sile_hip_kv_fork(int64_t n_in, int64_t n_out, int64_t ld_table, const int32_
       overlap(src, n_out, tables_out, n_out * ld_table))
     return fail(SILE_ERR_SHAPE, "a fork's src, old and new tables and lengths must not overlap");
   if ((rc = check_in_out(refs_in, refs_out, num_pages, "counts")) != SILE_OK) return rc;
+  if ((rc = check_apart({{"src", src, n_out, false}, {"tables", tables_in, n_in * ld_table, false},
+                         {"tables", tables_out, n_out * ld_table, true}, {"lengths", lengths_in, n_in, false},
+                         {"lengths", lengths_out, n_out, true}, {"counts", refs_in, num_pages, false},
+                         {"counts", refs_out, num_pages, true}})) != SILE_OK)
+    return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if ((rc = copy_ints(refs_in, refs_out, num_pages, s)) != SILE_OK) return rc;
   if (n_in + n_out == 0) return ok();
@@ -344,6 +371,12 @@ int sile_hip_kv_reserve(int64_t n_rows, int64_t ld_table, int64_t page_size, con
   if ((rc = check_workspace(workspace, workspace_bytes, 4 * kv_ints(n_rows, num_pages))) != SILE_OK) return rc;
   if (overlap(granted, n_rows, need, n_rows) || overlap(granted, n_rows, lengths, n_rows))
     return fail(SILE_ERR_SHAPE, "granted overlaps need or lengths");
+  if ((rc = check_apart({{"lengths", lengths, n_rows, false}, {"need", need, n_rows, false},
+                         {"tables", tables_in, n_rows * ld_table, false}, {"tables", tables_out, n_rows * ld_table, true},
+                         {"counts", refs_in, num_pages, false}, {"counts", refs_out, num_pages, true},
+                         {"granted", granted, n_rows, true},
+                         {"workspace", static_cast<int32_t*>(workspace), kv_ints(n_rows, num_pages), true}})) != SILE_OK)
+    return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (n_rows == 0) {
     rc = copy_ints(refs_in, refs_out, num_pages, s);
@@ -392,6 +425,11 @@ int sile_hip_kv_compact(int64_t n_rows, int64_t ld_table, const int32_t* tables_
       (rc = check_in_out(refs_in, refs_out, num_pages, "counts")) != SILE_OK)
     return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, 4 * kv_ints(n_rows, num_pages))) != SILE_OK) return rc;
+  if ((rc = check_apart({{"tables", tables_in, n_rows * ld_table, false}, {"tables", tables_out, n_rows * ld_table, true},
+                         {"counts", refs_in, num_pages, false}, {"counts", refs_out, num_pages, true},
+                         {"used", used, 1, true},
+                         {"workspace", static_cast<int32_t*>(workspace), kv_ints(n_rows, num_pages), true}})) != SILE_OK)
+    return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   int32_t* moves = static_cast<int32_t*>(workspace);
   int32_t* map = moves + 4;

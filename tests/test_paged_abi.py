@@ -258,3 +258,38 @@ def test_decode_limits(over):
     for at, value in over.items():
         args[at] = value
     refused("sile_hip_paged_attn_decode", args, 5, "too many for one call")
+
+
+def _apart():
+    """(call, arguments far apart, i, j): array i moved into array j, for every pair of them that
+    the call must not take: one of the two is written, and they are not the old and the new
+    form of the same thing."""
+    far = lambda n: n << 24  # noqa: E731
+    t, n, p, ws = 16, 4, 9, 1 << 18   # elements: 4 x 4 tables, 4 rows, 9 pages, the workspace
+    calls = {
+        "sile_hip_kv_free": ([4, 4, far(2), far(3), far(4), far(5), far(6), 9, far(8), far(9), None],
+                             {2: ("drop", n, 0), 3: ("tables", t, 0), 4: ("tables", t, 1), 5: ("lengths", n, 0),
+                              6: ("lengths", n, 1), 8: ("counts", p, 0), 9: ("counts", p, 1)}),
+        "sile_hip_kv_fork": ([4, 4, 4, far(3), far(4), far(5), far(6), far(7), 9, far(9), far(10), None],
+                             {3: ("src", n, 0), 4: ("tables", t, 0), 5: ("tables", t, 1), 6: ("lengths", n, 0),
+                              7: ("lengths", n, 1), 9: ("counts", p, 0), 10: ("counts", p, 1)}),
+        "sile_hip_kv_reserve": ([4, 4, 16, far(3), far(4), far(5), far(6), 9, far(8), far(9), far(10), None, 0, 0, 0, far(15),
+                                 4 * ws, None],
+                                {3: ("lengths", n, 0), 4: ("need", n, 0), 5: ("tables", t, 0), 6: ("tables", t, 1),
+                                 8: ("counts", p, 0), 9: ("counts", p, 1), 10: ("granted", n, 1), 15: ("workspace", 16, 1)}),
+        "sile_hip_kv_compact": ([4, 4, far(2), far(3), 9, far(5), far(6), far(7), None, 0, 0, 0, far(12), 4 * ws, None],
+                                {2: ("tables", t, 0), 3: ("tables", t, 1), 5: ("counts", p, 0), 6: ("counts", p, 1),
+                                 7: ("used", 1, 1), 12: ("workspace", 16, 1)})}
+    for name, (args, arrays) in calls.items():
+        for i, (what, _, written) in arrays.items():
+            for j, (other, size, written_j) in arrays.items():
+                if what != "workspace" and what != other and (written or written_j):
+                    for at in sorted({0, size - 1}):
+                        yield pytest.param(name, args, i, args[j] + 4 * at, id=f"{name[9:]}-{what}{i}-{other}{j}-{at}")
+
+
+@pytest.mark.parametrize("name,args,i,address", _apart())
+def test_arrays_that_a_call_writes_lie_apart(name, args, i, address):
+    args = list(args)
+    args[i] = address
+    refused(name, args, 5, "overlap")
