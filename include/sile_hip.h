@@ -573,7 +573,7 @@ int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_hea
  * unseen slots never reaches a result, NaN and Inf included.  fp32 throughout
  * but for the products' operands, where the probabilities are two 16-bit parts; a query
  * head that meets Inf or NaN in V of a key it sees is taken again with fp32 ones by one
- * wave: as the formula says, but slow.  One call takes at
+ * workgroup: as the formula says, but slow.  One call takes at
  * most 2^22 units (a row's key head with up to 16 or 32 query heads of it) and, of the table's
  * width or the window, some 2^36 keys over all units.
  * A row's keys may be split over workgroups, by the lengths of all rows, so its

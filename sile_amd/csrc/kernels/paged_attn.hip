@@ -150,21 +150,23 @@ struct DealLds {
 // row NaN, and it stays so).
 SILE_DEV bool finite_sum(float l) { return l > 0.0f && l < __builtin_inff(); }
 
-// A query head of a row by a wave, with p as one fp32 value, for a cache of 16 bits: where V has
-// an Inf in a seen key, the second part of P (zero, or of a sign of its own) makes a NaN of it
-// on the matrix cores.  64 keys at a time: a lane works out a key's score, then the lanes
-// take dims, with eight keys' loads in flight.
-template <bool kBF16>
-SILE_DEV void paged_row(const PagedArgs& a, int row, int kvh, int head, const KeySpan& span) {
-  const int lane = threadIdx.x & 63, d = a.d;
+// A query head of a row by a workgroup of kWaves, with p as one fp32 value, for a cache of 16
+// bits: where V has an Inf in a seen key, the second part of P (zero, or of a sign of its own)
+// makes a NaN of it on the matrix cores.  A wave takes every kWaves-th 64 keys: a lane works
+// out a key's score, then the lanes take two dims each, with 16 keys' loads in flight; the waves'
+// sums are added up through LDS, kWaves * (2 + 256) floats.  (One row of 131071 keys with an Inf:
+// 2.9 ms in place of 92 us, 32 rows of 2000 0.36 ms in place of 42 us.)
+template <bool kBF16, int kWaves>
+SILE_DEV void paged_row(const PagedArgs& a, int row, int kvh, int head, const KeySpan& span, float* lds) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = a.d;
   auto f32_of = [](uint32_t b) { return kBF16 ? bf16_to_f32((uint16_t)b) : f16_to_f32((uint16_t)b); };
   const uint16_t* q = a.q + (int64_t)row * a.ldq + (int64_t)head * d;
   const uint16_t* const k = reinterpret_cast<const uint16_t*>(a.k);
   const uint16_t* const v = reinterpret_cast<const uint16_t*>(a.v);
   const int32_t* table = a.tables + (int64_t)row * a.ld_table;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = kLowest, l = 0.0f;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = kLowest, l = 0.0f;   // dims 2 lane, 2 lane + 1, and 128 on
   const int64_t n = (int64_t)span.sink_end + span.len - span.first;
-  for (int64_t i0 = 0; i0 < n; i0 += 64) {
+  for (int64_t i0 = 64 * wave; i0 < n; i0 += 64 * kWaves) {
     const int64_t i = min(i0 + lane, n - 1);
     const int key = (int)(i < span.sink_end ? i : i - span.sink_end + span.first);
     const int32_t id = table[key >> a.page_shift];
@@ -173,6 +175,7 @@ SILE_DEV void paged_row(const PagedArgs& a, int row, int kvh, int head, const Ke
     const int64_t off = (int64_t)(ok ? id : 0) * a.page_stride +
                         (((int64_t)kvh << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * d;
     float s = 0.0f;
+#pragma unroll 4
     for (int c = 0; c < d; c += 8) {
       const u32x4 qw = *reinterpret_cast<const u32x4*>(q + c), kw = *reinterpret_cast<const u32x4*>(k + off + c);
 #pragma unroll
@@ -188,40 +191,56 @@ SILE_DEV void paged_row(const PagedArgs& a, int row, int kvh, int head, const Ke
     for (int t = 0; t < 4; ++t) acc[t] *= alpha;
     const uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
     const int off_lo = (int)(uint32_t)off, off_hi = (int)(off >> 32);
-    for (int k0 = 0; k0 < 64; k0 += 8) {
-      uint16_t w[8][4];
+    for (int k0 = 0; k0 < 64; k0 += 16) {
+      if (((seen >> k0) & 0xffff) == 0) continue;
+      uint32_t w[16][2];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < 16; ++u) {
         const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane(off_lo, k0 + u);
         const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane(off_hi, k0 + u);
-        const uint16_t* vr = v + (int64_t)((uint64_t)hi << 32 | lo);
+        const uint16_t* vr = v + (int64_t)((uint64_t)hi << 32 | lo) + 2 * lane;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) w[u][t] = lane + 64 * t < d ? vr[lane + 64 * t] : 0;
+        for (int t = 0; t < 2; ++t)
+          w[u][t] = 2 * lane + 128 * t < d ? *reinterpret_cast<const uint32_t*>(vr + 128 * t) : 0;
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < 16; ++u) {
         const float pu = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(p), k0 + u));
         if ((seen >> (k0 + u)) & 1)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) acc[t] += pu * f32_of(w[u][t]);
+          for (int t = 0; t < 4; ++t) acc[t] += pu * f32_of(w[u][t >> 1] >> (16 * (t & 1)));
       }
     }
   }
-  const float f = a.v_scale / l;
-  uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)head * d;
+  if (lane == 0) {
+    lds[2 * wave] = m;
+    lds[2 * wave + 1] = l;
+  }
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
-    if (lane + 64 * t < d) o[lane + 64 * t] = kBF16 ? bf16_rne(acc[t] * f) : f16_rne(acc[t] * f);
+  for (int t = 0; t < 4; ++t) lds[2 * kWaves + 256 * wave + 128 * (t >> 1) + 2 * lane + (t & 1)] = acc[t];
+  __syncthreads();
+  const int dim = threadIdx.x;
+  if (dim < d) {
+    float top = kLowest, sum = 0.0f, o = 0.0f;
+    for (int w = 0; w < kWaves; ++w) top = __builtin_fmaxf(top, lds[2 * w]);
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = exp2_fast(lds[2 * w] - top);
+      sum += f * lds[2 * w + 1];
+      o += f * lds[2 * kWaves + 256 * w + dim];
+    }
+    o *= a.v_scale / sum;
+    a.o[(int64_t)row * a.ldo + (int64_t)head * d + dim] = kBF16 ? bf16_rne(o) : f16_rne(o);
+  }
+  __syncthreads();   // (the next head's sums go to the same place)
 }
 
 // The query heads of this workgroup's whole units whose results are not finite, again.  Behind
 // the rounds and from what stands in LDS, so that they keep nothing for it (called where a unit
 // ends, it took 28 scalar registers of theirs: 32 rows of 1024 keys 23.4 -> 23.8 us, group 24 40 -> 43;
-// so 23.6 and 40.8).
+// so 23.7 and 41).
 template <bool kBF16, int kQT>
-SILE_DEV void paged_again(const PagedArgs& a, const DealLds* deal) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int heads = a.kv_heads * a.head_groups;
+SILE_DEV void paged_again(const PagedArgs& a, const DealLds* deal, float* lds) {
+  const int lane = threadIdx.x & 63, heads = a.kv_heads * a.head_groups;
   int32_t x = __builtin_amdgcn_readfirstlane(deal->x), row = __builtin_amdgcn_readfirstlane(deal->first_row);
   int32_t base = __builtin_amdgcn_readfirstlane(deal->base);
   const int32_t x1 = __builtin_amdgcn_readfirstlane(deal->x1);
@@ -238,15 +257,13 @@ SILE_DEV void paged_again(const PagedArgs& a, const DealLds* deal) {
     x += u1 - u0;
     if (u0 > kUnitTiles || u1 < size) continue;   // in parts: the join's
     const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
-    const int rows = min(16 * kQT, a.group - hg * 16 * kQT);
-    for (int r = 0; r < rows; ++r) {
-      if (((r >> 2) & 3) != wave) continue;   // (the wave that stored it)
-      const int head = kvh * a.group + hg * 16 * kQT + r;
-      const uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)head * a.d;
+    const int head0 = kvh * a.group + hg * 16 * kQT, rows = min(16 * kQT, a.group - hg * 16 * kQT);
+    for (int r = 0; r < rows; ++r) {   // (every wave sees the same: a head is stored anew behind a barrier)
+      const uint16_t* o = a.o + (int64_t)row * a.ldo + (int64_t)(head0 + r) * a.d;
       constexpr uint16_t kExp = kBF16 ? 0x7f80 : 0x7c00;
       bool bad = false;
       for (int c = lane; c < a.d; c += 64) bad |= (o[c] & kExp) == kExp;
-      if (__builtin_amdgcn_ballot_w64(bad) != 0) paged_row<kBF16>(a, row, kvh, head, span);
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) paged_row<kBF16, kTileWaves>(a, row, kvh, head0 + r, span, lds);
     }
   }
 }
@@ -656,7 +673,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
   }
   if constexpr (!kFp8) {
     __syncthreads();   // (a share may have no round and so no barrier since the flag was cleared)
-    if (__builtin_amdgcn_readfirstlane(deal->again) != 0) paged_again<kBF16, kQT>(a, deal);
+    if (__builtin_amdgcn_readfirstlane(deal->again) != 0) paged_again<kBF16, kQT>(a, deal, reinterpret_cast<float*>(smem));
   }
 }
 
@@ -668,7 +685,7 @@ __device__ __forceinline__ void paged_attn(const PagedArgs& a, uint8_t* smem, fl
 // the waves left over take the next query heads (blockIdx.y: groups of 8 / split).
 constexpr int kJoinWaves = 8;
 template <bool kBF16, int kQT>
-__device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float* lds) {
+__device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float* lds, int32_t* again) {
   const int heads = a.kv_heads * a.head_groups;
   const int row = blockIdx.x / heads, unit = blockIdx.x - row * heads;
   const int kvh = unit / a.head_groups, hg = unit - kvh * a.head_groups;
@@ -732,29 +749,36 @@ __device__ __forceinline__ void paged_join(const PagedArgs& a, int split, float*
 #pragma unroll
     for (int i = 0; i < 4; ++i) lds[2 * kJoinWaves + 256 * wave + 64 * i + lane] = acc[i];
     __syncthreads();
-    if (part0 != 0) return;
-    for (int w = wave; w < wave + split; ++w) top = __builtin_fmaxf(top, lds[2 * w]);
-    all = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-    for (int w = wave; w < wave + split; ++w) {
-      const float f = lds[2 * w] == -__builtin_inff() ? 0.0f : exp2_fast(lds[2 * w] - top);
-      all += f * lds[2 * w + 1];
+    if (part0 == 0) {
+      for (int w = wave; w < wave + split; ++w) top = __builtin_fmaxf(top, lds[2 * w]);
+      all = acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+      for (int w = wave; w < wave + split; ++w) {
+        const float f = lds[2 * w] == -__builtin_inff() ? 0.0f : exp2_fast(lds[2 * w] - top);
+        all += f * lds[2 * w + 1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] += f * lds[2 * kJoinWaves + 256 * w + 64 * i + lane];
+        for (int i = 0; i < 4; ++i) acc[i] += f * lds[2 * kJoinWaves + 256 * w + 64 * i + lane];
+      }
     }
   }
-  if (!in) return;
-  const float f = top == -__builtin_inff() ? 0.0f : a.v_scale / all;
-  float z = 0.0f;   // (dims past the head's: zeros)
+  bool bad = false;   // (codes of e4m3 have no Inf)
+  if (in && part0 == 0) {
+    const float f = top == -__builtin_inff() ? 0.0f : a.v_scale / all;
+    float z = 0.0f;   // (dims past the head's: zeros)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[i] * f, 0.0f, z);
-  if (!a.e4m3 && finite_sum(all) && __builtin_amdgcn_ballot_w64(!(z == 0.0f)) != 0) {
-    paged_row<kBF16>(a, row, kvh, kvh * a.group + hg * 16 * kQT + r, span);
-    return;
+    for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[i] * f, 0.0f, z);
+    bad = !a.e4m3 && finite_sum(all) && __builtin_amdgcn_ballot_w64(!(z == 0.0f)) != 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!bad && lane + 64 * i < a.d) o[lane + 64 * i] = kBF16 ? bf16_rne(acc[i] * f) : f16_rne(acc[i] * f);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < a.d)
-      o[lane + 64 * i] = kBF16 ? bf16_rne(acc[i] * f) : f16_rne(acc[i] * f);
+  if (a.e4m3) return;
+  if (lane == 0) again[wave] = bad;
+  __syncthreads();
+  uint64_t waves = __builtin_amdgcn_ballot_w64(lane < kJoinWaves && again[lane & (kJoinWaves - 1)] != 0);
+  for (; waves != 0; waves &= waves - 1) {
+    const int head = blockIdx.y * (kJoinWaves / split) + __builtin_ctzll(waves) / split;
+    paged_row<kBF16, kJoinWaves>(a, row, kvh, kvh * a.group + hg * 16 * kQT + head, span, lds);
+  }
 }
 
 }  // namespace
@@ -786,7 +810,8 @@ SILE_PAGED_DIM(256, 1, 1)
 #define SILE_PAGED_JOIN(NAME, BF, QT)                                             \
   extern "C" __global__ __launch_bounds__(64 * kJoinWaves) void NAME(PagedArgs a, int split) { \
     __shared__ float lds[(2 + 256) * kJoinWaves];                                 \
-    paged_join<BF, QT>(a, split, lds);                                            \
+    __shared__ int32_t again[kJoinWaves];                                         \
+    paged_join<BF, QT>(a, split, lds, again);                                         \
   }
 SILE_PAGED_JOIN(sile_paged_attn_join_f16_q1, false, 1)
 SILE_PAGED_JOIN(sile_paged_attn_join_bf16_q1, true, 1)

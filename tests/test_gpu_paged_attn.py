@@ -386,3 +386,34 @@ def test_values_that_are_not_finite(hip, dtype, lengths, hq, hkv, d, page, windo
             same = (got[i, h] == ref) | (np.isnan(got[i, h]) & np.isnan(ref))
             assert (same | (np.isfinite(ref) & (err <= bound))).all(), (i, h, got[i, h][:8], ref[:8])
             assert lengths[i] == 0 or np.isinf(ref).any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("hq,hkv,d,page", [(2, 1, 64, 16), (40, 2, 72, 4), (5, 1, 256, 32)])
+def test_values_that_are_not_finite_in_some_of_many_rows(hip, dtype, hq, hkv, d, page):
+    """Several whole rows a workgroup, every third with an Inf in V, every seventh with a NaN in
+    K (which makes all of the row's head NaN), beside one that is dealt out."""
+    lengths = [int(n) for n in rng(25).integers(0, 50, 400)]
+    lengths[100] = 3000
+    case = Case(25, dtype, lengths, hq, hkv, d, page)
+    views = [pool.reshape(case.num, hkv, page, d) for pool in case.pools]
+    for i, n in enumerate(lengths):
+        for which, every, dim, bits in ((1, 3, i % d, INF16[dtype]), (0, 7, 1, NAN16[dtype])):
+            if n and i % every == 1:
+                h, j = i % hkv, i % n
+                views[which][case.tables[i, j // page], h, j % page, dim] = bits
+                case.kv[i][which][h, j, dim] = as_f32(np.array([bits], np.uint16), dtype)[0]
+    say(f"paged attn Inf in V of some of 400 rows {dtype} {hq}/{hkv} d={d} page={page}")
+    case.upload(hip)
+    case.run(hip)
+    got = as_f32(case.result(hip), dtype).astype(np.float64)
+    infs = 0
+    for i in range(case.b):
+        for h in range(hq):
+            with np.errstate(invalid="ignore"):
+                ref, bound = case.reference(i, h)
+                err = np.abs(got[i, h] - ref)
+            same = (got[i, h] == ref) | (np.isnan(got[i, h]) & np.isnan(ref))
+            assert (same | (np.isfinite(ref) & (err <= bound))).all(), (i, h, got[i, h][:8], ref[:8])
+            infs += int(np.isinf(ref).any())
+    assert infs > 100
