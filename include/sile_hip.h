@@ -452,12 +452,15 @@ int sile_hip_flash_attn_fwd(sile_dtype dtype, int64_t batch, int64_t heads, int6
  * >= q_start + q_len is plain causal attention.  A query that sees no key gives zeros;
  * what lies in keys it does not see never reaches it, NaN and Inf included.  head_dim a
  * multiple of 8 up to 256 with 16-byte aligned operands and scale > 0 runs on the matrix
- * cores (the probabilities enter the second product in 16 bits; a row's rounding can depend on
+ * cores (the probabilities enter the second product in 16 bits, also where head_dim is an odd
+ * multiple of 8 and sile_hip_flash_attn_fwd keeps 16 bits more; a row's rounding can depend on
  * the shape of the call); others on a VALU kernel of one wave per query row.  A row
  * whose result is not finite, or meets Inf or NaN in V of a masked key of its block, is
  * taken again row by row: right, but slow.  q_start + q_len and kv_len <= 2^29, one head's
  * K at most 2^31 - 1 bytes, batch * q_heads * q_len < 2^31 (on the matrix cores some 2^24 blocks
- * of 32 to 128 query rows of one key head; more key heads take more launches).  Its form for single tokens: sile_hip_paged_attn_decode.
+ * of 32 to 128 query rows of one key head; more key heads take more launches).  Its form for
+ * single tokens: sile_hip_paged_attn_decode.  It reads contiguous keys only: a prompt taken in
+ * pieces keeps its keys contiguous beside the pages.
  * No reference counterpart, as sile_hip_flash_attn_fwd. */
 int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_heads,
                                    int64_t kv_heads, int64_t q_len, int64_t kv_len,
@@ -475,10 +478,11 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
  *   tables   int32 [n_rows][ld_table] page numbers, a row a sequence; token
  *            j of row r lies in page tables[r][j / page_size], slot
  *            j % page_size; a number outside [0, num_pages) names no page
- *   lengths  int32 [n_rows] tokens of the rows
+ *   lengths  int32 [n_rows] tokens of the rows: below 0 counts as 0, past what
+ *            the table's width holds as that
  *   refs     int32 [num_pages] table entries that hold the page; <= 0: free
- * Page numbers, lengths and positions are looked at on the device only: one
- * outside its range names nothing, and nothing is read or written for it.
+ * Page numbers, lengths and positions are looked at on the device only: a page or
+ * a position outside its range names nothing, and nothing is read or written for it.
  * At most 2^22 rows; the entries of a table and the pages each below 2^31.
  * All calls only enqueue, on the current device, and can be captured into a
  * graph (they are plain kernel launches); the same workspace serves calls
@@ -489,8 +493,9 @@ int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_he
 /* Stores n_tokens new tokens: K's rows k + t * ldk and V's v + t * ldv, each
  * [kv_heads][head_dim] (so both may point into one fused projection), at position
  * positions[t] of row rows[t] (rows NULL: row t).  dtype f16 or bf16; cache_type the
- * same (head_dim a multiple of 8), or f8e4m3 (a multiple of 16): x / scale to nearest
- * even, saturating at 448, NaN kept.  head_dim <= 256; k, v 16-byte aligned,
+ * same (head_dim a multiple of 8), or f8e4m3 (a multiple of 16): x / scale as an
+ * fp32 quotient, and that to the nearest code (even on a tie), saturating at 448, NaN
+ * kept.  head_dim <= 256; k, v 16-byte aligned,
  * ldk, ldv multiples of 8.  A token whose row, position or page does not exist is
  * left out.  Two tokens of one position: each 16 bytes are one of theirs. */
 int sile_hip_kv_append(sile_dtype dtype, sile_dtype cache_type, int64_t n_tokens, int64_t kv_heads,
@@ -568,8 +573,9 @@ int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_hea
  * window > 0 only j >= len - window or j < sinks (the token is at position len - 1 and
  * its own key is in the cache).  q[b], o[b] at q + b * ldq, o + b * ldo, [q_heads][head_dim],
  * f16 or bf16, 16-byte aligned, ldq and ldo multiples of 8.  The cache as for
- * sile_hip_kv_append; an f8e4m3 one holds k / k_scale and v / v_scale (1 otherwise).  A key whose page does not
- * exist counts as unseen; a row without any seen key gives zeros; what lies in
+ * sile_hip_kv_append; an f8e4m3 one holds k / k_scale and v / v_scale (pass 1 for another, which
+ * holds k and v).  A key whose page does not exist counts as unseen; a row without
+ * any seen key gives zeros; what lies in
  * unseen slots never reaches a result, NaN and Inf included.  fp32 throughout
  * but for the products' operands, where the probabilities are two 16-bit parts; a query
  * head that meets Inf or NaN in V of a key it sees is taken again with fp32 ones by one

@@ -4,11 +4,13 @@
 //   O = softmax(Q K^T * scale + mask) V    Q, O [B, Hq, Sq, D]   K, V [B, Hk, Sk, D]
 //   query i, at position p = start + i, sees key j <= p with j > p - window or j < sinks
 //
-// The matrix cores bound it: 4 D flop for each seen pair, and the keys of a window are
-// read again for every block of queries, out of the L2.  The pipeline is that of the
-// causal kernel (flash_attn.hip): a workgroup of 4 waves, two of them a CU up to D = 128, takes 32 queries a wave;
-// K and V blocks go from memory to LDS by LDS-DMA, two stages of each; iteration j
-// issues S_{j+1} = K_{j+1} Q^T and O^T += V_{j-1}^T P_{j-1} on the matrix cores beside
+// Its work is the matrix cores', 4 D flop for each seen pair, and the keys of a window are
+// read again for every block of queries, out of the L2; but they are not what holds it (39 % busy at
+// 2.1 GHz in the first case measured below, the causal kernel's 55 % at 1.78): a block of queries
+// has few rounds of keys, each with its barrier, around a start and an end of some 5 us.  The
+// pipeline is that of the causal kernel (flash_attn.hip): a workgroup of 4 waves, two of them a
+// CU up to D = 128, takes 32 queries a wave; K and V blocks go from memory to LDS by
+// LDS-DMA, two stages of each; iteration j issues S_{j+1} = K_{j+1} Q^T and O^T += V_{j-1}^T P_{j-1} on the matrix cores beside
 // the online softmax of S_j, whose accumulator holds one query a lane; V^T is read
 // with ds_read_b64_tr_b16.  What the window changes:
 //
@@ -34,9 +36,11 @@
 // dealt to groups of the waves of a workgroup of 8, which join their (m, l, O) at the end.
 //
 // Measured: 8192 queries, 32 heads of 128 over 8 key heads, window 1024 and 4 sinks: 154 - 169 us by
-// card (765 - 840 TFLOP/s of seen pairs, MFMA 39 % and softmax VALU 34 % of the cycles at 2.1 GHz);
-// window 4096 on the slowest of these cards 413 (1000); 2 x 512 queries x 16 heads behind 7680 keys,
-// window 4096, 45 - 49.
+// card (765 - 840 TFLOP/s of seen pairs; MFMA 39 %, VALU 34 % of the cycles; of the waves' 40 %
+// wait to issue, 27 % for data or a barrier); window 4096 381 - 413 (1000 - 1080); heads of 64, window
+// 1024, 96 - 98 (670); 4096 queries, heads of 192 and 256, window 1024, 168 (540) and 207 (580); 2 x
+// 4096 queries, 32 heads of 96, window 256, 60 (415); 2 x 512 queries x 16 heads behind 7680 keys,
+// window 4096, 45 - 49 (740).
 //
 // The head dimension is rounded up to kDh (32, 64, 96, 128, 192 or 256): the chunks of a
 // row past D are loaded as zeros and its O^T rows past D are not stored.

@@ -536,15 +536,18 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   // A workgroup a unit, in one launch, where a unit is short (what the table's width or the
   // window allows, as the lengths stand on the device): up to 512 keys in any case, up to 2048
   // (1024 of 256 16-bit dims) where there is a unit for every CU.  Us a call, dealt and so, 8
-  // key heads of 128: 1 x 256 keys 9.9, 7.3; 1 x 512 10.2, 9.1; 1 x 1024 10.7, 13.3; 32 x 1024
-  // 35, 27; 128 x 1024 99, 94; 32 x 2048 58, 49; 8 x 2048 21.3, 22.9; 4 of 256, 64 x 2000 56,
-  // 71.  Past that a single long row among short ones would keep its workgroups alone for long.
+  // key heads of 128: 1 x 256 keys 10.7, 6.9; 1 x 512 10.9, 9.2; 1 x 1024 10.8, 13.3; 32 x 1024
+  // 30.6, 23.5; 128 x 1024 90.6, 84.2; 32 x 2048 53.3, 44.7; 8 x 2048 22.1, 22.9; 4 of 256, 64 x
+  // 2000 56, 71.  (A table wider than its rows takes the first of each.)  Past that a single
+  // long row among short ones would keep its workgroups alone for long.
   a.direct = (seen <= 512 || (seen <= 2048 && seen * head_dim * es <= (1 << 19) && units >= plan.cus));
   const int32_t grid = a.direct ? (int32_t)units : sile::deal_workgroups(batch * row_tiles, a.groups);
   rc = launch(Module::kPagedAttn, name, dim3((unsigned)grid), dim3(256), params, s);
   if (rc != SILE_OK || a.direct) return rc == SILE_OK ? ok() : rc;
-  // a unit has at most about grid / units parts (and one or two more): up to 16 for one wave,
-  // two rounds of eight, then more waves
+  // Units of one length have about grid / units parts (and one or two more): up to 16 for one
+  // wave, two rounds of eight, then more waves.  A long row among short ones has more than that and
+  // is joined by as few waves: one row of 100000 keys, 8 key heads of 128, takes 74 us alone, 89
+  // beside 63 rows of 100.
   const int64_t heads = std::min<int64_t>(a.group, 16 * plan.q_tiles);
   const int64_t parts = grid / units + 2;
   int split = parts <= 16 ? 1 : parts <= 32 ? 2 : parts <= 64 ? 4 : 8;
