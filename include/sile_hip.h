@@ -572,18 +572,18 @@ int sile_hip_paged_attn_workspace(int64_t batch, int64_t q_heads, int64_t kv_hea
  * over the keys j < len of row b's pages, of key head h / (q_heads / kv_heads); with
  * window > 0 only j >= len - window or j < sinks (the token is at position len - 1 and
  * its own key is in the cache).  q[b], o[b] at q + b * ldq, o + b * ldo, [q_heads][head_dim],
- * f16 or bf16, 16-byte aligned, ldq and ldo multiples of 8.  The cache as for
- * sile_hip_kv_append; an f8e4m3 one holds k / k_scale and v / v_scale (pass 1 for another, which
- * holds k and v).  A key whose page does not exist counts as unseen; a row without
- * any seen key gives zeros; what lies in
- * unseen slots never reaches a result, NaN and Inf included.  fp32 throughout
- * but for the products' operands, where the probabilities are two 16-bit parts; a query
- * head that meets Inf or NaN in V of a key it sees is taken again with fp32 ones by one
- * workgroup: as the formula says, but slow.  One call takes at
- * most 2^22 units (a row's key head with up to 16 or 32 query heads of it) and, of the table's
- * width or the window, some 2^36 keys over all units.
+ * f16 or bf16, 16-byte aligned, ldq and ldo multiples of 8; o overlaps nothing that the
+ * call reads.  The cache as for sile_hip_kv_append; an f8e4m3 one holds k / k_scale and
+ * v / v_scale (pass 1 for another, which holds k and v).  A key whose page does not exist
+ * counts as unseen; a row without any seen key gives zeros; what lies in unseen slots
+ * never reaches a result, NaN and Inf included.  fp32 throughout but for the products'
+ * operands, where the probabilities are two 16-bit parts; a query head that meets Inf or
+ * NaN in V of a key it sees is taken again with fp32 ones by one workgroup: as the formula
+ * says, but slow.
  * A row's keys may be split over workgroups, by the lengths of all rows, so its
- * rounding can depend on the batch; the same call gives the same bits. */
+ * rounding can depend on the batch; the same call gives the same bits.  One call takes at
+ * most 2^22 units (a row's key head with up to 16 or 32 query heads of it) and, of the
+ * table's width or the window, some 2^36 keys over all units. */
 int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t batch,
                                int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void *q,
                                int64_t ldq, const void *k_pages, const void *v_pages,

@@ -417,3 +417,32 @@ def test_values_that_are_not_finite_in_some_of_many_rows(hip, dtype, hq, hkv, d,
             assert (same | (np.isfinite(ref) & (err <= bound))).all(), (i, h, got[i, h][:8], ref[:8])
             infs += int(np.isinf(ref).any())
     assert infs > 100
+
+
+@pytest.mark.parametrize("lengths", [[1, 40, 300], [3000, 2, 700]])
+@pytest.mark.parametrize("page", [8, 32])
+def test_nan_codes(hip, lengths, page):
+    """An e4m3 cache (which has no Inf): NaN in V stays in its dimension, NaN in K takes its key
+    head's row."""
+    case = Case(26, "bf16", lengths, 6, 2, 64, page, fp8=True)
+    kp, vp = (pool.reshape(case.num, 2, page, 64) for pool in case.pools)
+    for i, n in enumerate(lengths):
+        j = n // 2
+        at = case.tables[i, j // page]
+        vp[at, 0, j % page, 5] = 0xFF
+        case.kv[i][1][0, j, 5] = np.nan
+        if i == 1:
+            kp[at, 1, j % page, 9] = 0x7F
+    say(f"paged attn NaN codes {lengths} page={page}")
+    case.upload(hip)
+    case.run(hip)
+    got = as_f32(case.result(hip), "bf16").astype(np.float64)
+    for i in range(case.b):
+        for h in range(6):
+            if i == 1 and h >= 3:
+                assert np.isnan(got[i, h]).all()
+                continue
+            ref, bound = case.reference(i, h)
+            assert (np.isnan(got[i, h]) == np.isnan(ref)).all() and np.isnan(ref).sum() == (h < 3), (i, h)
+            ok = ~np.isnan(ref)
+            assert (np.abs(got[i, h] - ref)[ok] <= bound[ok]).all(), (i, h)
