@@ -57,6 +57,20 @@ typedef enum {
 /* Row reduce ops: TileIrOp::ReduceMax / ReduceSum (crates/sile-tile-ir/src/ir.rs:128-262). */
 typedef enum { SILE_REDUCE_MAX = 0, SILE_REDUCE_SUM = 1 } sile_reduce_op;
 
+/* Which dims of a head a rotation turns together: j and rot_dim / 2 + j, or 2 j and 2 j + 1. */
+typedef enum { SILE_ROPE_HALF = 0, SILE_ROPE_PAIRS = 1 } sile_rope_layout;
+
+/* How sile_hip_rope_turns stretches positions over a longer context. */
+typedef enum {
+  SILE_ROPE_UNSCALED = 0,
+  SILE_ROPE_LINEAR = 1, /* every pair turns 1 / factor as fast */
+  SILE_ROPE_BASE = 2,   /* the base grows by factor^(rot_dim / (rot_dim - 2)): the slowest pair as LINEAR, the first as is */
+  SILE_ROPE_TURNS = 3,  /* pairs with at least `high` turns over the original length as they are, those with at most `low`
+                           as LINEAR, linearly in the turns between */
+  SILE_ROPE_DIMS = 4    /* the same between the pairs that have `high` and `low` turns (rounded outwards), linearly in
+                           their number */
+} sile_rope_scaling;
+
 typedef void *sile_hip_stream;   /* hipStream_t */
 typedef void *sile_hip_event;    /* hipEvent_t */
 typedef void *sile_hip_module;   /* hipModule_t */
@@ -592,6 +606,91 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
                                void *o, int64_t ldo, float scale, float k_scale, float v_scale,
                                int64_t window, int64_t sinks, void *workspace,
                                size_t workspace_bytes, sile_hip_stream stream);
+
+/* ---- a serving step around the cache: tokens, positions, norms, answers -------
+ * No counterparts in the reference, as the cache above.  All only enqueue, on the current
+ * device, and can be captured into a graph (they are plain kernel launches). */
+
+/* The token list of a step over n_rows (at most 65536) rows, each with need[r] new tokens
+ * behind its lengths[r] (both: below 0 counts as 0), none where granted is given and
+ * granted[r] == 0 (as sile_hip_kv_reserve leaves it): row r's are starts[r] .. starts[r + 1] - 1
+ * of the list, in the rows' order, with rows[t] = r and positions[t] = lengths[r] + t - starts[r];
+ * starts [n_rows + 1], rows and positions [max_tokens], from the last token on -1, which
+ * every call here that takes them passes over.  lengths_out[r] = lengths[r] + its tokens.
+ * Tokens past max_tokens, and past position 2^31 - 2, are left out.  No array overlaps another
+ * that the call writes. */
+int sile_hip_kv_slots(int64_t n_rows, const int32_t *lengths, const int32_t *need,
+                      const int32_t *granted, int64_t max_tokens, int32_t *starts, int32_t *rows,
+                      int32_t *positions, int32_t *lengths_out, sile_hip_stream stream);
+
+/* Turns a position of the pairs j < rot_dim / 2, into the HOST array `turns`:
+ * base^(-2 j / rot_dim) / (2 pi), changed as `scaling` says.  original, low and high only
+ * for the last two (0 < low < high).  Needs no GPU. */
+int sile_hip_rope_turns(sile_rope_scaling scaling, int64_t rot_dim, double base, double factor,
+                        double original, double low, double high, double *turns);
+
+/* Rotary positions: pair j < rot_dim / 2 of every head of token t is turned by the angle
+ * x = 2 pi turns[j] positions[t] (turns: device, 64 bits, kept there to its fraction of a turn),
+ *   (a, b) -> magnitude * (a cos x - b sin x, b cos x + a sin x),
+ * and dims from rot_dim on are copied; fp32, rounded once.  Negative turns turn back.  dtype f32, f16
+ * or bf16; tokens at q + t * ldq, k + t * ldk, [heads][head_dim], any alignment and head_dim up to
+ * 2048 (16-byte aligned and rot_dim a multiple of 16 is fastest); q_heads or kv_heads may be
+ * 0.  An output is its input (same pointer and leading dimension) or apart from it.  A token
+ * at a position below 0 is left out: its outputs stay as they are. */
+int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, int64_t q_heads,
+                  int64_t kv_heads, int64_t head_dim, int64_t rot_dim, const void *q, int64_t ldq,
+                  void *q_out, int64_t ldqo, const void *k, int64_t ldk, void *k_out, int64_t ldko,
+                  const int32_t *positions, const double *turns, float magnitude,
+                  sile_hip_stream stream);
+
+/* sile_hip_rope of the queries, and sile_hip_kv_append of the rotated keys and of the values, in
+ * one launch: the keys are rounded once, to the cache's type (e4m3: k / scale of the fp32
+ * result).  Arguments and what is left out as for the two; a token without a page in the
+ * cache still has its queries turned. */
+int sile_hip_rope_append(sile_dtype dtype, sile_dtype cache_type, sile_rope_layout layout,
+                         int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                         int64_t rot_dim, const void *q, int64_t ldq, void *q_out, int64_t ldqo,
+                         const void *k, int64_t ldk, const void *v, int64_t ldv,
+                         const int32_t *rows, const int32_t *positions, const double *turns,
+                         float magnitude, void *k_pages, void *v_pages, int64_t num_pages,
+                         int64_t page_size, int64_t page_stride, const int32_t *tables,
+                         int64_t n_rows, int64_t ld_table, float k_scale, float v_scale,
+                         sile_hip_stream stream);
+
+/* Row norm: s = x + residual (residual NULL: x), y = s / sqrt(mean(s^2) + eps) * weight
+ * (NULL: 1; one value a column) of a [rows, cols] matrix, fp32; s goes on unrounded, and to `sum`
+ * (may be NULL) rounded.  in_type f32, f16, bf16 for x, residual, sum and weight; out_type the
+ * same, or f8e4m3: codes of y / scale (fp32 quotient, nearest code, saturating at 448, NaN kept) with
+ * scale as given (group 0), or worked out for each `group` columns (a divisor of cols; cols: one a
+ * row) as max |y| / 448, the maximum at least 2^-100, and stored in scales [rows][cols / group].
+ * sum may be x or residual, and y (of in_type) x or residual, with the same leading
+ * dimension; else outputs overlap nothing.  A row with a NaN gives NaN; with an Inf NaN
+ * there and 0 elsewhere, as the formula.  Fastest: cols a multiple of 8 up to 16384, rows 16-byte
+ * aligned, group 0, cols or a power of two from 8 to 512. */
+int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows, int64_t cols,
+                          const void *x, int64_t ldx, const void *residual, int64_t ldr, void *sum,
+                          int64_t lds, const void *weight, float eps, void *y, int64_t ldy,
+                          float scale, float *scales, int64_t group, sile_hip_stream stream);
+
+/* Workspace bytes that sile_hip_logprobs_rows needs on the current device (0: none). */
+int sile_hip_logprobs_workspace(int64_t rows, int64_t cols, int64_t top_k, size_t *bytes);
+
+/* Of each row x[r] of logits (f32, f16, bf16; any ldx >= cols), with p = softmax(scale * x[r])
+ * (scale: one over a temperature), fp32:
+ *   logp[r]      log p of column targets[r]; 0 for a target outside [0, cols)
+ *   entropy[r]   - sum p log p
+ *   top_ids[r], top_logp[r]   [top_k], the columns of the largest x, largest first, of equal
+ *                ones the lowest first, and their log p; top_k at most 64
+ * logp and entropy may be NULL, and top_k 0.  Columns of -inf have log p -inf and are never among
+ * the top ones: where fewer than top_k are left the rest is -1 with -inf.  A row of nothing else:
+ * logp and top_logp -inf, entropy 0.  A NaN or +inf makes the row's numbers NaN; its top_ids are
+ * those of the comparisons (+inf first, NaN never).  A row's chunks may be shared out over
+ * workgroups, by rows and cols, so its rounding can depend on both; the same call gives the same
+ * bits. */
+int sile_hip_logprobs_rows(sile_dtype in_type, int64_t rows, int64_t cols, const void *x,
+                           int64_t ldx, float scale, const int32_t *targets, float *logp,
+                           float *entropy, int64_t top_k, float *top_logp, int32_t *top_ids,
+                           void *workspace, size_t workspace_bytes, sile_hip_stream stream);
 
 /* ---- pattern router: Tile IR -> hand-written kernels ---------------------
  * Generalises the reference's canonical-matmul detector

@@ -29,6 +29,8 @@ STATUS_NAMES = {
 F32, F16, BF16, F8E4M3 = 0, 1, 2, 3
 ROW_MAJOR, COL_MAJOR = 0, 1
 REDUCE_MAX, REDUCE_SUM = 0, 1
+ROPE_HALF, ROPE_PAIRS = 0, 1
+ROPE_UNSCALED, ROPE_LINEAR, ROPE_BASE, ROPE_TURNS, ROPE_DIMS = range(5)
 
 _DTYPE_BYTES = {F32: 4, F16: 2, BF16: 2, F8E4M3: 1}
 
@@ -46,6 +48,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 _SZ = ctypes.c_size_t
 
 
@@ -169,6 +172,17 @@ SIGNATURES = {
     "sile_hip_paged_attn_decode": [_I32, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _I64,
                                    _I64, _P, _I64, _P, _P, _I64, _F32, _F32, _F32, _I64, _I64, _P,
                                    _SZ, _P],
+    "sile_hip_kv_slots": [_I64, _P, _P, _P, _I64, _P, _P, _P, _P, _P],
+    "sile_hip_rope_turns": [_I32, _I64, _F64, _F64, _F64, _F64, _F64, _P],
+    "sile_hip_rope": [_I32, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
+                      _P, _P, _F32, _P],
+    "sile_hip_rope_append": [_I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P,
+                             _I64, _P, _I64, _P, _P, _P, _F32, _P, _P, _I64, _I64, _I64, _P, _I64, _I64,
+                             _F32, _F32, _P],
+    "sile_hip_rmsnorm_rows": [_I32, _I32, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _F32, _P, _I64,
+                              _F32, _P, _I64, _P],
+    "sile_hip_logprobs_workspace": [_I64, _I64, _I64, ctypes.POINTER(_SZ)],
+    "sile_hip_logprobs_rows": [_I32, _I64, _I64, _P, _I64, _F32, _P, _P, _P, _I64, _P, _P, _P, _SZ, _P],
     "sile_hip_tile_ir_route": [ctypes.c_char_p, _P, _I64, _I64, ctypes.POINTER(Route)],
     "sile_hip_tile_ir_launch": [ctypes.POINTER(Route), _P, _I64, _P, _I64, _I64, _P],
 }
@@ -586,6 +600,59 @@ def paged_attn_decode(dtype, cache_type, batch, q_heads, kv_heads, head_dim, q, 
     call("sile_hip_paged_attn_decode", dtype, cache_type, batch, q_heads, kv_heads, head_dim, q, ldq,
          k_pages, v_pages, num_pages, page_size, page_stride, tables, ld_table, lengths, o, ldo,
          scale, k_scale, v_scale, window, sinks, workspace or None, workspace_bytes, _sh(stream))
+
+
+# ---------------------------------------------------------------------------
+# a serving step around the cache (asynchronous on the stream)
+# ---------------------------------------------------------------------------
+
+def kv_slots(n_rows, lengths, need, granted, max_tokens, starts, rows, positions, lengths_out,
+             stream=None):
+    call("sile_hip_kv_slots", n_rows, lengths, need, granted or None, max_tokens, starts, rows,
+         positions, lengths_out, _sh(stream))
+
+
+def rope_turns(scaling, rot_dim, base, factor=1.0, original=0.0, low=0.0, high=0.0) -> np.ndarray:
+    """Turns a position of each rotated pair, float64 [rot_dim / 2] (host; needs no GPU)."""
+    out = np.zeros(max(rot_dim, 0) // 2, np.float64)
+    call("sile_hip_rope_turns", scaling, rot_dim, base, factor, original, low, high, out.ctypes.data)
+    return out
+
+
+def rope(dtype, layout, n_tokens, q_heads, kv_heads, head_dim, rot_dim, q, ldq, q_out, ldqo, k, ldk,
+         k_out, ldko, positions, turns, magnitude=1.0, stream=None):
+    call("sile_hip_rope", dtype, layout, n_tokens, q_heads, kv_heads, head_dim, rot_dim, q or None, ldq,
+         q_out or None, ldqo, k or None, ldk, k_out or None, ldko, positions, turns, magnitude,
+         _sh(stream))
+
+
+def rope_append(dtype, cache_type, layout, n_tokens, q_heads, kv_heads, head_dim, rot_dim, q, ldq, q_out,
+                ldqo, k, ldk, v, ldv, rows, positions, turns, magnitude, k_pages, v_pages, num_pages,
+                page_size, page_stride, tables, n_rows, ld_table, k_scale=1.0, v_scale=1.0, stream=None):
+    call("sile_hip_rope_append", dtype, cache_type, layout, n_tokens, q_heads, kv_heads, head_dim,
+         rot_dim, q or None, ldq, q_out or None, ldqo, k, ldk, v, ldv, rows or None, positions, turns,
+         magnitude, k_pages, v_pages, num_pages, page_size, page_stride, tables, n_rows, ld_table,
+         k_scale, v_scale, _sh(stream))
+
+
+def rmsnorm_rows(in_type, out_type, rows, cols, x, ldx, residual, ldr, sum_out, lds, weight, eps, y, ldy,
+                 scale=1.0, scales=0, group=0, stream=None):
+    call("sile_hip_rmsnorm_rows", in_type, out_type, rows, cols, x, ldx, residual or None, ldr,
+         sum_out or None, lds, weight or None, eps, y, ldy, scale, scales or None, group, _sh(stream))
+
+
+def logprobs_workspace(rows, cols, top_k) -> int:
+    """Workspace bytes of logprobs_rows on the current device (0: none)."""
+    n = _SZ(0)
+    call("sile_hip_logprobs_workspace", rows, cols, top_k, ctypes.byref(n))
+    return n.value
+
+
+def logprobs_rows(in_type, rows, cols, x, ldx, scale, targets, logp, entropy, top_k, top_logp, top_ids,
+                  workspace=0, workspace_bytes=0, stream=None):
+    call("sile_hip_logprobs_rows", in_type, rows, cols, x, ldx, scale, targets or None, logp or None,
+         entropy or None, top_k, top_logp or None, top_ids or None, workspace or None, workspace_bytes,
+         _sh(stream))
 
 
 def dtype_bytes(t: int) -> int:

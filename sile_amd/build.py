@@ -2,8 +2,8 @@
 
 1. Each kernels/<name>.hip is compiled for gfx950 into a raw ELF code object
    sile_amd/_build/<name>.hsaco (hipcc --genco --no-gpu-bundle-output).
-2. The host runtime (runtime.cpp, ops.cpp, paged.cpp, llir.cpp,
-   tile_ir.cpp) is compiled with g++ against the HIP runtime headers;
+2. The host runtime (runtime.cpp, ops.cpp, paged.cpp, serving.cpp,
+   llir.cpp, tile_ir.cpp) is compiled with g++ against the HIP runtime headers;
    runtime.cpp assembles the code objects into the library image with
    .incbin.  launch_noalloc.hip (host code plus the device array its entry
    point uses) is compiled by hipcc for the host and gfx950.
@@ -30,8 +30,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 KERNELS = ["dsl", "softmax", "gemm", "attention", "flash_attn", "flash_window", "paged_attn",
-           "kv_cache"]
-HOST_SOURCES = ["runtime.cpp", "ops.cpp", "paged.cpp", "llir.cpp", "tile_ir.cpp"]
+           "kv_cache", "rope", "rmsnorm", "logprobs"]
+HOST_SOURCES = ["runtime.cpp", "ops.cpp", "paged.cpp", "serving.cpp", "llir.cpp", "tile_ir.cpp"]
 HIP_HOST_SOURCES = ["launch_noalloc.hip"]
 
 # Device code: gfx950 only; packed-fp32 instructions disabled (the compiler

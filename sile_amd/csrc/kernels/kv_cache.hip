@@ -14,6 +14,7 @@
 // cache take 33 us with plain stores and 24 so (5.5 TB/s), closing up a pool of 4700 pages
 // 39 and 31; loads that way are slower (24 us, 32).
 #include "common.h"
+#include "e4m3.h"
 
 using namespace sile;
 
@@ -35,25 +36,6 @@ struct AppendArgs {
   int32_t heads, d, num_pages, page_shift, n_rows, per_group;   // tokens a workgroup
   float k_scale, v_scale, k_rcp, v_rcp;   // rcp: 1 / scale, 0 for a scale outside [2^-60, 2^60]
 };
-
-// x / scale, correctly rounded, held to e4m3's range; NaN stays NaN.  rcp is 1 / scale,
-// correctly rounded: one correction of x * rcp by its remainder is then the quotient
-// (Markstein), wherever it is neither past the range, where it saturates in any case,
-// nor so small that it rounds to zero, and scale is no extreme; else (rcp = 0) the division
-// (a third of the kernel's instructions: with plain stores, 16382 tokens of 8 heads of 128
-// take 31 us with it and 26 so).
-SILE_DEV float e4m3_in(float x, float scale, float rcp) {
-  float y;
-  if (rcp == 0.0f) {
-    y = x / scale;
-  } else {
-    const float q = x * rcp;
-    const float exact = __builtin_fmaf(__builtin_fmaf(-q, scale, x), rcp, q);
-    const float m = __builtin_fabsf(q);
-    y = m < 1024.0f && m > 0x1p-12f ? exact : q;   // (outside: the range's end, or a zero of q's sign)
-  }
-  return y != y ? y : __builtin_amdgcn_fmed3f(y, -448.0f, 448.0f);
-}
 
 // A workgroup takes per_group tokens (K's and V's rows of all heads: `each` chunks
 // of 16 bytes of the cache), a thread one chunk at a time.  kIn: 0 the type as it
@@ -94,14 +76,113 @@ SILE_DEV void append(const AppendArgs& a) {
           f[j] = e4m3_in(kIn == 1 ? f16_to_f32(b) : bf16_to_f32(b), scale, rcp);
         }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          int code = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j], f[4 * j + 1], 0, false);
-          code = __builtin_amdgcn_cvt_pk_fp8_f32(f[4 * j + 2], f[4 * j + 3], code, true);
-          out[2 * h + j] = (uint32_t)code;
-        }
+        for (int j = 0; j < 2; ++j) out[2 * h + j] = e4m3_pack4(f + 4 * j);
       }
       __builtin_nontemporal_store(out, reinterpret_cast<u32x4_t*>((is_v ? a.v_pages : a.k_pages) + at));
     }
+  }
+}
+
+// ---- a step's tokens ----
+
+struct SlotsArgs {
+  const int32_t* lengths;
+  const int32_t* need;
+  const int32_t* granted;   // NULL: every row
+  int32_t* starts;
+  int32_t* rows;
+  int32_t* positions;
+  int32_t* lengths_out;
+  int32_t n_rows, tokens;
+};
+constexpr int kSlotTokens = 1024;   // of the list, a workgroup
+
+// One launch for a list of any length: every workgroup of 256 adds up the rows' tokens (a
+// run of rows a thread, a scan over the threads; rows up to 65536 are in the L2), marks
+// where the rows of its own 1024 tokens begin, and a running maximum over the marks names
+// each token's row.  Every 256th run of rows (or all, where there is one workgroup) also
+// goes to starts and lengths_out.  Bound by the launch and three dependent reads: 256 rows
+// and 1800 tokens 4 us, 4000 rows and 134000 tokens 8.
+SILE_DEV void slots(const SlotsArgs& a) {
+  __shared__ int64_t wave_sum[4];
+  __shared__ int32_t mark_row[kSlotTokens], mark_base[kSlotTokens];   // by token: row + 1 that begins there, length - start
+  __shared__ int32_t wave_top[4], first_row, first_base;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.n_rows + 255) / 256;
+  const int r0 = min(tid * per, a.n_rows), r1 = min(r0 + per, a.n_rows);
+  const int32_t t0 = blockIdx.x * kSlotTokens;
+  // a row's length, and how many tokens it asks for: no position passes 2^31 - 1
+  auto row = [&](int r, int32_t* length) {
+    const int32_t len = max(a.lengths[r], 0), n = a.granted && a.granted[r] == 0 ? 0 : max(a.need[r], 0);
+    *length = len;
+    return min(n, 0x7fffffff - len);
+  };
+  for (int i = tid; i < kSlotTokens; i += 256) mark_row[i] = 0;
+  int64_t mine = 0;
+  int32_t length;
+  for (int r = r0; r < r1; ++r) mine += row(r, &length);
+  int64_t incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t up = __shfl_up((long long)incl, off);
+    if (lane >= off) incl += up;
+  }
+  if (lane == 63) wave_sum[wave] = incl;
+  __syncthreads();
+  int64_t at = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) at += wave_sum[w];
+    total += wave_sum[w];
+  }
+  const bool keeps = tid % gridDim.x == blockIdx.x;
+  if (keeps || (at < (int64_t)t0 + kSlotTokens && at + mine > t0))
+    for (int r = r0; r < r1; ++r) {
+      const int32_t n = row(r, &length);
+      const int32_t s = (int32_t)min(at, (int64_t)a.tokens), e = (int32_t)min(at + n, (int64_t)a.tokens);
+      at += n;
+      if (keeps) {
+        a.starts[r] = s;
+        a.lengths_out[r] = length + (e - s);
+      }
+      if (e <= s || e <= t0 || s - t0 >= kSlotTokens) continue;
+      if (s < t0) {   // (one row at most)
+        first_row = r;
+        first_base = length - s;
+      } else {
+        mark_row[s - t0] = r + 1;
+        mark_base[s - t0] = length - s;
+      }
+    }
+  if (blockIdx.x == 0 && tid == 0) a.starts[a.n_rows] = (int32_t)min(total, (int64_t)a.tokens);
+  __syncthreads();
+  // the last mark at or before each of the thread's four tokens
+  int top[4], run = -1;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (mark_row[4 * tid + i] != 0) run = 4 * tid + i;
+    top[i] = run;
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int up = __shfl_up(run, off);
+    if (lane >= off) run = max(run, up);
+  }
+  if (lane == 63) wave_top[wave] = run;
+  int before = __shfl_up(run, 1);
+  if (lane == 0) before = -1;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+    if (w < wave) before = max(before, wave_top[w]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int32_t left = a.tokens - t0, k = 4 * tid + i;
+    if (k >= left) break;
+    const int m = max(top[i], before);
+    const bool there = (int64_t)t0 + k < total;
+    a.rows[t0 + k] = !there ? -1 : m < 0 ? first_row : mark_row[m] - 1;
+    a.positions[t0 + k] = !there ? -1 : t0 + k + (m < 0 ? first_base : mark_base[m]);
   }
 }
 
@@ -200,6 +281,7 @@ SILE_DEV bool wanted(const ReserveArgs& a, int row, int64_t* first, int64_t* las
 
 }  // namespace
 
+extern "C" __global__ __launch_bounds__(256) void sile_kv_slots(SlotsArgs a) { slots(a); }
 extern "C" __global__ __launch_bounds__(256) void sile_kv_append(AppendArgs a) { append<0>(a); }
 extern "C" __global__ __launch_bounds__(256) void sile_kv_append_f16_fp8(AppendArgs a) { append<1>(a); }
 extern "C" __global__ __launch_bounds__(256) void sile_kv_append_bf16_fp8(AppendArgs a) { append<2>(a); }

@@ -1,0 +1,286 @@
+// Row norm by the root of the mean square, with the residual's addition before it and, if
+// asked, an 8-bit output with scales behind it.
+//
+//   s = x + residual     y = s / sqrt(mean(s^2) + eps) * weight     (codes: y / scale)
+//
+// fp32 throughout: s goes into the norm unrounded and is stored rounded once, y is rounded once
+// (to e4m3: to the fp32 quotient and then to the code).  A scale is the given one, or max |y| of
+// each `group` columns over 448 (the maximum counts as at least 2^-100).
+//
+// Every element is read once and written once, so memory bounds it: a row stays in the
+// registers of its threads between the sum and the result.  Rows of up to 512 columns take a
+// wave each, others a workgroup; the weights are read once a workgroup, which goes on to
+// further rows.
+#include "common.h"
+#include "e4m3.h"
+
+using namespace sile;
+
+namespace {
+
+constexpr float kTop = 448.0f;
+constexpr float kLeast = 0x1p-100f;
+
+struct NormArgs {
+  const void *x, *residual, *weight;   // residual, weight: may be NULL
+  void *sum, *y;                       // sum: may be NULL
+  float* scales;                       // group > 0: [rows][cols / group]
+  int64_t rows, ldx, ldr, lds, ldy;
+  int32_t cols, group;
+  float eps, inv_cols, scale, rcp;
+};
+
+template <int kType>   // sile_dtype
+SILE_DEV float load1(const void* p, int64_t i) {
+  if constexpr (kType == 0) return static_cast<const float*>(p)[i];
+  const uint16_t h = static_cast<const uint16_t*>(p)[i];
+  return kType == 1 ? f16_to_f32(h) : bf16_to_f32(h);
+}
+template <int kType>
+SILE_DEV void store1(void* p, int64_t i, float v) {
+  if constexpr (kType == 0)
+    static_cast<float*>(p)[i] = v;
+  else
+    static_cast<uint16_t*>(p)[i] = kType == 1 ? f16_rne(v) : bf16_rne(v);
+}
+
+// 8 elements as they lie in memory
+template <int kType>
+struct Vec {
+  u32x4 w[kType == 0 ? 2 : 1];
+  SILE_DEV void load(const void* p, int64_t i) {
+    const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p) + i * (kType == 0 ? 4 : 2));
+    w[0] = q[0];
+    if constexpr (kType == 0) w[1] = q[1];
+  }
+  SILE_DEV void unpack(float* f) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (kType == 0) {
+        const uint32_t u = w[j >> 2][j & 3];
+        f[j] = bits_f32(u);
+      } else {
+        const uint32_t u = w[0][j >> 1];
+        if constexpr (kType == 2)
+          f[j] = bits_f32((j & 1) ? u & 0xffff0000u : u << 16);
+        else
+          f[j] = f16_to_f32((uint16_t)(u >> (16 * (j & 1))));
+      }
+    }
+  }
+};
+template <int kType>
+SILE_DEV void store8(void* p, int64_t i, const float* f) {
+  if constexpr (kType == 0) {
+    f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + i);
+    q[0] = f32x4{f[0], f[1], f[2], f[3]};
+    q[1] = f32x4{f[4], f[5], f[6], f[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = kType == 1 ? pack_f16x2(f[2 * j], f[2 * j + 1]) : pack_bf16x2(f[2 * j], f[2 * j + 1]);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = w;
+  }
+}
+
+// the sum or maximum over the row's kThreads threads; lds: 2 * 16 floats, used in turn
+template <int kThreads, bool kMax>
+SILE_DEV float row_reduce(float v, float* lds) {
+  v = kMax ? wave_max(v) : wave_sum(v);
+  if constexpr (kThreads == 64) return v;
+  constexpr int kWaves = kThreads / 64;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float r = lds[0];
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) r = kMax ? fmax_ordered(r, lds[w]) : r + lds[w];
+  return r;
+}
+
+// max over groups of `lanes` lanes (a power of two up to 64)
+SILE_DEV float lanes_max(float v, int lanes) {
+  if (lanes >= 2) v = fmax_ordered(v, dpp<kDppXor1>(v));
+  if (lanes >= 4) v = fmax_ordered(v, dpp<kDppXor2>(v));
+  if (lanes >= 8) v = fmax_ordered(v, dpp<kDppHalfMirror>(v));
+  if (lanes >= 16) v = fmax_ordered(v, dpp<kDppMirror>(v));
+  if (lanes >= 32) v = fmax_ordered(v, swizzle_xor16(v));
+  if (lanes >= 64) v = pair32_max(v);
+  return v;
+}
+
+SILE_DEV float scale_of(float top) { return __builtin_fmaxf(top, kLeast) / kTop; }
+SILE_DEV float rcp_of(float scale) { return scale >= 0x1p-60f && scale <= 0x1p60f ? 1.0f / scale : 0.0f; }
+
+// Columns in vectors of 8, all of them aligned: a row takes kThreads threads of kV vectors.
+// kF8: codes out.  kWg: threads of the workgroup.
+template <int kType, bool kF8, int kThreads, int kV, int kWg>
+SILE_DEV void norm_rows(const NormArgs& a) {
+  __shared__ float lds[2][2][16];
+  const int tid = threadIdx.x % kThreads, cols = a.cols;
+  float w[kV][8];
+  Vec<kType> wv[kV];
+#pragma unroll
+  for (int v = 0; v < kV; ++v)
+    if (a.weight && 8 * (v * kThreads + tid) < cols) wv[v].load(a.weight, 8 * (v * kThreads + tid));
+  int turn = 0;
+  constexpr int kRows = kWg / kThreads;
+  for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads; r < a.rows;
+       r += (int64_t)gridDim.x * kRows, turn ^= 1) {
+    Vec<kType> xv[kV], rv[kV];
+#pragma unroll
+    for (int v = 0; v < kV; ++v) {
+      const int c = 8 * (v * kThreads + tid);
+      if (c < cols) {
+        xv[v].load(a.x, r * a.ldx + c);
+        if (a.residual) rv[v].load(a.residual, r * a.ldr + c);
+      }
+    }
+    float s[kV][8], ss = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kV; ++v) {
+      const int c = 8 * (v * kThreads + tid);
+      if (c < cols) {
+        xv[v].unpack(s[v]);
+        if (a.residual) {
+          float f[8];
+          rv[v].unpack(f);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[v][j] += f[j];
+        }
+        if (a.sum) store8<kType>(a.sum, r * a.lds + c, s[v]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[v][j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(s[v][j], s[v][j], ss);
+    }
+    ss = row_reduce<kThreads, false>(ss, lds[0][turn]);
+    const float inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, a.inv_cols, a.eps));
+    float top = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kV; ++v) {
+      const int c = 8 * (v * kThreads + tid);
+      if (a.weight && c < cols) wv[v].unpack(w[v]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[v][j] *= inv;
+        if (a.weight && c < cols) s[v][j] *= w[v][j];
+        if constexpr (kF8) top = __builtin_fmaxf(top, __builtin_fabsf(s[v][j]));
+      }
+    }
+    if constexpr (!kF8) {
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        const int c = 8 * (v * kThreads + tid);
+        if (c < cols) store8<kType>(a.y, r * a.ldy + c, s[v]);
+      }
+    } else {
+      float scale = a.scale, rcp = a.rcp;
+      if (a.group == cols) {
+        scale = scale_of(row_reduce<kThreads, true>(top, lds[1][turn]));
+        rcp = rcp_of(scale);
+        if (tid == 0) a.scales[r] = scale;
+      }
+#pragma unroll
+      for (int v = 0; v < kV; ++v) {
+        const int c = 8 * (v * kThreads + tid);
+        if (a.group != 0 && a.group != cols) {   // 8 to 512 columns: lanes of one wave
+          float m = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = __builtin_fmaxf(m, __builtin_fabsf(s[v][j]));
+          scale = scale_of(lanes_max(m, a.group / 8));
+          rcp = rcp_of(scale);
+          if (c < cols && c % a.group == 0) a.scales[r * (cols / a.group) + c / a.group] = scale;
+        }
+        if (c < cols) {
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = e4m3_in(s[v][j], scale, rcp);
+          const u32x2 out = {e4m3_pack4(f), e4m3_pack4(f + 4)};
+          *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.y) + r * a.ldy + c) = out;
+        }
+      }
+    }
+  }
+}
+
+// Any width, alignment and group: a workgroup of 256 a row, which reads it once for the sum and
+// once more for each pass behind it.  s is kept nowhere: `sum` may be x or the residual itself,
+// so it is written by the last pass, each element by the thread that reads it there.
+template <int kType, bool kF8>
+SILE_DEV void norm_any(const NormArgs& a) {
+  __shared__ float lds[2][2][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int turn = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
+    auto at = [&](int c) {
+      const float v = load1<kType>(a.x, r * a.ldx + c);
+      return a.residual ? v + load1<kType>(a.residual, r * a.ldr + c) : v;
+    };
+    float ss = 0.0f;
+    for (int c = tid; c < a.cols; c += 256) {
+      const float s = at(c);
+      ss = __builtin_fmaf(s, s, ss);
+    }
+    ss = row_reduce<256, false>(ss, lds[0][turn]);
+    const float inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, a.inv_cols, a.eps));
+    auto norm = [&](float s, int c) {
+      s *= inv;
+      return a.weight ? s * load1<kType>(a.weight, c) : s;
+    };
+    auto put = [&](int c, float scale, float rcp) {
+      const float s = at(c), y = norm(s, c);
+      if (a.sum) store1<kType>(a.sum, r * a.lds + c, s);
+      if constexpr (kF8)
+        static_cast<uint8_t*>(a.y)[r * a.ldy + c] = e4m3_code(e4m3_in(y, scale, rcp));
+      else
+        store1<kType>(a.y, r * a.ldy + c, y);
+    };
+    if (!kF8 || a.group == 0) {
+      for (int c = tid; c < a.cols; c += 256) put(c, a.scale, a.rcp);
+    } else if (a.group == a.cols) {
+      float top = 0.0f;
+      for (int c = tid; c < a.cols; c += 256) top = __builtin_fmaxf(top, __builtin_fabsf(norm(at(c), c)));
+      const float scale = scale_of(row_reduce<256, true>(top, lds[1][turn])), rcp = rcp_of(scale);
+      if (tid == 0) a.scales[r] = scale;
+      for (int c = tid; c < a.cols; c += 256) put(c, scale, rcp);
+    } else {   // a wave a group
+      const int groups = a.cols / a.group;
+      for (int g = wave; g < groups; g += 4) {
+        const int c0 = g * a.group, c1 = c0 + a.group;
+        float top = 0.0f;
+        for (int c = c0 + lane; c < c1; c += 64) top = __builtin_fmaxf(top, __builtin_fabsf(norm(at(c), c)));
+        const float scale = scale_of(wave_max(top)), rcp = rcp_of(scale);
+        if (lane == 0) a.scales[r * groups + g] = scale;
+        for (int c = c0 + lane; c < c1; c += 64) put(c, scale, rcp);
+      }
+    }
+  }
+}
+
+}  // namespace
+
+// t<threads of a row>_v<vectors of a thread>; w: four rows a workgroup, a wave each
+#define SILE_NORM(NAME, TYPE, F8, T, V, WG)                                                       \
+  extern "C" __global__ __launch_bounds__(WG) void sile_rmsnorm_##NAME##_t##T##_v##V(NormArgs a) { \
+    norm_rows<TYPE, F8, T, V, WG>(a);                                                             \
+  }
+#define SILE_NORM_TYPES(NAME, TYPE, F8)                                                        \
+  SILE_NORM(NAME, TYPE, F8, 64, 1, 256)                                                        \
+  SILE_NORM(NAME, TYPE, F8, 256, 1, 256)                                                       \
+  SILE_NORM(NAME, TYPE, F8, 256, 2, 256)                                                       \
+  SILE_NORM(NAME, TYPE, F8, 256, 4, 256)                                                       \
+  SILE_NORM(NAME, TYPE, F8, 1024, 1, 1024)                                                     \
+  SILE_NORM(NAME, TYPE, F8, 1024, 2, 1024)                                                     \
+  SILE_NORM(NAME, TYPE, F8, 1024, 4, 1024)                                                     \
+  extern "C" __global__ __launch_bounds__(256) void sile_rmsnorm_##NAME##_any(NormArgs a) {    \
+    norm_any<TYPE, F8>(a);                                                                     \
+  }
+SILE_NORM_TYPES(f32, 0, false)
+SILE_NORM_TYPES(f16, 1, false)
+SILE_NORM_TYPES(bf16, 2, false)
+SILE_NORM_TYPES(f32_fp8, 0, true)
+SILE_NORM_TYPES(f16_fp8, 1, true)
+SILE_NORM_TYPES(bf16_fp8, 2, true)

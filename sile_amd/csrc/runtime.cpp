@@ -44,6 +44,9 @@ SILE_EMBED(sile_co_flash_attn, "flash_attn.hsaco")
 SILE_EMBED(sile_co_paged_attn, "paged_attn.hsaco")
 SILE_EMBED(sile_co_kv_cache, "kv_cache.hsaco")
 SILE_EMBED(sile_co_flash_window, "flash_window.hsaco")
+SILE_EMBED(sile_co_rope, "rope.hsaco")
+SILE_EMBED(sile_co_rmsnorm, "rmsnorm.hsaco")
+SILE_EMBED(sile_co_logprobs, "logprobs.hsaco")
 
 namespace sile_rt {
 namespace {
@@ -63,6 +66,9 @@ const Image kImages[static_cast<int>(Module::kCount)] = {
     {sile_co_paged_attn_begin, sile_co_paged_attn_end, "paged_attn"},
     {sile_co_kv_cache_begin, sile_co_kv_cache_end, "kv_cache"},
     {sile_co_flash_window_begin, sile_co_flash_window_end, "flash_window"},
+    {sile_co_rope_begin, sile_co_rope_end, "rope"},
+    {sile_co_rmsnorm_begin, sile_co_rmsnorm_end, "rmsnorm"},
+    {sile_co_logprobs_begin, sile_co_logprobs_end, "logprobs"},
 };
 
 struct DeviceState {

@@ -36,7 +36,10 @@ enum class Module : int {
   kPagedAttn = 5,
   kKvCache = 6,
   kFlashWindow = 7,
-  kCount = 8
+  kRope = 8,
+  kNorm = 9,
+  kLogprobs = 10,
+  kCount = 11
 };
 
 inline const char* dtype_name(int t) {
