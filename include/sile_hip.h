@@ -607,6 +607,34 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
                                int64_t window, int64_t sinks, void *workspace,
                                size_t workspace_bytes, sile_hip_stream stream);
 
+/* Workspace bytes that sile_hip_paged_attn_chunk needs on the current device (for any lengths;
+ * at most some 71 MB beside 4 for each 128 rows of tokens x query heads a key head). */
+int sile_hip_paged_attn_chunk_workspace(int64_t n_rows, int64_t n_tokens, int64_t q_heads,
+                                        int64_t kv_heads, int64_t head_dim, size_t *bytes);
+
+/* Attention of the new tokens of n_rows sequences over the cache: pieces of prompts and single
+ * tokens in one call.  Row r's tokens are starts[r] .. starts[r + 1] - 1 of the n_tokens rows of q and
+ * o (starts [n_rows + 1], not falling, as sile_hip_kv_slots makes it; clamped to
+ * [0, n_tokens]); the last of them is at position lengths[r] - 1, lengths[r] counting all of the row's keys,
+ * the new tokens' own, already stored, among them.  The token at position p sees the keys j <= p, and
+ * with window > 0 of these only j > p - window or j < sinks.  Rows of q and o that no sequence
+ * has are left as they are; a token at a position below 0 (lengths[r] below its tokens), or without any
+ * seen key, gives zeros.  Everything else as for sile_hip_paged_attn_decode: q, o, the cache and
+ * its e4m3 form, missing pages, NaN and Inf in keys that a token does not see, splitting and its
+ * rounding; at most 2^29 keys a row.  o overlaps nothing that the call reads.  The
+ * probabilities enter the second product in 16 bits (one part, where sile_hip_paged_attn_decode has
+ * two), as in sile_hip_flash_attn_window_fwd; a token whose result is not finite, or that meets
+ * Inf or NaN in V of a masked key of its blocks, is taken again in fp32: right, but slow. */
+int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n_rows,
+                              int64_t n_tokens, int64_t q_heads, int64_t kv_heads,
+                              int64_t head_dim, const void *q, int64_t ldq, const int32_t *starts,
+                              const void *k_pages, const void *v_pages, int64_t num_pages,
+                              int64_t page_size, int64_t page_stride, const int32_t *tables,
+                              int64_t ld_table, const int32_t *lengths, void *o, int64_t ldo,
+                              float scale, float k_scale, float v_scale, int64_t window,
+                              int64_t sinks, void *workspace, size_t workspace_bytes,
+                              sile_hip_stream stream);
+
 /* ---- a serving step around the cache: tokens, positions, norms, answers -------
  * No counterparts in the reference, as the cache above.  All only enqueue, on the current
  * device, and can be captured into a graph (they are plain kernel launches). */

@@ -172,6 +172,10 @@ SIGNATURES = {
     "sile_hip_paged_attn_decode": [_I32, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _I64,
                                    _I64, _P, _I64, _P, _P, _I64, _F32, _F32, _F32, _I64, _I64, _P,
                                    _SZ, _P],
+    "sile_hip_paged_attn_chunk_workspace": [_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)],
+    "sile_hip_paged_attn_chunk": [_I32, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I64,
+                                  _I64, _P, _I64, _P, _P, _I64, _F32, _F32, _F32, _I64, _I64, _P, _SZ,
+                                  _P],
     "sile_hip_kv_slots": [_I64, _P, _P, _P, _I64, _P, _P, _P, _P, _P],
     "sile_hip_rope_turns": [_I32, _I64, _F64, _F64, _F64, _F64, _F64, _P],
     "sile_hip_rope": [_I32, _I32, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I64,
@@ -600,6 +604,23 @@ def paged_attn_decode(dtype, cache_type, batch, q_heads, kv_heads, head_dim, q, 
     call("sile_hip_paged_attn_decode", dtype, cache_type, batch, q_heads, kv_heads, head_dim, q, ldq,
          k_pages, v_pages, num_pages, page_size, page_stride, tables, ld_table, lengths, o, ldo,
          scale, k_scale, v_scale, window, sinks, workspace or None, workspace_bytes, _sh(stream))
+
+
+def paged_attn_chunk_workspace(n_rows, n_tokens, q_heads, kv_heads, head_dim) -> int:
+    """Workspace bytes of paged_attn_chunk on the current device."""
+    n = _SZ(0)
+    call("sile_hip_paged_attn_chunk_workspace", n_rows, n_tokens, q_heads, kv_heads, head_dim,
+         ctypes.byref(n))
+    return n.value
+
+
+def paged_attn_chunk(dtype, cache_type, n_rows, n_tokens, q_heads, kv_heads, head_dim, q, ldq, starts,
+                     k_pages, v_pages, num_pages, page_size, page_stride, tables, ld_table, lengths, o,
+                     ldo, scale, k_scale=1.0, v_scale=1.0, window=0, sinks=0, workspace=0,
+                     workspace_bytes=0, stream=None):
+    call("sile_hip_paged_attn_chunk", dtype, cache_type, n_rows, n_tokens, q_heads, kv_heads, head_dim, q,
+         ldq, starts, k_pages, v_pages, num_pages, page_size, page_stride, tables, ld_table, lengths, o,
+         ldo, scale, k_scale, v_scale, window, sinks, workspace or None, workspace_bytes, _sh(stream))
 
 
 # ---------------------------------------------------------------------------

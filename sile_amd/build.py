@@ -30,7 +30,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 KERNELS = ["dsl", "softmax", "gemm", "attention", "flash_attn", "flash_window", "paged_attn",
-           "kv_cache", "rope", "rmsnorm", "logprobs"]
+           "kv_cache", "rope", "rmsnorm", "logprobs", "paged_chunk"]
 HOST_SOURCES = ["runtime.cpp", "ops.cpp", "paged.cpp", "serving.cpp", "llir.cpp", "tile_ir.cpp"]
 HIP_HOST_SOURCES = ["launch_noalloc.hip"]
 

@@ -9,7 +9,7 @@
 #include <cstdio>
 #include <cstring>
 
-#include "kernels/paged_plan.h"
+#include "kernels/chunk_plan.h"
 #include "paged_checks.h"
 
 using namespace sile_rt;
@@ -48,6 +48,19 @@ struct PagedArgs {
   float *part_ml, *part_o;
   int64_t ldq, ldo, page_stride, ld_table, capacity, window, sinks;
   int32_t batch, kv_heads, group, head_groups, d, num_pages, page_shift, groups, direct, e4m3;
+  float scale_log2, v_scale;
+};
+
+struct ChunkArgs {
+  const void *q, *k, *v;
+  void* o;
+  const int32_t *starts, *tables, *lengths;
+  int32_t* plan;
+  float* parts;
+  int64_t ldq, ldo, page_stride, ld_table;
+  sile::ChunkShape shape;
+  int32_t kv_heads, d, num_pages, page_shift, tiles, groups, direct;
+  uint32_t q_and, q_xor;
   float scale_log2, v_scale;
 };
 
@@ -117,6 +130,33 @@ int paged_plan(bool fp8, int64_t batch, int64_t q_heads, int64_t kv_heads, int64
   p->plan_ints = ints16(batch + 1);
   p->slots = 2 * p->groups * 16 * p->q_tiles;   // two a workgroup
   p->bytes = 4 * (p->plan_ints + p->slots * (2 + head_dim));
+  return SILE_OK;
+}
+
+// The attention of pieces of prompts: width of the padded head dimension, keys of a block, the
+// workgroups of a dealt list (a multiple of 8) and its workspace.
+struct ChunkPlan {
+  int dp, block;
+  int64_t tiles, groups, plan_ints, bytes;
+};
+int check_chunk(int64_t n_rows, int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
+  const int rc = check_heads(n_rows, q_heads, kv_heads, head_dim);
+  if (rc != SILE_OK) return rc;
+  if (n_rows > kMaxRows || n_tokens < 0 || n_tokens > kIntMax / 2 / (q_heads / kv_heads))
+    return fail(SILE_ERR_SHAPE, "%lld tokens of %lld rows: negative or too many", (long long)n_tokens, (long long)n_rows);
+  return SILE_OK;
+}
+int chunk_plan(int64_t n_rows, int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, ChunkPlan* p) {
+  p->dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  p->block = p->dp == 64 ? 64 : 32;
+  p->tiles = sile::chunk_tiles(n_tokens, n_rows, q_heads / kv_heads);
+  int cus = 0;
+  const int rc = device_cus(&cus);
+  if (rc != SILE_OK) return rc;
+  p->groups = std::max<int64_t>(8, (int64_t)(p->dp == 256 ? 1 : 2) * cus / 8 * 8);
+  p->plan_ints = ints16(p->tiles + 1);
+  // O and (m, l) of a tile's 128 rows, two parts a workgroup
+  p->bytes = 4 * (p->plan_ints + 2 * p->groups * 4 * (p->dp / 8 + 1) * 256);
   return SILE_OK;
 }
 
@@ -457,6 +497,112 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   snprintf(name, sizeof name, "sile_paged_attn_join_%s_q%d", dt, plan.q_tiles);
   void* join[] = {&a, &split};
   rc = launch(Module::kPagedAttn, name, dim3((unsigned)units, (unsigned)groups), dim3(512), join, s);
+  return rc == SILE_OK ? ok() : rc;
+}
+
+int sile_hip_paged_attn_chunk_workspace(int64_t n_rows, int64_t n_tokens, int64_t q_heads, int64_t kv_heads,
+                                        int64_t head_dim, size_t* bytes) {
+  if (!bytes) return fail(SILE_ERR_SHAPE, "bytes is NULL");
+  *bytes = 0;
+  int rc = check_chunk(n_rows, n_tokens, q_heads, kv_heads, head_dim);
+  if (rc != SILE_OK) return rc;
+  ChunkPlan plan;
+  if ((rc = chunk_plan(n_rows, n_tokens, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
+  *bytes = (size_t)plan.bytes;
+  return ok();
+}
+
+int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n_rows, int64_t n_tokens,
+                              int64_t q_heads, int64_t kv_heads, int64_t head_dim, const void* q, int64_t ldq,
+                              const int32_t* starts, const void* k_pages, const void* v_pages, int64_t num_pages,
+                              int64_t page_size, int64_t page_stride, const int32_t* tables, int64_t ld_table,
+                              const int32_t* lengths, void* o, int64_t ldo, float scale, float k_scale,
+                              float v_scale, int64_t window, int64_t sinks, void* workspace,
+                              size_t workspace_bytes, sile_hip_stream stream) {
+  int64_t es = 0;
+  int rc = check_chunk(n_rows, n_tokens, q_heads, kv_heads, head_dim);
+  if (rc != SILE_OK) return rc;
+  if ((rc = check_cache(dtype, cache_type, kv_heads, head_dim, num_pages, page_size, page_stride, &es)) != SILE_OK)
+    return rc;
+  if ((rc = check_table(n_rows, ld_table)) != SILE_OK) return rc;
+  if (window < 0 || sinks < 0) return fail(SILE_ERR_SHAPE, "negative window or sinks");
+  const float product = scale * k_scale;
+  if (!(std::fabs(product) <= 3.402823466e38f)) return fail(SILE_ERR_SHAPE, "scale * k_scale is not finite");
+  if (n_rows == 0 || n_tokens == 0) return ok();
+  if (!q || !o || !starts || !lengths || (num_pages > 0 && (!k_pages || !v_pages)) || (ld_table > 0 && !tables))
+    return fail(SILE_ERR_SHAPE, "NULL operand");
+  const int64_t width = q_heads * head_dim;
+  if (ldq < width || ldo < width) return fail(SILE_ERR_SHAPE, "leading dimension smaller than a token's heads");
+  if (!aligned16(q) || !aligned16(o) || !aligned16(k_pages) || !aligned16(v_pages) || ldq % 8 || ldo % 8)
+    return fail(SILE_ERR_SHAPE, "q, o and the pages have to be 16-byte aligned");
+  if (ldq > (1ll << 40) || ldo > (1ll << 40)) return fail(SILE_ERR_SHAPE, "leading dimension too large");
+  if (ld_table * page_size > (1ll << 29))
+    return fail(SILE_ERR_SHAPE, "a table of %lld pages of %lld keys: at most 2^29 keys a row", (long long)ld_table,
+                (long long)page_size);
+  if (o < static_cast<const char*>(q) + ((n_tokens - 1) * ldq + width) * 2 &&
+      static_cast<const char*>(q) < static_cast<const char*>(o) + ((n_tokens - 1) * ldo + width) * 2)
+    return fail(SILE_ERR_SHAPE, "o overlaps q");
+  ChunkPlan plan{};
+  const int block = head_dim <= 64 ? 64 : 32;
+  // without a page every row is empty
+  const int64_t capacity = num_pages > 0 ? ld_table * page_size : 0;
+  const int64_t tiles = sile::chunk_tiles(n_tokens, n_rows, q_heads / kv_heads);
+  // blocks of a unit: what a row holds, or its tokens' windows and the sinks
+  const int64_t tokens = std::min<int64_t>(n_tokens, sile::kChunkRows / (q_heads / kv_heads) + 2);
+  const int64_t seen = window > 0 ? std::min<int64_t>(capacity, std::min<int64_t>(window, kIntMax) + tokens +
+                                                                    std::min<int64_t>(sinks, kIntMax))
+                                  : capacity;
+  const int64_t unit = seen / block + 4 + sile::kChunkUnit;
+  if (tiles > (1 << 24) / kv_heads || tiles > (kIntMax - (1 << 20)) / (unit * kv_heads))
+    return fail(SILE_ERR_SHAPE, "%lld tokens of %lld rows of up to %lld keys: too many for one call",
+                (long long)n_tokens, (long long)n_rows, (long long)seen);
+  if ((rc = chunk_plan(n_rows, n_tokens, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
+  if ((rc = check_workspace(workspace, workspace_bytes, plan.bytes)) != SILE_OK) return rc;
+  ChunkArgs a{};
+  a.q = q;
+  a.k = k_pages;
+  a.v = v_pages;
+  a.o = o;
+  a.starts = starts;
+  a.tables = tables;
+  a.lengths = lengths;
+  a.plan = static_cast<int32_t*>(workspace);
+  a.parts = reinterpret_cast<float*>(a.plan + plan.plan_ints);
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.page_stride = page_stride;
+  a.ld_table = ld_table;
+  a.shape = {n_tokens, capacity, window, sinks, (int32_t)n_rows, (int32_t)(q_heads / kv_heads), block};
+  a.kv_heads = (int32_t)kv_heads;
+  a.d = (int32_t)head_dim;
+  a.num_pages = (int32_t)num_pages;
+  a.page_shift = page_shift_of(page_size);
+  a.tiles = (int32_t)tiles;
+  a.groups = (int32_t)plan.groups;
+  // the kernel wants a positive scale: a negative one's sign goes into q, under 0 all of it
+  a.q_and = product == 0.0f ? 0u : 0xffffffffu;
+  a.q_xor = product < 0.0f ? 0x80008000u : 0u;
+  a.scale_log2 = product == 0.0f ? 1.0f : std::fabs(product) * 1.4426950408889634f;
+  a.v_scale = v_scale;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const char* dt = dtype == SILE_F16 ? "f16" : "bf16";
+  const bool fp8 = cache_type != dtype;
+  char name[64];
+  // a DMA instruction covers 1 KiB of keys, which have to lie in one page
+  snprintf(name, sizeof name, "sile_paged_chunk_%s%s_%c%d", dt, fp8 ? "_fp8" : "",
+           !fp8 && page_size < 512 / plan.dp ? 's' : 'd', plan.dp);
+  void* params[] = {&a};
+  const int64_t units = tiles * kv_heads;
+  a.direct = seen <= 512;
+  int64_t grid = a.direct ? units : plan.groups;
+  if (!a.direct) {
+    const int64_t most = (tiles * unit * kv_heads + sile::kChunkShare + sile::kChunkUnit - 1) / (sile::kChunkShare + sile::kChunkUnit);
+    grid = std::min(grid, (most + 7) / 8 * 8);
+  }
+  rc = launch(Module::kPagedChunk, name, dim3((unsigned)grid), dim3(256), params, s);
+  if (rc != SILE_OK || a.direct) return rc == SILE_OK ? ok() : rc;
+  snprintf(name, sizeof name, "sile_paged_chunk_join_%s%s_d%d", dt, fp8 ? "_fp8" : "", plan.dp);
+  rc = launch(Module::kPagedChunk, name, dim3((unsigned)units, sile::kChunkRows / 32), dim3(256), params, s);
   return rc == SILE_OK ? ok() : rc;
 }
 

@@ -45,6 +45,7 @@ SILE_EMBED(sile_co_paged_attn, "paged_attn.hsaco")
 SILE_EMBED(sile_co_kv_cache, "kv_cache.hsaco")
 SILE_EMBED(sile_co_flash_window, "flash_window.hsaco")
 SILE_EMBED(sile_co_rope, "rope.hsaco")
+SILE_EMBED(sile_co_paged_chunk, "paged_chunk.hsaco")
 SILE_EMBED(sile_co_rmsnorm, "rmsnorm.hsaco")
 SILE_EMBED(sile_co_logprobs, "logprobs.hsaco")
 
@@ -69,6 +70,7 @@ const Image kImages[static_cast<int>(Module::kCount)] = {
     {sile_co_rope_begin, sile_co_rope_end, "rope"},
     {sile_co_rmsnorm_begin, sile_co_rmsnorm_end, "rmsnorm"},
     {sile_co_logprobs_begin, sile_co_logprobs_end, "logprobs"},
+    {sile_co_paged_chunk_begin, sile_co_paged_chunk_end, "paged_chunk"},
 };
 
 struct DeviceState {

@@ -39,7 +39,8 @@ enum class Module : int {
   kRope = 8,
   kNorm = 9,
   kLogprobs = 10,
-  kCount = 11
+  kPagedChunk = 11,
+  kCount = 12
 };
 
 inline const char* dtype_name(int t) {

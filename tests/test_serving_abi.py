@@ -131,3 +131,26 @@ def test_nothing_to_do():
     _abi.rmsnorm_rows(**{**NORM, "rows": 0, "x": None})
     _abi.rmsnorm_rows(**{**NORM, "cols": 0, "y": None})
     _abi.logprobs_rows(**{**LOGPROBS, "rows": 0, "x": None})
+
+
+CHUNK = dict(dtype=_abi.BF16, cache_type=_abi.BF16, n_rows=4, n_tokens=30, q_heads=4, kv_heads=2, head_dim=64, q=P, ldq=256, starts=2 * P,
+             k_pages=3 * P, v_pages=4 * P, num_pages=10, page_size=16, page_stride=2048, tables=5 * P, ld_table=3, lengths=6 * P, o=7 * P,
+             ldo=256, scale=0.125, workspace=8 * P, workspace_bytes=1 << 30)
+
+
+def test_chunk_refused():
+    f = _abi.paged_attn_chunk
+    for change in (dict(dtype=_abi.F32), dict(cache_type=_abi.F16), dict(head_dim=264, ldq=2000, ldo=2000),
+                   dict(head_dim=72, cache_type=_abi.F8E4M3, ldq=2000, ldo=2000, page_stride=1 << 20)):
+        refused("UnsupportedBackend", f, **{**CHUNK, **change})
+    for change in (dict(n_rows=-1), dict(n_tokens=-1), dict(n_tokens=2 ** 31), dict(q_heads=5), dict(q_heads=0), dict(kv_heads=0), dict(q=None),
+                   dict(o=None), dict(starts=None), dict(lengths=None), dict(tables=None), dict(k_pages=None), dict(v_pages=None),
+                   dict(ldq=255), dict(ldo=248), dict(ldq=260), dict(q=P + 2), dict(o=7 * P + 8), dict(k_pages=3 * P + 8), dict(page_size=24),
+                   dict(page_stride=2047), dict(num_pages=-1), dict(ld_table=-1), dict(window=-1), dict(sinks=-1), dict(o=P), dict(o=P + 256),
+                   dict(scale=float("nan")), dict(scale=float("inf")), dict(k_scale=float("inf")), dict(ld_table=1 << 26),
+                   dict(n_rows=1 << 22, ld_table=500, page_size=65536, page_stride=1 << 24)):
+        refused("Shape", f, **{**CHUNK, **change})
+    f(**{**CHUNK, "n_tokens": 0, "q": None})
+    f(**{**CHUNK, "n_rows": 0, "starts": None})
+    refused("Shape", _abi.paged_attn_chunk_workspace, 1, -1, 4, 2, 64)
+    refused("Shape", _abi.paged_attn_chunk_workspace, 1, 1, 5, 2, 64)
