@@ -7,15 +7,20 @@
 // Memory bounds it: every logit is read once (16 bytes a load, two chunks of 8192 in flight) and
 // kept in registers while a lane folds it into its own running (max m, sum l of p = 2^(c (x - m)),
 // sum e of p (x - m)), c = scale log2 e.  The difference comes first, so that logits at the type's
-// lowest value stay numbers; e keeps the entropy's digits where one token has nearly all the mass.  What the top ones cost beside that: one comparison of a chunk's
-// largest value of a lane with the k-th best so far, and where one passes (rarely, after the
-// first chunk) one of each element.  Candidates go to a list in LDS, and whoever has fewer than k
-// before it stays.  The first chunk has no k-th best: the ceil(k / 4)-th largest of a wave's lanes, the
-// least of the four waves', has k elements at or above it, and so has the k-th largest of any wave.
-// Where more than the list holds are as good (rows of equal logits), the k best are looked for one
-// at a time.
+// lowest value stay numbers; e keeps the entropy's digits where one token has nearly all the mass.  What the top ones cost
+// beside that: every wave keeps the k best of its columns in order, an entry a lane, and a chunk's largest
+// value of a lane is compared with the k-th; where one passes (rarely, after the first chunk) its
+// elements are, and what passes is put in its place by a shift of the lanes behind it.  In the first
+// chunk the ceil(k / 4)-th largest of the lanes' maxima, the least of the four waves', stands for the k-th best:
+// k elements reach it.  After that no wave waits for another before its last column.  (Candidates of the workgroup in LDS, ranked by counting
+// after each chunk: 77 us both below; sorted and merged by one wave: 24 and 82.)
 //
 // Few long rows: a row's chunks go to several workgroups, and a second launch joins their parts.
+//
+// Measured: 64 rows of 131072 in bf16, 20 top ones, 20 us (14 and the join 6; without top ones 9), one
+// row 14; 2000 rows of 32001 in f32, 5 top ones, 54 (4.8 TB/s; without 45), of 32000 in bf16, 20 top ones,
+// 50 (without 27).  What holds them is the latency of the list's steps, then instructions: a quarter
+// of the time without top ones is exp2's.
 #include <type_traits>
 
 #include "common.h"
@@ -27,8 +32,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kElems = 32;                    // of a thread, a chunk
 constexpr int kChunk = kThreads * kElems;
-constexpr int kCap = 1024;                    // of the list
 constexpr int kMaxTop = 64;
+constexpr float kLowest = -3.402823466e38f;
 
 struct LogprobArgs {
   const void* x;
@@ -37,7 +42,7 @@ struct LogprobArgs {
   int32_t* top_ids;
   float* part_sums;                           // [rows][parts][4]: m, l, e
   float* part_top;                            // [rows][parts][top]: values
-  int32_t* part_ids;                          // their columns, -1: none
+  int32_t* part_ids;                          // their columns
   int64_t ldx;
   int32_t rows, cols, top, parts, chunks, per_part;   // chunks of a row, of a part
   float scale, scale_log2;
@@ -49,15 +54,10 @@ typedef uint32_t raw_f32 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t raw_16 __attribute__((ext_vector_type(4), aligned(2)));
 
 struct List {
-  float value[kCap + kMaxTop];
-  int32_t column[kCap + kMaxTop];
-  float kept_value[kMaxTop];
-  int32_t kept_column[kMaxTop];
-  int32_t added[3];     // entries that a chunk added, three chunks in turn
-  float wave_least[4], wave_kth[4];
-  float best_value[4];
-  int32_t best_column[4];
+  float value[4][kMaxTop];      // the waves' lists; [0]: the workgroup's
+  int32_t column[4][kMaxTop];
   float sums[4][3];
+  float quarter[4];
 };
 
 template <int kType>   // sile_dtype
@@ -65,21 +65,6 @@ SILE_DEV float logit(const void* x, int64_t i) {
   if constexpr (kType == 0) return static_cast<const float*>(x)[i];
   const uint16_t h = static_cast<const uint16_t*>(x)[i];
   return kType == 1 ? f16_to_f32(h) : bf16_to_f32(h);
-}
-
-// (m, l, e) of two sets of elements, joined; m = -inf: an empty set, or one of probability 0
-SILE_DEV void join_sums(const LogprobArgs& a, float& m, float& l, float& e, float m2, float l2, float e2) {
-  const float top = __builtin_fmaxf(m, m2);
-  if (top == -__builtin_inff()) {   // (sums of NaN stay)
-    l += l2;
-    e += e2;
-    return;
-  }
-  const float d1 = m - top, d2 = m2 - top;   // <= 0, -inf of an empty set; NaN if top is +inf
-  const float a1 = exp2_fast(d1 * a.scale_log2), a2 = exp2_fast(d2 * a.scale_log2);
-  e = a1 * (e + l * __builtin_fmaxf(d1, a.floor)) + a2 * (e2 + l2 * __builtin_fmaxf(d2, a.floor));
-  l = a1 * l + a2 * l2;
-  m = top;
 }
 
 // The largest float, of 16 significant bits, that at least k of the wave's values reach; -inf
@@ -101,98 +86,147 @@ SILE_DEV float reached_by(float v, int k) {
 
 SILE_DEV bool before(float v, int32_t c, float w, int32_t d) { return v > w || (v == w && c < d); }
 
-// Keeps the `top` first of the list's n entries (at most kCap + kMaxTop), in order, and returns how
-// many they are; all threads.
-SILE_DEV int keep_first(List* s, int n, int top) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const float v = s->value[i];
-    const int32_t c = s->column[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += before(s->value[j], s->column[j], v, c) ? 1 : 0;
-    if (rank < top) {
-      s->kept_value[rank] = v;
-      s->kept_column[rank] = c;
-    }
+// ---- up to 64 entries in order, one a lane ----
+struct Entry {
+  float v;
+  int32_t c;
+};
+SILE_DEV Entry no_entry() { return {-__builtin_inff(), 0x7fffffff}; }
+// v of lane ^ kMask, by moves between lanes alone (through LDS each of a merge's steps, one after the
+// other, waits some 100 cycles)
+template <int kMask>
+SILE_DEV int lane_xor(int v) {
+  constexpr int kRowRor8 = 0x128, kQuadReverse = 0x1B;
+  if constexpr (kMask == 1) return dpp_int<kDppXor1>(v);
+  if constexpr (kMask == 2) return dpp_int<kDppXor2>(v);
+  if constexpr (kMask == 4) return dpp_int<kQuadReverse>(dpp_int<kDppHalfMirror>(v));   // ^ 7 ^ 3
+  if constexpr (kMask == 8) return dpp_int<kRowRor8>(v);
+  const unsigned u = (unsigned)v;
+  if constexpr (kMask == 16) {   // two copies trade odd and even rows: (0, 0, 2, 2) and (1, 1, 3, 3)
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned even = r[0], odd = r[1];
+    return (int)((threadIdx.x & 16) ? even : odd);
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned lo = r[0], hi = r[1];
+  return (int)((threadIdx.x & 32) ? lo : hi);
+}
+template <int kMask>
+SILE_DEV Entry lane_xor(const Entry& t) {
+  return {bits_f32((uint32_t)lane_xor<kMask>((int)f32_bits(t.v))), lane_xor<kMask>(t.c)};
+}
+// the earlier of the lane's entry and that of lane ^ kMask in the lower lane, the later in the upper
+template <int kMask>
+SILE_DEV void exchange(Entry& t) {
+  const Entry u = lane_xor<kMask>(t);
+  if (before(u.v, u.c, t.v, t.c) == ((threadIdx.x & kMask) == 0)) t = u;
+}
+// puts (x, col), which all lanes have, in its place
+SILE_DEV void insert(Entry& t, float x, int32_t col) {
+  const uint64_t ahead = __builtin_amdgcn_ballot_w64(before(t.v, t.c, x, col));
+  const int place = (int)__builtin_popcountll(ahead), lane = threadIdx.x & 63;
+  constexpr int kWaveShr1 = 0x138;   // lane i takes lane i - 1's
+  const float v = dpp<kWaveShr1>(t.v);
+  const int32_t c = dpp_int<kWaveShr1>(t.c);
+  t.v = lane == place ? x : lane > place ? v : t.v;
+  t.c = lane == place ? col : lane > place ? c : t.c;
+}
+// The first 64 of two lists in order, of which the first `top` count: what of u precedes t's last of
+// them is put in its place one by one, or, where that is more than a few, by a bitonic merge.
+SILE_DEV void merge64(Entry& t, const Entry& u, int top) {
+  const float kth = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(t.v), top - 1));
+  const int32_t kth_c = __builtin_amdgcn_readlane(t.c, top - 1);
+  const int n = (int)__builtin_popcountll(__builtin_amdgcn_ballot_w64(before(u.v, u.c, kth, kth_c)));
+  if (n <= 6) {
+    for (int i = 0; i < n; ++i)
+      insert(t, bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(u.v), i)), __builtin_amdgcn_readlane(u.c, i));
+    return;
+  }
+  // u backwards: lane ^ 63, and a row's mirror is ^ 15
+  const Entry m = {dpp<kDppMirror>(u.v), dpp_int<kDppMirror>(u.c)};
+  const Entry w = lane_xor<32>(lane_xor<16>(m));
+  if (before(w.v, w.c, t.v, t.c)) t = w;
+  exchange<32>(t);
+  exchange<16>(t);
+  exchange<8>(t);
+  exchange<4>(t);
+  exchange<2>(t);
+  exchange<1>(t);
+}
+// the waves' lists into one, in s->value[0]
+SILE_DEV void merge_waves(List* s, Entry t, int top) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (wave > 0) {
+    s->value[wave][lane] = t.v;
+    s->column[wave][lane] = t.c;
   }
   __syncthreads();
-  const int kept = min(n, top);
-  if ((int)threadIdx.x < kept) {
-    s->value[threadIdx.x] = s->kept_value[threadIdx.x];
-    s->column[threadIdx.x] = s->kept_column[threadIdx.x];
+  if (wave == 0) {
+#pragma unroll 1
+    for (int w = 1; w < 4; ++w) merge64(t, {s->value[w][lane], s->column[w][lane]}, top);
+    s->value[0][lane] = t.v;
+    s->column[0][lane] = t.c;
   }
   __syncthreads();
-  return kept;
 }
 
+// the lane's sums as those of a maximum of `top`, which is at least m (both -inf: nothing to scale)
+SILE_DEV void rescale(const LogprobArgs& a, float m, float& l, float& e, float top) {
+  const float d = m == top ? 0.0f : m - top, f = exp2_fast(d * a.scale_log2);
+  e = f * (e + l * __builtin_fmaxf(d, a.floor));
+  l *= f;
+}
 // the sums of all threads, joined
 SILE_DEV void all_sums(const LogprobArgs& a, List* s, float& m, float& l, float& e) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const float m2 = __shfl_xor(m, off), l2 = __shfl_xor(l, off), e2 = __shfl_xor(e, off);
-    join_sums(a, m, l, e, m2, l2, e2);
-  }
+  const float top = wave_max(m);
+  rescale(a, m, l, e, top);
+  l = wave_sum(l);
+  e = wave_sum(e);
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) {
-    s->sums[wave][0] = m;
+    s->sums[wave][0] = top;
     s->sums[wave][1] = l;
     s->sums[wave][2] = e;
   }
   __syncthreads();
-  m = s->sums[0][0];
-  l = s->sums[0][1];
-  e = s->sums[0][2];
+  m = __builtin_fmaxf(__builtin_fmaxf(s->sums[0][0], s->sums[1][0]), __builtin_fmaxf(s->sums[2][0], s->sums[3][0]));
+  l = e = 0.0f;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) join_sums(a, m, l, e, s->sums[w][0], s->sums[w][1], s->sums[w][2]);
+  for (int w = 0; w < 4; ++w) {
+    float lw = s->sums[w][1], ew = s->sums[w][2];
+    rescale(a, s->sums[w][0], lw, ew, m);
+    l += lw;
+    e += ew;
+  }
 }
 
-// the workgroup's first of one (value, column) a thread; all threads have it
-SILE_DEV void first_of_all(List* s, float& v, int32_t& c) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const float w = __shfl_xor(v, off);
-    const int32_t d = __shfl_xor(c, off);
-    if (before(w, d, v, c)) {
-      v = w;
-      c = d;
-    }
-  }
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) {
-    s->best_value[wave] = v;
-    s->best_column[wave] = c;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; ++w)
-    if (before(s->best_value[w], s->best_column[w], v, c)) {
-      v = s->best_value[w];
-      c = s->best_column[w];
-    }
-  __syncthreads();
-}
-
-// the results of a row from its sums and its list
+// the logit of the row's target, asked for ahead of its use; thread 0
 template <int kType>
-SILE_DEV void finish(const LogprobArgs& a, const List* s, int row, int n, float m, float l, float e) {
+SILE_DEV float target_logit(const LogprobArgs& a, int row, bool* there) {
+  *there = false;
+  if (threadIdx.x != 0 || !a.logp) return 0.0f;
+  const int32_t t = a.targets[row];
+  *there = t >= 0 && t < a.cols;
+  return *there ? logit<kType>(a.x, row * a.ldx + t) : 0.0f;
+}
+// the results of a row from its sums and the list
+SILE_DEV void finish(const LogprobArgs& a, const List* s, int row, float target, bool there, float m, float l, float e) {
   const int tid = threadIdx.x;
   const float log_l = logf(l);
   const bool none = m == -__builtin_inff() && l == 0.0f;   // every logit is -inf
-  auto logp_of = [&](float x) {
-    return none ? -__builtin_inff() : (x - m) * a.scale - log_l;
-  };
+  auto logp_of = [&](float x) { return none ? -__builtin_inff() : (x - m) * a.scale - log_l; };
   if (tid == 0) {
-    if (a.logp) {
-      const int32_t t = a.targets[row];
-      a.logp[row] = t >= 0 && t < a.cols ? logp_of(logit<kType>(a.x, row * a.ldx + t)) : 0.0f;
-    }
+    if (a.logp) a.logp[row] = there ? logp_of(target) : 0.0f;
     if (a.entropy) {
       const float h = none ? 0.0f : log_l - e / l * a.scale;
       a.entropy[row] = h < 0.0f ? 0.0f : h;   // (by rounding; NaN stays)
     }
   }
   if (a.top_ids && tid < a.top) {
-    a.top_logp[(int64_t)row * a.top + tid] = tid < n ? logp_of(s->value[tid]) : -__builtin_inff();
-    a.top_ids[(int64_t)row * a.top + tid] = tid < n ? s->column[tid] : -1;
+    const float v = s->value[0][tid];
+    const bool is = v > -__builtin_inff();
+    a.top_logp[(int64_t)row * a.top + tid] = is ? logp_of(v) : -__builtin_inff();
+    a.top_ids[(int64_t)row * a.top + tid] = is ? s->column[0][tid] : -1;
   }
 }
 
@@ -205,34 +239,22 @@ SILE_DEV void logprobs(const LogprobArgs& a, List* s) {
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   const int c_first = part * a.per_part, c_last = min(c_first + a.per_part, a.chunks);
   const uint8_t* base = static_cast<const uint8_t*>(a.x) + (int64_t)row * a.ldx * (kType == 0 ? 4 : 2);
-  if (tid == 0) s->added[0] = 0;
+  bool there = false;
+  const float target = a.parts == 1 ? target_logit<kType>(a, row, &there) : 0.0f;
   const float c = a.scale_log2;
 
   u32x4 next[kLoads];
-  // (loads need no alignment beyond the element's; a load that runs past the row's end is made
-  // element by element, the rest as -inf)
+  // (loads need no alignment beyond the element's; what the last one of a row would read past its end
+  // comes behind the chunks)
+  const int whole = a.cols / kPer * kPer;
   auto load = [&](int chunk) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int64_t at = (int64_t)chunk * kChunk + (i * kThreads + tid) * kPer;
-      if (at + kPer <= a.cols) {
-        next[i] = *reinterpret_cast<const raw_t*>(base + at * (kType == 0 ? 4 : 2));
-      } else {
-        u32x4 w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = kType == 0 ? 0xff800000u : kType == 1 ? 0xfc00fc00u : 0xff80ff80u;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j)
-          if (at + j < a.cols) {
-            if constexpr (kType == 0) {
-              w[j] = reinterpret_cast<const uint32_t*>(base)[at + j];
-            } else {
-              const uint32_t h = reinterpret_cast<const uint16_t*>(base)[at + j];
-              w[j >> 1] = (j & 1) ? (w[j >> 1] & 0xffffu) | h << 16 : (w[j >> 1] & 0xffff0000u) | h;
-            }
-          }
-        next[i] = w;
-      }
+      constexpr uint32_t kNone = kType == 0 ? 0xff800000u : kType == 1 ? 0xfc00fc00u : 0xff80ff80u;   // -inf
+      u32x4 w = {kNone, kNone, kNone, kNone};
+      if (at < whole) w = *reinterpret_cast<const raw_t*>(base + at * (kType == 0 ? 4 : 2));
+      next[i] = w;
     }
   };
   auto element = [](const u32x4* w, int i) {   // i: constant after unrolling
@@ -243,11 +265,36 @@ SILE_DEV void logprobs(const LogprobArgs& a, List* s) {
   };
 
   float m = -__builtin_inff(), l = 0.0f, e = 0.0f;
-  float kth = -__builtin_inff();   // the list's last, once it has `top` entries
-  bool full = false;
-  int had = 0;                     // entries of the list
+  const int few = max((a.top + 3) / 4, 1);
+  Entry best = no_entry();
+  float least = kLowest;           // what does not reach it, or is -inf, cannot be among the wave's best
+  float kth = -__builtin_inff();   // the list's last, -inf while it has fewer than `top`
+  int32_t kth_c = 0x7fffffff;
+  auto grow = [&](float v) {   // the lane's maximum is at least v
+    if (v > m) {
+      const float d = m - v, f = exp2_fast(d * c);
+      e = f * (e + l * __builtin_fmaxf(d, a.floor));
+      l *= f;
+      m = v;
+    }
+  };
+  auto add = [&](float v, float m_use) {
+    const float d = v - m_use, p = exp2_fast(d * c);
+    l += p;
+    e = __builtin_fmaf(p, __builtin_fmaxf(d, a.floor), e);
+  };
+  auto place = [&](float v, int32_t col) {   // the lanes' values into the list, where they belong there
+    uint64_t in = __builtin_amdgcn_ballot_w64(v >= least && before(v, col, kth, kth_c));
+    for (; in != 0; in &= in - 1) {
+      const int from = __builtin_ctzll(in);
+      insert(best, bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(v), from)),
+             __builtin_amdgcn_readlane(col, from));
+    }
+    kth = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(best.v), a.top - 1));
+    kth_c = __builtin_amdgcn_readlane(best.c, a.top - 1);
+    least = __builtin_fmaxf(least, kth);
+  };
   load(c_first);
-  __syncthreads();
   for (int chunk = c_first; chunk < c_last; ++chunk) {
     u32x4 w[kLoads];
 #pragma unroll
@@ -257,154 +304,102 @@ SILE_DEV void logprobs(const LogprobArgs& a, List* s) {
 #pragma unroll
     for (int i = 0; i < kElems; ++i) most = __builtin_fmaxf(most, element(w, i));
     // the lane's sums
-    const float m_new = __builtin_fmaxf(m, most);
-    const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
-    if (m_new > m) {
-      const float d = m - m_new, f = exp2_fast(d * c);
-      e = f * (e + l * __builtin_fmaxf(d, a.floor));
-      l *= f;
-      m = m_new;
-    }
+    grow(most);
+    const float m_use = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) {
-      const float d = element(w, i) - m_use;
-      const float p = exp2_fast(d * c);
-      l += p;
-      e = __builtin_fmaf(p, __builtin_fmaxf(d, a.floor), e);
-    }
+    for (int i = 0; i < kElems; ++i) add(element(w, i), m_use);
     if (a.top == 0) continue;
-    // ---- candidates ----
-    float least = kth;
-    if (!full) {
-      const float quarter = reached_by(most, (a.top + 3) / 4), alone = reached_by(most, a.top);
-      if (lane == 0) {
-        s->wave_least[wave] = quarter;
-        s->wave_kth[wave] = alone;
-      }
-      __syncthreads();
-      float q = s->wave_least[0];
-      least = s->wave_kth[0];
-#pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        q = __builtin_fminf(q, s->wave_least[i]);
-        least = __builtin_fmaxf(least, s->wave_kth[i]);
-      }
-      least = __builtin_fmaxf(least, q);
-    }
-    const int32_t col0 = chunk * kChunk + tid * kPer;
-    auto column = [&](int i) { return col0 + (i / kPer) * kThreads * kPer + i % kPer; };
-    // (the list's entries are of lower columns: an equal one is behind them)
-    auto enters = [&](float v) { return full ? v > least : v >= least && v > -__builtin_inff(); };
-    const int turn = (chunk - c_first) % 3;
-    if (tid == 0) s->added[turn == 2 ? 0 : turn + 1] = 0;   // (last read two chunks ago)
-    if (__builtin_amdgcn_ballot_w64(enters(most)) != 0) {
-#pragma unroll
-      for (int i = 0; i < kElems; ++i) {
-        const float v = element(w, i);
-        if (enters(v)) {
-          const int at = had + atomicAdd(&s->added[turn], 1);
-          if (at < kCap + kMaxTop) {
-            s->value[at] = v;
-            s->column[at] = column(i);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    int n = had + s->added[turn];
-    if (n == had) continue;
-    if (n > kCap + kMaxTop) {   // the chunk's best after (v, d), one at a time
-      float v = __builtin_inff();
-      int32_t d = -1;
-      n = had;
-      for (int k = 0; k < a.top; ++k) {
-        float bv = -__builtin_inff();
-        int32_t bc = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < kElems; ++i) {
-          const float x = element(w, i);
-          if (before(v, d, x, column(i)) && before(x, column(i), bv, bc)) {
-            bv = x;
-            bc = column(i);
-          }
-        }
-        first_of_all(s, bv, bc);
-        if (bv == -__builtin_inff()) break;
-        if (tid == 0) {
-          s->value[n] = bv;
-          s->column[n] = bc;
-        }
-        ++n;
-        v = bv;
-        d = bc;
-      }
+    // ---- the wave's best ----
+    // (what every wave has ceil(top / 4) of, the workgroup has top of; later than it was written will do)
+    if (chunk == c_first) {
+      const float some = reached_by(most, few);
+      if (lane == 0) s->quarter[wave] = some;
       __syncthreads();
     }
-    had = keep_first(s, n, a.top);
-    full = had == a.top;
-    if (full) kth = s->value[a.top - 1];
+    float all = __builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      all = __builtin_fminf(all, __hip_atomic_load(&s->quarter[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    if (chunk == c_first && all == -__builtin_inff()) all = reached_by(most, a.top);
+    least = __builtin_fmaxf(least, all);
+    if (__builtin_amdgcn_ballot_w64(most >= least) == 0) continue;
+    // a lane's elements that reach it, as bits; they are loaded again, one of each lane at a time (with
+    // the insertion behind each of the 32 its code was 10 KB, fetched anew in each launch)
+    uint32_t passed = 0;
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) passed |= element(w, i) >= least ? 1u << i : 0u;
+    while (__builtin_amdgcn_ballot_w64(passed != 0) != 0) {
+      const int i = __builtin_ctz(passed | 0x80000000u);
+      const int32_t col = chunk * kChunk + tid * kPer + (i / kPer) * kThreads * kPer + i % kPer;
+      const float v = passed != 0 ? logit<kType>(base, col) : -__builtin_inff();
+      passed &= passed - 1;
+      place(v, col);
+    }
+    const float some = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(best.v), few - 1));
+    if (lane == 0 && chunk != c_first) __hip_atomic_store(&s->quarter[wave], some, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
+  if (part == a.parts - 1 && whole < a.cols && wave == 0) {   // the row's last few: a lane one
+    const float v = tid < a.cols - whole ? logit<kType>(base, whole + tid) : -__builtin_inff();
+    grow(v);
+    add(v, m == -__builtin_inff() ? 0.0f : m);
+    if (a.top != 0) place(v, whole + tid);
+  }
+  if (a.top != 0) merge_waves(s, best, a.top);
   all_sums(a, s, m, l, e);
   if (a.parts == 1) {
-    finish<kType>(a, s, row, had, m, l, e);
+    finish(a, s, row, target, there, m, l, e);
     return;
   }
   const int64_t at = (int64_t)row * a.parts + part;
   if (tid == 0) *reinterpret_cast<f32x4*>(a.part_sums + 4 * at) = f32x4{m, l, e, 0.0f};
   if (tid < a.top) {
-    a.part_top[at * a.top + tid] = tid < had ? s->value[tid] : -__builtin_inff();
-    a.part_ids[at * a.top + tid] = tid < had ? s->column[tid] : -1;
+    a.part_top[at * a.top + tid] = s->value[0][tid];
+    a.part_ids[at * a.top + tid] = s->column[0][tid];
   }
 }
 
 // Joins the parts of row blockIdx.x.
 template <int kType>
 SILE_DEV void logprobs_join(const LogprobArgs& a, List* s) {
-  const int tid = threadIdx.x, row = blockIdx.x;
+  const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t first = (int64_t)row * a.parts;
+  bool there;
+  const float target = target_logit<kType>(a, row, &there);
   float m = -__builtin_inff(), l = 0.0f, e = 0.0f;
-  // a part that has `top` entries has that many at or above its last
-  float least = -__builtin_inff();
   for (int p = tid; p < a.parts; p += kThreads) {
     const f32x4 w = *reinterpret_cast<const f32x4*>(a.part_sums + 4 * (first + p));
-    join_sums(a, m, l, e, w[0], w[1], w[2]);
-    if (a.top) least = __builtin_fmaxf(least, a.part_top[(first + p) * a.top + a.top - 1]);
+    const float top = __builtin_fmaxf(m, w[0]);
+    float lw = w[1], ew = w[2];
+    rescale(a, m, l, e, top);
+    rescale(a, w[0], lw, ew, top);
+    m = top;
+    l += lw;
+    e += ew;
+  }
+  if (a.top) {
+    // a part's list is in order; the next one is on its way
+    auto list = [&](int p) {
+      Entry u = no_entry();
+      if (lane < a.top && p < a.parts) u = {a.part_top[(first + p) * a.top + lane], a.part_ids[(first + p) * a.top + lane]};
+      return u;
+    };
+    Entry t = list(wave), u = list(wave + 4);
+#pragma unroll 1
+    for (int p = wave + 4; p < a.parts; p += 4) {
+      const Entry ahead = list(p + 4);
+      merge64(t, u, a.top);
+      u = ahead;
+    }
+    merge_waves(s, t, a.top);
   }
   all_sums(a, s, m, l, e);
-  int had = 0;
-  if (a.top) {
-    int32_t none = 0;
-    first_of_all(s, least, none);
-    const int64_t entries = (int64_t)a.parts * a.top;
-    int turn = 0;
-    if (tid == 0) s->added[0] = 0;
-    __syncthreads();
-    for (int64_t e0 = 0; e0 < entries; e0 += kCap, turn = turn == 2 ? 0 : turn + 1) {
-      if (tid == 0) s->added[turn == 2 ? 0 : turn + 1] = 0;
-#pragma unroll
-      for (int u = 0; u < kCap / kThreads; ++u) {
-        const int64_t i = e0 + u * kThreads + tid;
-        if (i >= entries) break;
-        const float v = a.part_top[first * a.top + i];
-        const int32_t c = a.part_ids[first * a.top + i];
-        if (c >= 0 && v >= least) {
-          const int at = had + atomicAdd(&s->added[turn], 1);
-          s->value[at] = v;
-          s->column[at] = c;
-        }
-      }
-      __syncthreads();
-      const int n = had + s->added[turn];
-      if (n != had) had = keep_first(s, n, a.top);
-    }
-  }
-  finish<kType>(a, s, row, had, m, l, e);
+  finish(a, s, row, target, there, m, l, e);
 }
 
 }  // namespace
 
 #define SILE_LOGPROBS(NAME, TYPE)                                                                       \
-  extern "C" __global__ __launch_bounds__(kThreads) void sile_logprobs_##NAME(LogprobArgs a) {          \
+  extern "C" __global__ __launch_bounds__(kThreads, 4) void sile_logprobs_##NAME(LogprobArgs a) {          \
     __shared__ List s;                                                                                  \
     logprobs<TYPE>(a, &s);                                                                              \
   }                                                                                                     \
