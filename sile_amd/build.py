@@ -41,6 +41,9 @@ DEVICE_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
+# The attention of pieces of prompts: the default scheduler puts each fragment's read from LDS right
+# before the product that takes it.
+KERNEL_FLAGS = {"paged_chunk": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]}
 
 
 def _run(cmd):
@@ -53,7 +56,7 @@ def _run(cmd):
 def build_kernel(name: str) -> str:
     src = os.path.join(KDIR, name + ".hip")
     out = os.path.join(BUILD, name + ".hsaco")
-    _run([HIPCC, *DEVICE_FLAGS, "-o", out + ".tmp", src])
+    _run([HIPCC, *DEVICE_FLAGS, *KERNEL_FLAGS.get(name, []), "-o", out + ".tmp", src])
     os.replace(out + ".tmp", out)
     return out
 

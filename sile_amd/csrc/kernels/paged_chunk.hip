@@ -257,7 +257,9 @@ template <int kDh>
 constexpr int kPartFloats = 4 * (4 * (kDh / 32) + 1) * 64 * 4;
 
 template <bool kBF16, Source kSrc, int kNK, int kDh, int kDp>
-__device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, ChunkLds* deal) {
+__device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* __restrict__ Q, const uint8_t* __restrict__ K,
+                                           const uint8_t* __restrict__ V, uint16_t* __restrict__ O, uint8_t* smem,
+                                           ChunkLds* deal) {
   constexpr int kWG = 4;
   constexpr int kST = kNK / 32;
   constexpr int kRow = 2 * kDp;          // bytes of a K or V row in LDS
@@ -285,9 +287,12 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
   int32_t tile, kvh, seq;
   int32_t x, x1, base;
   if (a.direct) {
-    // the last tiles of a piece see the most keys: first
-    kvh = __builtin_amdgcn_readfirstlane((int)blockIdx.x / a.tiles);
-    tile = a.tiles - 1 - __builtin_amdgcn_readfirstlane((int)blockIdx.x - kvh * a.tiles);
+    // (an XCD takes a contiguous run of units; the last tiles of a piece see the most keys: first)
+    const int units = a.tiles * a.kv_heads, per_xcd = (units + 7) / 8;
+    const int unit = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (unit >= units) return;
+    kvh = sgpr(unit / a.tiles);
+    tile = a.tiles - 1 - (unit - kvh * a.tiles);
     seq = __builtin_amdgcn_readfirstlane(seq_of_tile(a, tile));
     const ChunkTile t = chunk_tile(a.shape, load_seq(a, seq),
                                    tile - chunk_base(a.shape, chunk_clamp(a.starts[seq], a.shape.n_tokens), seq));
@@ -376,9 +381,27 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
     deal->seq = seq;
     deal->again = 0;
   }
+  __syncthreads();
   ChunkAt at{x, x1, base, tile, kvh, seq};
   ChunkUnitAt u;
-  while (next_unit(a, at, u)) {
+  // A share's first unit, where it is the rest of one whose start another workgroup has, comes last: the
+  // workgroups of an XCD, each with the end of one tile and the start of the next, then go over the
+  // same keys at the same time.
+  int32_t first_end = -1;   // where that unit ends; -1: none is left over
+  bool begun = false;
+  for (;;) {
+    if (!next_unit(a, at, u)) {
+      if (first_end < 0) break;
+      at = {sgpr(deal->x), first_end, sgpr(deal->base), sgpr(deal->first_tile), sgpr(deal->kvh), sgpr(deal->seq)};
+      first_end = -1;
+      if (!next_unit(a, at, u)) break;
+    } else if (!begun) {
+      begun = true;
+      if (u.b0 > 0 && at.x < at.x1) {
+        first_end = at.x;
+        continue;
+      }
+    }
     const ChunkTile& tl = u.tile;
     const int32_t b0 = u.b0, b1 = u.b1, n_blocks = tl.blocks, len = u.seq.len, rows = tl.rows, kvh = at.kvh;
     const bool whole = b0 == 0 && b1 >= n_blocks;
@@ -397,7 +420,7 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
 
     u32x4 qf[kKK];
     {
-      const uint16_t* qrow = a.q + q_off + 8 * g;
+      const uint16_t* qrow = Q + q_off + 8 * g;
 #pragma unroll
       for (int kk = 0; kk < kKK; ++kk) {
         u32x4 w = {0u, 0u, 0u, 0u};
@@ -417,45 +440,47 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
       return e >= b0 && e < b1 && k0 <= pw1 && (k0 + kNK - 1 > pw0 - win || k0 < sinks);
     };
 
-    // ---- page numbers: lane's key of an entry (past the part: of its last) ----
-    auto ids_of = [&](int e) {
-      const int key = block_of(min(e, b1 - 1)) * kNK + (lane & (kNK - 1));
-      return table[min(key, len - 1) >> a.page_shift];
+    // ---- where an entry's keys lie, a key a lane (past the part: its last entry's) ----
+    auto key_of = [&](int e) { return block_of(min(e, b1 - 1)) * kNK + (lane & (kNK - 1)); };
+    auto ids_of = [&](int e) { return table[min(key_of(e), len - 1) >> a.page_shift]; };
+    struct Keys {
+      uint32_t lo;   // byte offset of the key's row
+      int32_t hi;    // below 0: no such page
     };
-    auto pages_there = [&](int32_t id) {   // of the entry's keys; past the last key it does not count
-      return __builtin_amdgcn_ballot_w64((uint32_t)id < (uint32_t)a.num_pages);
+    auto keys_at = [&](int e, int32_t id) {
+      const uint64_t off = ((uint64_t)(uint32_t)id * (uint64_t)a.page_stride +
+                            (((uint64_t)kvh << a.page_shift) + (uint32_t)(key_of(e) & page_mask)) * (uint32_t)d) * kEs;
+      return Keys{(uint32_t)off, (uint32_t)id < (uint32_t)a.num_pages ? (int32_t)(off >> 32) : -1};
     };
+    // of the entry's keys those whose page is there (past the last key: as the last)
+    auto pages_there = [&](const Keys& k) { return __builtin_amdgcn_ballot_w64(k.hi >= 0); };
 
     // ---- K and V of an entry to a stage ----
-    auto dma = [&](const uint8_t* from, const int (&voff)[kDmaPerWave], uint8_t* to, int e, int32_t id) {
-      const int key0 = block_of(min(e, b1 - 1)) * kNK;
+    auto dma = [&](const uint8_t* from, const int (&voff)[kDmaPerWave], uint8_t* to, int e, const Keys& k) {
+      const int end = len - block_of(min(e, b1 - 1)) * kNK;   // of the sequence's keys, from the entry's first
 #pragma unroll
       for (int i = 0; i < kDmaPerWave; ++i) {
         const int row0 = kDmaRows * (wave + kWG * i);
-        const int32_t page = __builtin_amdgcn_readlane(id, row0);
-        const bool ok = (uint32_t)page < (uint32_t)a.num_pages;
-        const int left = __builtin_amdgcn_readfirstlane(ok ? min(max(len - key0 - row0, 0), kDmaRows) : 0);
-        const int64_t at = (int64_t)(ok ? page : 0) * a.page_stride +
-                           (((int64_t)kvh << a.page_shift) + ((key0 + row0) & page_mask)) * d;
+        const int hi = __builtin_amdgcn_readlane(k.hi, row0);
+        const uint64_t at = (uint64_t)(uint32_t)hi << 32 | (uint32_t)__builtin_amdgcn_readlane((int)k.lo, row0);
+        const int rows_in = sgpr(min(max(end - row0, 0), kDmaRows));
         const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(from + at * 2), (short)0, left * row_b, 0x00020000);
+            (void*)(from + at), (short)0, hi < 0 ? 0 : rows_in * row_b, 0x00020000);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(to + (wave + i * kWG) * 1024), 16, voff[i], 0, 0, 0);
       }
     };
     // through registers: thread t takes chunks t, t + 256, .. of the block's rows
     u32x4 stage_k[kLoads], stage_v[kLoads];
-    auto fetch = [&](const uint8_t* from, u32x4 (&to)[kLoads], int e, int32_t id) {
+    auto fetch = [&](const uint8_t* from, u32x4 (&to)[kLoads], int e, const Keys& k) {
+      const int end = len - block_of(min(e, b1 - 1)) * kNK;
       constexpr int kPer = kDp / kLoadElems;   // loads of a row
-      const int key0 = block_of(min(e, b1 - 1)) * kNK;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = (tid + 256 * i) / kPer, ch = (tid + 256 * i) % kPer;
-        const int32_t page = __shfl(id, row);
-        const int64_t at = (int64_t)page * a.page_stride + (((int64_t)kvh << a.page_shift) + ((key0 + row) & page_mask)) * d +
-                           ch * kLoadElems;
+        const int hi = __shfl(k.hi, row);
+        const uint64_t at = (uint64_t)(uint32_t)hi << 32 | (uint32_t)__shfl((int)k.lo, row);
         u32x4 w = {0u, 0u, 0u, 0u};
-        if ((uint32_t)page < (uint32_t)a.num_pages && key0 + row < len && ch * kLoadElems < d)
-          w = *reinterpret_cast<const u32x4*>(from + at * kEs);
+        if (hi >= 0 && row < end && ch * kLoadElems < d) w = *reinterpret_cast<const u32x4*>(from + at + ch * 16);
         to[i] = w;
       }
     };
@@ -478,13 +503,13 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
     };
     auto k_stage = [&](int s) { return smem + s * kStageB; };
     auto v_stage = [&](int s) { return smem + s * kStageB + kTileB; };
-    auto begin_k = [&](int e, int stage, int32_t id) {
-      if constexpr (kSrc == kDma) dma(a.k, k_voff, k_stage(stage), e, id);
-      else fetch(a.k, stage_k, e, id);
+    auto begin_k = [&](int e, int stage, const Keys& k) {
+      if constexpr (kSrc == kDma) dma(K, k_voff, k_stage(stage), e, k);
+      else fetch(K, stage_k, e, k);
     };
-    auto begin_v = [&](int e, int stage, int32_t id) {
-      if constexpr (kSrc == kDma) dma(a.v, v_voff, v_stage(stage), e, id);
-      else fetch(a.v, stage_v, e, id);
+    auto begin_v = [&](int e, int stage, const Keys& k) {
+      if constexpr (kSrc == kDma) dma(V, v_voff, v_stage(stage), e, k);
+      else fetch(V, stage_v, e, k);
     };
     auto end_k = [&](int stage) {
       if constexpr (kSrc != kDma) commit(stage_k, k_stage(stage), false);
@@ -560,18 +585,36 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
     if (nb > 0 && n_blocks > 0) {
       // K_0, K_1 and, for the empty PV_{-1}, a V tile in stage 1: P_{-1} = 0 meets V_0, whose NaN a
       // seen row may well hold only in a masked key; such rows are taken again in any case
-      int32_t id0 = ids_of(b0), id1 = ids_of(b0 + 1), id2 = ids_of(b0 + 2);
-      begin_k(b0, 0, id0);
-      begin_v(b0, 1, id0);
+      const int32_t id0 = ids_of(b0), id1 = ids_of(b0 + 1), id2 = ids_of(b0 + 2);
+      int32_t id3 = ids_of(b0 + 3);
+      Keys keys0 = keys_at(b0, id0), keys1 = keys_at(b0 + 1, id1), keys2 = keys_at(b0 + 2, id2);
+      begin_k(b0, 0, keys0);
+      begin_v(b0, 1, keys0);
       end_k(0);
       end_v(1);
-      begin_k(b0 + 1, 1, id1);
+      begin_k(b0 + 1, 1, keys1);
       end_k(1);
       __syncthreads();
       f32x16 sa[kST], sb[kST];
       if (active) s_block(0, sa);
       __syncthreads();
 
+      auto loads = [&](int e, int stage) {
+        begin_k(e + 2, stage, keys2);
+        begin_v(e, stage, keys0);
+        keys0 = keys1;
+        keys1 = keys2;
+        keys2 = keys_at(e + 3, id3);
+        id3 = ids_of(e + 4);
+      };
+      if (!active) {   // a wave without rows loads its share only
+        for (int j = 0; j < nb; ++j) {
+          loads(b0 + j, j & 1);
+          end_k(j & 1);
+          end_v(j & 1);
+          __syncthreads();
+        }
+      } else {
       auto softmax_block = [&](int j, auto masked, uint64_t there, f32x16 (&s)[kST], u32x4 (&pnew)[kPN]) {
         constexpr bool kMasked = decltype(masked)::value;
         if constexpr (kMasked) {
@@ -641,13 +684,10 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
         constexpr int kS = decltype(stage_c)::value;
         constexpr bool kMasked = decltype(masked)::value;
         const int e = b0 + j;
-        const uint64_t there = kMasked ? pages_there(id0) : 0;
-        begin_k(e + 2, kS, id2);
-        begin_v(e, kS, id0);
-        id0 = id1;
-        id1 = id2;
-        id2 = ids_of(e + 3);
-        if (active && (!kMasked || wave_sees(e - 1) || wave_sees(e) || wave_sees(e + 1))) {
+        const uint64_t there = kMasked ? pages_there(keys0) : 0;
+        loads(e, kS);
+        // (the unmasked form without a branch: behind one the compiler waits for the loads first)
+        if (!kMasked || wave_sees(e - 1) || wave_sees(e) || wave_sees(e + 1)) {
           mma_block(kS ^ 1, snext, pprev, oacc);
           softmax_block(j, masked, there, scur, pnew);
         } else {
@@ -675,13 +715,14 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
       const int j0 = min((max(whole0 - b0, 0) + 1) / 2 * 2, nb), j1 = max((min(whole1, b1) - b0) / 2 * 2, j0);
       masked_pairs(0, j0);
       int j = j0;
-      for (; j < j1 && (pages_there(id0) & pages_there(id1)) == ~0ull; j += 2) {
+      for (; j < j1 && (pages_there(keys0) & pages_there(keys1)) == ~0ull; j += 2) {
         iteration(j, Z{}, std::false_type{}, sa, sb, pa, pb);
         iteration(j + 1, One{}, std::false_type{}, sb, sa, pb, pa);
       }
       masked_pairs(j, nb);
       // PV of the last block (nb is even: P_{nb-1} is in pa, V_{nb-1} in stage 1)
-      if (active && wave_sees(b0 + nb - 1)) pv_block(1, pa, oacc);
+      if (wave_sees(b0 + nb - 1)) pv_block(1, pa, oacc);
+      }
     }
 
     // ---- the end of the unit ----
@@ -709,7 +750,7 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, uint8_t* smem, Ch
       const bool none = len - u.seq.tokens + tk < 0;   // no key: zeros
       const float inv = none ? 0.0f : a.v_scale / l;
       float z = none ? 0.0f : l * inv * 0.0f;
-      uint16_t* orow = a.o + (int64_t)(u.seq.start + tk) * a.ldo + (int64_t)hd * d;
+      uint16_t* orow = O + (int64_t)(u.seq.start + tk) * a.ldo + (int64_t)hd * d;
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt)
 #pragma unroll
@@ -826,12 +867,14 @@ __device__ __forceinline__ void chunk_join(const ChunkArgs& a, ChunkLds* deal) {
 
 }  // namespace
 
+// One LDS array for all of it, and the operands as restrict pointers: else (two arrays have an alias scope
+// each; without restrict the transposing reads have none at all) the compiler takes every read of LDS for one of
+// what a DMA has just been told to write, and waits for the next blocks before the products of this one.
 // d<D>: head dimensions up to D; s: pages below a DMA instruction's keys
 #define SILE_CHUNK_KERNEL(NAME, BF, SRC, EU, NK, DH, DP)                                  \
   extern "C" __global__ __launch_bounds__(256, EU) void NAME(ChunkArgs a) {               \
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * 2 * NK * 2 * DP];          \
-    __shared__ ChunkLds deal;                                                             \
-    chunk_attn<BF, SRC, NK, DH, DP>(a, smem, &deal);                                      \
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * 2 * NK * 2 * DP + sizeof(ChunkLds)]; \
+    chunk_attn<BF, SRC, NK, DH, DP>(a, a.q, a.k, a.v, a.o, smem, reinterpret_cast<ChunkLds*>(smem + 2 * 2 * NK * 2 * DP)); \
   }
 #define SILE_CHUNK_JOIN(NAME, BF, F8, DH)                                     \
   extern "C" __global__ __launch_bounds__(256) void NAME(ChunkArgs a) {       \

@@ -594,7 +594,7 @@ int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n
   void* params[] = {&a};
   const int64_t units = tiles * kv_heads;
   a.direct = seen <= 512;
-  int64_t grid = a.direct ? units : plan.groups;
+  int64_t grid = a.direct ? (units + 7) / 8 * 8 : plan.groups;
   if (!a.direct) {
     const int64_t most = (tiles * unit * kv_heads + sile::kChunkShare + sile::kChunkUnit - 1) / (sile::kChunkShare + sile::kChunkUnit);
     grid = std::min(grid, (most + 7) / 8 * 8);
