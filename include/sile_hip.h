@@ -661,8 +661,8 @@ int sile_hip_rope_turns(sile_rope_scaling scaling, int64_t rot_dim, double base,
  * x = 2 pi turns[j] positions[t] (turns: device, 64 bits, kept there to its fraction of a turn),
  *   (a, b) -> magnitude * (a cos x - b sin x, b cos x + a sin x),
  * and dims from rot_dim on are copied; fp32, rounded once.  Negative turns turn back.  dtype f32, f16
- * or bf16; tokens at q + t * ldq, k + t * ldk, [heads][head_dim], any alignment and head_dim up to
- * 2048 (16-byte aligned and rot_dim a multiple of 16 is fastest); q_heads or kv_heads may be
+ * or bf16; tokens at q + t * ldq, k + t * ldk, [heads][head_dim] (leading dimensions up to 2^25), any
+ * alignment and head_dim up to 2048 (16-byte aligned and rot_dim a multiple of 16 is fastest); q_heads or kv_heads may be
  * 0.  An output is its input (same pointer and leading dimension) or apart from it.  A token
  * at a position below 0 is left out: its outputs stay as they are. */
 int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, int64_t q_heads,

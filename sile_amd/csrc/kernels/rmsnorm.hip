@@ -125,6 +125,7 @@ SILE_DEV void norm_rows(const NormArgs& a) {
     if (a.weight && 8 * (v * kThreads + tid) < cols) wv[v].load(a.weight, 8 * (v * kThreads + tid));
   int turn = 0;
   constexpr int kRows = kWg / kThreads;
+  const int groups = a.group > 0 ? cols / a.group : 0;
   for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / kThreads; r < a.rows;
        r += (int64_t)gridDim.x * kRows, turn ^= 1) {
     Vec<kType> xv[kV], rv[kV];
@@ -192,14 +193,23 @@ SILE_DEV void norm_rows(const NormArgs& a) {
           for (int j = 0; j < 8; ++j) m = __builtin_fmaxf(m, __builtin_fabsf(s[v][j]));
           scale = scale_of(lanes_max(m, a.group / 8));
           rcp = rcp_of(scale);
-          if (c < cols && c % a.group == 0) a.scales[r * (cols / a.group) + c / a.group] = scale;
+          if (c < cols && tid % (a.group / 8) == 0) a.scales[r * groups + c / 8 * 8 / a.group] = scale;
         }
         if (c < cols) {
           float f[8];
+          // a group's own scale leaves no quotient past 448 but by a rounding, which the code takes back
+          if (a.group != 0 && rcp != 0.0f) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[j] = e4m3_in(s[v][j], scale, rcp);
+            for (int j = 0; j < 8; ++j) {
+              const float q = s[v][j] * rcp;
+              f[j] = __builtin_fmaf(__builtin_fmaf(-q, scale, s[v][j]), rcp, q);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = e4m3_in(s[v][j], scale, rcp);
+          }
           const u32x2 out = {e4m3_pack4(f), e4m3_pack4(f + 4)};
-          *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.y) + r * a.ldy + c) = out;
+          __builtin_nontemporal_store(out, reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.y) + r * a.ldy + c));
         }
       }
     }

@@ -35,6 +35,11 @@ struct RopeArgs {
   int32_t q_heads, kv_heads, d, rot, num_pages, page_shift, n_rows;
   int32_t per_group;                // tokens of a workgroup
   int32_t rot_items, head_items, items;   // of a head's rotated dims, of a head, of a token
+  int32_t value_items;              // of a head of values
+  int32_t past;                     // 1: the queries' stores past the caches
+  int32_t head_shift, value_shift;  // log2 of head_items and value_items, -1: no powers of two
+  int32_t k_exact, v_exact;         // 1: x * rcp is x / scale (the scale is a power of two)
+  float inv_head, inv_items, inv_value;   // 1 / head_items, items, value_items
   float magnitude, k_scale, v_scale, k_rcp, v_rcp;
 };
 
@@ -89,6 +94,20 @@ SILE_DEV void rope(const RopeArgs& a) {
   const int n = tokens * a.items;
   const int first = blockIdx.y * (256 * kItems);
 
+  // n / by for n below 2^24 (inv: 1 / by, so the product's whole part is off by one at most)
+  auto divide = [](int n, int by, float inv, int* rest) {
+    int q = (int)((float)n * inv);
+    int m = n - q * by;
+    if (m < 0) {
+      --q;
+      m += by;
+    } else if (m >= by) {
+      ++q;
+      m -= by;
+    }
+    *rest = m;
+    return q;
+  };
   // item i: token, head (queries', then keys', then values'), its two vectors' dims
   struct Item {
     int tok, head, o0, o1, pair;   // pair: of the first dim, -1 where nothing turns
@@ -96,18 +115,27 @@ SILE_DEV void rope(const RopeArgs& a) {
   };
   auto item = [&](int i) {
     Item m;
-    m.tok = i / a.items;
-    const int r = i - m.tok * a.items;
+    int r = i, c;
+    m.tok = a.per_group == 1 ? 0 : divide(i, a.items, a.inv_items, &r);
     const int turned = (a.q_heads + a.kv_heads) * a.head_items;
-    int c;
     m.two = true;
     if (r < turned) {
-      m.head = r / a.head_items;
-      c = r - m.head * a.head_items;
+      if (a.head_shift >= 0) {
+        m.head = r >> a.head_shift;
+        c = r & (a.head_items - 1);
+      } else {
+        m.head = divide(r, a.head_items, a.inv_head, &c);
+      }
     } else {   // a value's head has only dims that stay
-      const int per = (a.d + 2 * kE - 1) / (2 * kE), u = r - turned;
-      m.head = a.q_heads + a.kv_heads + u / per;
-      c = a.rot_items + u % per;
+      r -= turned;
+      if (a.value_shift >= 0) {
+        m.head = r >> a.value_shift;
+        c = r & (a.value_items - 1);
+      } else {
+        m.head = divide(r, a.value_items, a.inv_value, &c);
+      }
+      m.head += a.q_heads + a.kv_heads;
+      c += a.rot_items;
     }
     if (c < a.rot_items) {
       m.pair = c * kE;
@@ -121,12 +149,19 @@ SILE_DEV void rope(const RopeArgs& a) {
     }
     return m;
   };
+  // (offsets from the workgroup's first token fit 32 bits)
+  const uint8_t* const qb = static_cast<const uint8_t*>(a.q) + t0 * a.ldq * kEs;
+  const uint8_t* const kb = static_cast<const uint8_t*>(a.k) + t0 * a.ldk * kEs;
+  const uint8_t* const vb = static_cast<const uint8_t*>(a.v) + t0 * a.ldv * kEs;
+  uint8_t* const qo = static_cast<uint8_t*>(a.q_out) + t0 * a.ldqo * kEs;
+  uint8_t* const ko = static_cast<uint8_t*>(a.k_out) + (kCache == 0 ? t0 * a.ldko * kEs : 0);
+  const uint32_t ldq = (uint32_t)a.ldq, ldk = (uint32_t)a.ldk, ldv = (uint32_t)a.ldv, ldqo = (uint32_t)a.ldqo, ldko = (uint32_t)a.ldko;
+  // key or value head of an item's head
   auto source = [&](const Item& m) -> const uint8_t* {
-    const int64_t t = t0 + m.tok;
-    if (m.head < a.q_heads) return static_cast<const uint8_t*>(a.q) + (t * a.ldq + (int64_t)m.head * a.d) * kEs;
-    if (m.head < a.q_heads + a.kv_heads)
-      return static_cast<const uint8_t*>(a.k) + (t * a.ldk + (int64_t)(m.head - a.q_heads) * a.d) * kEs;
-    return static_cast<const uint8_t*>(a.v) + (t * a.ldv + (int64_t)(m.head - a.q_heads - a.kv_heads) * a.d) * kEs;
+    if (m.head < a.q_heads) return qb + (m.tok * ldq + (uint32_t)m.head * a.d) * kEs;
+    const int u = m.head - a.q_heads;
+    if (u < a.kv_heads) return kb + (m.tok * ldk + (uint32_t)u * a.d) * kEs;
+    return vb + (m.tok * ldv + (uint32_t)(u - a.kv_heads) * a.d) * kEs;
   };
 
   V raw[kItems][2];
@@ -197,8 +232,21 @@ SILE_DEV void rope(const RopeArgs& a) {
       const float scale = is_v ? a.v_scale : a.k_scale, rcp = is_v ? a.v_rcp : a.k_rcp;
       uint8_t* to = static_cast<uint8_t*>(is_v ? a.v_out : a.k_out) + slot_off[m.tok] +
                     ((int64_t)head << a.page_shift) * a.d;
+      if (is_v ? a.v_exact : a.k_exact) {
 #pragma unroll
-      for (int e = 0; e < 2 * kE; ++e) x[e] = e4m3_in(x[e], scale, rcp);
+        for (int e = 0; e < 2 * kE; ++e) {
+          const float y = x[e] * rcp;
+          x[e] = y != y ? y : __builtin_amdgcn_fmed3f(y, -448.0f, 448.0f);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2 * kE; ++e) x[e] = e4m3_in(x[e], scale, rcp);
+      }
+      if (kE == 8 && m.two && m.o1 == m.o0 + kE && (m.o0 & 15) == 0) {
+        const u32x4 out = {e4m3_pack4(x), e4m3_pack4(x + 4), e4m3_pack4(x + 8), e4m3_pack4(x + 12)};
+        __builtin_nontemporal_store(out, reinterpret_cast<u32x4*>(to + m.o0));
+        continue;
+      }
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint8_t* w = to + (half ? m.o1 : m.o0);
@@ -216,9 +264,9 @@ SILE_DEV void rope(const RopeArgs& a) {
     }
     uint8_t* to;
     if (is_q)
-      to = static_cast<uint8_t*>(a.q_out) + ((t0 + m.tok) * a.ldqo + (int64_t)m.head * a.d) * kEs;
+      to = qo + (m.tok * ldqo + (uint32_t)m.head * a.d) * kEs;
     else if (kCache == 0)
-      to = static_cast<uint8_t*>(a.k_out) + ((t0 + m.tok) * a.ldko + (int64_t)(m.head - a.q_heads) * a.d) * kEs;
+      to = ko + (m.tok * ldko + (uint32_t)(m.head - a.q_heads) * a.d) * kEs;
     else
       to = static_cast<uint8_t*>(is_v ? a.v_out : a.k_out) +
            (slot_off[m.tok] + ((int64_t)(m.head - a.q_heads - (is_v ? a.kv_heads : 0)) << a.page_shift) * a.d) * kEs;
@@ -236,7 +284,7 @@ SILE_DEV void rope(const RopeArgs& a) {
     for (int half = 0; half < 2; ++half) {
       if (half && !m.two) break;
       V* w = reinterpret_cast<V*>(to + (half ? m.o1 : m.o0) * kEs);
-      if (cached)
+      if (cached || a.past)
         __builtin_nontemporal_store(out[half], w);
       else
         *w = out[half];

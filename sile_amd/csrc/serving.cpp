@@ -27,8 +27,9 @@ struct RopeArgs {
   const int32_t *rows, *positions, *tables;
   const double* turns;
   int64_t tokens, ldq, ldk, ldv, ldqo, ldko, page_stride, ld_table, capacity;
-  int32_t q_heads, kv_heads, d, rot, num_pages, page_shift, n_rows, per_group, rot_items, head_items, items;
-  float magnitude, k_scale, v_scale, k_rcp, v_rcp;
+  int32_t q_heads, kv_heads, d, rot, num_pages, page_shift, n_rows, per_group, rot_items, head_items, items,
+      value_items, past, head_shift, value_shift, k_exact, v_exact;
+  float inv_head, inv_items, inv_value, magnitude, k_scale, v_scale, k_rcp, v_rcp;
 };
 constexpr int64_t kRopeItems = 1024, kRopeTokens = 16, kRopeAngles = 1024;   // of a workgroup
 struct NormArgs {
@@ -103,8 +104,20 @@ int launch_rope(sile_dtype dtype, sile_rope_layout layout, const char* cache, bo
   const int64_t e = rope_width((int64_t)dtype_bytes(dtype), *a);
   a->rot_items = (int32_t)(a->rot / (2 * e));
   a->head_items = (int32_t)(a->rot_items + (a->d - a->rot + 2 * e - 1) / (2 * e));
-  a->items = (a->q_heads + a->kv_heads) * a->head_items +
-             (values ? a->kv_heads * (int32_t)((a->d + 2 * e - 1) / (2 * e)) : 0);
+  a->value_items = (int32_t)((a->d + 2 * e - 1) / (2 * e));
+  a->items = (a->q_heads + a->kv_heads) * a->head_items + (values ? a->kv_heads * a->value_items : 0);
+  if (a->items > (1 << 23)) return fail(SILE_ERR_SHAPE, "too many heads of %d dims", a->d);
+  a->inv_head = 1.0f / (float)a->head_items;
+  a->inv_items = 1.0f / (float)a->items;
+  a->inv_value = 1.0f / (float)a->value_items;
+  auto log2_of = [](int32_t n) { return n > 0 && (n & (n - 1)) == 0 ? __builtin_ctz((unsigned)n) : -1; };
+  a->head_shift = log2_of(a->head_items);
+  a->value_shift = log2_of(a->value_items);
+  auto power = [](float x) { int e; return std::frexp(std::fabs(x), &e) == 0.5f && std::fabs(x) >= 0x1p-60f && std::fabs(x) <= 0x1p60f; };
+  a->k_exact = power(a->k_scale);
+  a->v_exact = power(a->v_scale);
+  // queries and keys that the caches cannot hold anyway go past them
+  a->past = a->tokens * (a->q_heads + a->kv_heads) * a->d * (int64_t)dtype_bytes(dtype) > (32 << 20);
   const int64_t angles = std::max(1, a->rot / 2);
   // enough tokens for one item a thread and more where there are tokens for all CUs
   int64_t per = std::min({kRopeItems / a->items, kRopeTokens, kRopeAngles / angles});
@@ -196,7 +209,8 @@ int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, i
       (kv_heads > 0 && (ldk < kv_heads * head_dim || ldko < kv_heads * head_dim)))
     return fail(SILE_ERR_SHAPE, "leading dimension smaller than a token's heads");
   const int64_t es = (int64_t)dtype_bytes(dtype), nq = q_heads * head_dim, nk = kv_heads * head_dim;
-  if (std::max({ldq, ldqo, ldk, ldko}) > (1ll << 40) / n_tokens * 64) return fail(SILE_ERR_SHAPE, "leading dimension too large");
+  // (a workgroup's offsets, of up to 16 tokens, are counted in 32 bits)
+  if (std::max({ldq, ldqo, ldk, ldko}) > (1 << 25)) return fail(SILE_ERR_SHAPE, "leading dimension past 2^25");
   for (const void* p : {q, (const void*)q_out, k, (const void*)k_out})
     if (!aligned_to(p, es)) return fail(SILE_ERR_SHAPE, "tokens not aligned to their type");
   if ((q_heads > 0 && !in_place_or_apart(q, ldq, q_out, ldqo, n_tokens, nq, es)) ||
@@ -246,7 +260,7 @@ int sile_hip_rope_append(sile_dtype dtype, sile_dtype cache_type, sile_rope_layo
   const int64_t nq = q_heads * head_dim, nk = kv_heads * head_dim;
   if ((q_heads > 0 && (ldq < nq || ldqo < nq)) || ldk < nk || ldv < nk)
     return fail(SILE_ERR_SHAPE, "leading dimension smaller than a token's heads");
-  if (std::max({ldq, ldqo, ldk, ldv}) > (1ll << 40) / n_tokens * 64) return fail(SILE_ERR_SHAPE, "leading dimension too large");
+  if (std::max({ldq, ldqo, ldk, ldv}) > (1 << 25)) return fail(SILE_ERR_SHAPE, "leading dimension past 2^25");
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || ldk % 8 || ldv % 8 ||
       (q_heads > 0 && (!aligned16(q) || !aligned16(q_out) || ldq % 8 || ldqo % 8)))
     return fail(SILE_ERR_SHAPE, "tokens and pages have to be 16-byte aligned");
