@@ -85,6 +85,12 @@ SILE_HD void chunk_whole(const ChunkShape& s, const ChunkTile& t, int32_t* whole
 // What a unit counts.
 SILE_HD int32_t chunk_size(const ChunkTile& t) { return t.rows > 0 ? t.blocks + kChunkUnit : 0; }
 
+// What the attention's launch leaves of a tile for the one that joins its parts: the blocks before
+// it, its sequence, that one's first tile, and its rows.
+struct ChunkRec {
+  int32_t at, seq, first, rows;
+};
+
 // The shares of `total` blocks for `groups` workgroups.
 SILE_HD int64_t chunk_share(int64_t total, int32_t groups) {
   const int64_t per = (total + groups - 1) / groups;
@@ -109,12 +115,13 @@ SILE_HD int32_t sgpr(int32_t v) {
 template <class A>
 SILE_HD int32_t seq_of_tile(const A& a, int32_t t) {
   int32_t lo = 0, hi = a.shape.n_rows;   // base(lo) <= t < base(hi)
-  while (hi - lo > 1) {
-    const int32_t mid = (lo + hi) >> 1;
-    if (chunk_base(a.shape, chunk_clamp(a.starts[mid], a.shape.n_tokens), mid) <= t)
-      lo = mid;
-    else
-      hi = mid;
+  while (hi - lo > 1) {   // (in nine parts: their loads do not wait for one another)
+    const int32_t step = (hi - lo + 8) / 9, from = lo;
+    for (int32_t i = 1; i < 9; ++i) {
+      const int32_t r = from + i * step < hi ? from + i * step : hi - 1;
+      if (chunk_base(a.shape, chunk_clamp(a.starts[r], a.shape.n_tokens), r) <= t && r > lo) lo = r;
+    }
+    hi = lo + step < hi ? lo + step : hi;
   }
   return lo;
 }
@@ -171,7 +178,7 @@ SILE_HD bool next_unit(const A& a, ChunkAt& at, ChunkUnitAt& u) {
   return false;
 }
 
-// visit(t, size of tile t) for c0 <= t < c1, in order
+// visit(t, size of tile t, its sequence, that one's first tile, tile t's rows) for c0 <= t < c1, in order
 template <class A, class F>
 SILE_HD void chunk_run(const A& a, int32_t c0, int32_t c1, F&& visit) {
   if (c0 >= c1) return;
@@ -186,7 +193,8 @@ SILE_HD void chunk_run(const A& a, int32_t c0, int32_t c1, F&& visit) {
       q = load_seq(a, r);
       first = next;
     }
-    visit(t, chunk_size(chunk_tile(a.shape, q, t - first)));
+    const ChunkTile tile = chunk_tile(a.shape, q, t - first);
+    visit(t, chunk_size(tile), r, first, tile.rows);
   }
 }
 

@@ -25,12 +25,18 @@
 //  * Workgroups of one XCD take a contiguous run of the list, key head by key head, so that tiles of a
 //    sequence read its keys from that XCD's L2.
 //  * Rows past the tile's last and waves without any compute nothing and store nothing.
+//  * A tile of at most 32 rows (single tokens, drafts) has another code: each wave takes every fourth key block
+//    for all of its rows, with no barrier, and the four results are joined in LDS.
 //  * A row whose result is not finite (Inf or NaN in a masked key's V makes it so: 0 times it) is
 //    taken again by the workgroup over its seen keys, in fp32.
 //
 // The probabilities enter the product in 16 bits (half a step, 2^-8 of each in bf16, 2^-11 in f16,
 // their sum is of the rounded ones); f16 ones carry a factor 2^7 beside the up to 2^8 that the lazy
 // maximum allows, so that those far below the maximum keep their bits.
+//
+// Measured, 32 query heads of 128 over 8 key heads: 2048 tokens behind 30000 keys 1.19 ms (875 TFLOP/s, the
+// matrix cores and their power), 8192 from none 0.71 ms; 32 pieces of 8 tokens over up to 8192 keys 130 us
+// (4.3 TB/s; a key more costs its bytes at 5.1 TB/s), as e4m3 codes 90 us; 1 piece of 4 over 300 13 us.
 #include <type_traits>
 
 #include "common.h"
@@ -94,7 +100,7 @@ struct ChunkArgs {
   const int32_t* starts;
   const int32_t* tables;
   const int32_t* lengths;
-  int32_t* plan;         // workspace: blocks of a key head's tiles before each tile, then of all
+  ChunkRec* plan;        // workspace: of a key head's tiles, then all of its blocks
   float* parts;          // workspace: [slots][4 waves][4 d-tiles x 4 + 1][64 lanes][4]
   int64_t ldq, ldo, page_stride, ld_table;
   ChunkShape shape;
@@ -108,7 +114,7 @@ struct ChunkArgs {
 
 struct ChunkLds {
   int64_t wave_sum[4];
-  int32_t tile, before;
+  int32_t tile, before, rows;   // the share's first tile
   int32_t x, x1, base;   // the workgroup's share, for chunk_again
   int32_t first_tile, kvh, seq;
   int32_t again;         // rows that are not finite: 1 in a tile of its own, in the join their bits
@@ -136,10 +142,10 @@ SILE_DEV void load8(const uint8_t* p, float* f) {
 
 // One query row, at position p, of sequence `seq`, by the workgroup, in fp32 and over the seen
 // keys only.  A wave takes every fourth 64 keys: a lane a key's score, then 8 dims of 2 keys at a
-// time; the waves' sums are joined through LDS.
+// time; the waves' sums are joined through LDS.  Its dims dim0 .. dim1 - 1 are stored.
 template <bool kBF16, bool kFp8>
 SILE_DEV void chunk_row(const ChunkArgs& a, int32_t seq, int kvh, int32_t p, const uint16_t* q, uint16_t* o,
-                                       ChunkLds* lds) {
+                        int dim0, int dim1, ChunkLds* lds) {
   constexpr int kEs = kFp8 ? 1 : 2;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = a.d;
   const KeySpan span = key_span(p + 1, a.shape.capacity, a.shape.window, a.shape.sinks);
@@ -217,7 +223,7 @@ SILE_DEV void chunk_row(const ChunkArgs& a, int32_t seq, int kvh, int32_t p, con
       any = (uint32_t)table[key >> a.page_shift] < (uint32_t)a.num_pages;
     }
     r = any ? r * (a.v_scale / sum) : 0.0f;
-    o[threadIdx.x] = kBF16 ? bf16_rne(r) : f16_rne(r);
+    if ((int)threadIdx.x >= dim0 && (int)threadIdx.x < dim1) o[threadIdx.x] = kBF16 ? bf16_rne(r) : f16_rne(r);
   }
   __syncthreads();
 }
@@ -241,7 +247,7 @@ SILE_DEV void chunk_again(const ChunkArgs& a, ChunkLds* lds) {
       for (int c = lane; c < a.d; c += 64) bad |= (o[c] & kExp) == kExp;
       if (__builtin_amdgcn_ballot_w64(bad) != 0)
         chunk_row<kBF16, kFp8>(a, at.seq, at.kvh, u.seq.len - u.seq.tokens + token,
-                               a.q + t * a.ldq + (int64_t)head * a.d, o, lds);
+                               a.q + t * a.ldq + (int64_t)head * a.d, o, 0, a.d, lds);
     }
   }
 }
@@ -256,10 +262,17 @@ enum Source { kDma = 0, kStaged = 1, kCodes = 2 };
 template <int kDh>
 constexpr int kPartFloats = 4 * (4 * (kDh / 32) + 1) * 64 * 4;
 
-template <bool kBF16, Source kSrc, int kNK, int kDh, int kDp>
-__device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* __restrict__ Q, const uint8_t* __restrict__ K,
-                                           const uint8_t* __restrict__ V, uint16_t* __restrict__ O, uint8_t* smem,
-                                           ChunkLds* deal) {
+// Whether units of at most 32 rows have a code of their own.  (Not staged 16-bit keys, whose loads of a wave's
+// block take 64 registers: 32 pieces of 8 over up to 8192 keys, a page each, 173 us for 151.)
+template <Source kSrc>
+constexpr bool kOwnTiles = kSrc != kStaged;
+
+// This workgroup's units of more than 32 rows, or (kNarrow) those of at most 32: two codes, each with the
+// registers to itself.  True: it has units of the other kind.
+template <bool kBF16, Source kSrc, int kNK, int kDh, int kDp, bool kNarrow>
+__device__ __forceinline__ bool chunk_units(const ChunkArgs& a, const uint16_t* __restrict__ Q, const uint8_t* __restrict__ K,
+                                            const uint8_t* __restrict__ V, uint16_t* __restrict__ O, uint8_t* smem,
+                                            ChunkLds* deal) {
   constexpr int kWG = 4;
   constexpr int kST = kNK / 32;
   constexpr int kRow = 2 * kDp;          // bytes of a K or V row in LDS
@@ -276,79 +289,14 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
   constexpr int kLoads = kNK * kDp / kLoadElems / 256;       // staged loads of a thread
   static_assert(kDh % 32 == 0 && kDh <= kDp && (kDp == 64 || kDp == 128 || kDp == 256), "row width");
   static_assert((kNK == 32 || kNK == 64) && kDmaPerWave >= 1 && kLoads >= 1, "tiles in 1 KiB slices over the waves");
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // (the thread's number through an empty asm: what the two codes work out from it is not kept from one
+  // for the other)
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 5, l32 = lane & 31;
   const int d = a.d, row_b = 2 * d, chunks_g = row_b / 16;
   const int G = a.shape.group;
-
-  // ---- this workgroup's blocks: x .. x1 - 1 of the list, in tile `tile` of key head kvh, which
-  // begins at `base` ----
-  int32_t tile, kvh, seq;
-  int32_t x, x1, base;
-  if (a.direct) {
-    // (an XCD takes a contiguous run of units; the last tiles of a piece see the most keys: first)
-    const int units = a.tiles * a.kv_heads, per_xcd = (units + 7) / 8;
-    const int unit = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (unit >= units) return;
-    kvh = sgpr(unit / a.tiles);
-    tile = a.tiles - 1 - (unit - kvh * a.tiles);
-    seq = __builtin_amdgcn_readfirstlane(seq_of_tile(a, tile));
-    const ChunkTile t = chunk_tile(a.shape, load_seq(a, seq),
-                                   tile - chunk_base(a.shape, chunk_clamp(a.starts[seq], a.shape.n_tokens), seq));
-    base = x = 0;
-    x1 = sgpr(chunk_size(t));
-    if (x1 == 0) return;
-  } else {
-    const int per = (a.tiles + 255) / 256;
-    const int32_t c0 = min(tid * per, a.tiles), c1 = min(c0 + per, a.tiles);
-    // the sizes of a run of tiles, in order
-    auto run = [&](auto visit) { chunk_run(a, c0, c1, visit); };
-    int64_t mine = 0;
-    run([&](int32_t, int32_t size) { mine += size; });
-    int64_t incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t up = __shfl_up((long long)incl, off);
-      if (lane >= off) incl += up;
-    }
-    if (lane == 63) deal->wave_sum[wave] = incl;
-    __syncthreads();
-    int64_t before = incl - mine, head_total = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += deal->wave_sum[w];
-      head_total += deal->wave_sum[w];
-    }
-    // (at most 2^31 - 1 by the host's bound)
-    const int32_t per_head = __builtin_amdgcn_readfirstlane((int32_t)head_total);
-    const int64_t total = (int64_t)per_head * a.kv_heads;
-    const int64_t share = chunk_share(total, a.groups);
-    // an XCD (workgroup i runs on XCD i % 8) takes a contiguous run of shares
-    const int32_t w = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    x = sgpr((int32_t)min((int64_t)w * share, total));
-    x1 = sgpr((int32_t)min(x + share, total));
-    if (w != 0 && x >= x1) return;
-    kvh = per_head == 0 ? 0 : sgpr(x / per_head);
-    const int32_t in_head = x - kvh * per_head;
-    if (w == 0 || (in_head >= before && in_head < before + mine)) {
-      int64_t at = before;
-      run([&](int32_t t, int32_t size) {
-        if (w == 0) a.plan[t] = (int32_t)at;
-        if (in_head >= at && in_head < at + size) {
-          deal->tile = t;
-          deal->before = (int32_t)at;
-        }
-        at += size;
-      });
-    }
-    if (w == 0 && tid == 0) a.plan[a.tiles] = per_head;
-    if (x >= x1) return;
-    __syncthreads();
-    tile = __builtin_amdgcn_readfirstlane(deal->tile);
-    seq = __builtin_amdgcn_readfirstlane(seq_of_tile(a, tile));
-    base = kvh * per_head + sgpr(deal->before);
-  }
 
   auto kswz = [](int r) { return kChunks == 8 ? ((r >> 1) & 7) : (r & 15); };
   auto vswz = [](int r) { return (kChunks == 8 ? 2 : 4) * (r & 3); };
@@ -372,30 +320,24 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
   const int kf_off = l32 * kRow, kf_swz = kswz(l32);
   const int tr_i = lane & 15, tr_s = (lane >> 4) & 1;
 
-  if (tid == 0) {
-    deal->x = x;
-    deal->x1 = x1;
-    deal->base = base;
-    deal->first_tile = tile;
-    deal->kvh = kvh;
-    deal->seq = seq;
-    deal->again = 0;
-  }
-  __syncthreads();
-  ChunkAt at{x, x1, base, tile, kvh, seq};
+  ChunkAt at{sgpr(deal->x), sgpr(deal->x1), sgpr(deal->base), sgpr(deal->first_tile), sgpr(deal->kvh), sgpr(deal->seq)};
   ChunkUnitAt u;
   // A share's first unit, where it is the rest of one whose start another workgroup has, comes last: the
   // workgroups of an XCD, each with the end of one tile and the start of the next, then go over the
   // same keys at the same time.
+  bool others = false;
   int32_t first_end = -1;   // where that unit ends; -1: none is left over
   bool begun = false;
   for (;;) {
     if (!next_unit(a, at, u)) {
-      if (first_end < 0) break;
+      if (kNarrow || first_end < 0) break;
       at = {sgpr(deal->x), first_end, sgpr(deal->base), sgpr(deal->first_tile), sgpr(deal->kvh), sgpr(deal->seq)};
       first_end = -1;
       if (!next_unit(a, at, u)) break;
-    } else if (!begun) {
+    } else if (kOwnTiles<kSrc> && kNarrow != (u.tile.rows <= 32)) {
+      others = true;
+      continue;
+    } else if (!kNarrow && !begun) {
       begun = true;
       if (u.b0 > 0 && at.x < at.x1) {
         first_end = at.x;
@@ -407,10 +349,11 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
     const bool whole = b0 == 0 && b1 >= n_blocks;
     const int32_t first_row = (at.tile - u.first) * kChunkRows;
     const int32_t* table = a.tables + (int64_t)at.seq * a.ld_table;
-    const bool active = 32 * wave < rows;
+    const int rw = kNarrow ? 0 : wave;   // the wave's 32 rows; a tile of at most 32 is all waves'
+    const bool active = 32 * rw < rows;
 
     // the lane's query row: token t of the sequence, query head `head` of the key head's
-    const int m_row = min(32 * wave + l32, rows - 1);
+    const int m_row = min(32 * rw + l32, rows - 1);
     const uint32_t packed = (uint32_t)(first_row + m_row);
     const int32_t token = (int32_t)(packed / (uint32_t)G), head = (int32_t)(packed - (uint32_t)token * G);
     const int32_t p = len - u.seq.tokens + token;
@@ -484,21 +427,24 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
         to[i] = w;
       }
     };
+    // load number ch of a row to the row's place in LDS
+    auto put = [&](const u32x4& from, uint8_t* row, int ch, int swz) {
+      if constexpr (kSrc == kCodes) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x2 lo = widen4<kBF16>(from[2 * h]), hi = widen4<kBF16>(from[2 * h + 1]);
+          *reinterpret_cast<u32x4*>(row + (((2 * ch + h) ^ swz) << 4)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+      } else {
+        *reinterpret_cast<u32x4*>(row + ((ch ^ swz) << 4)) = from;
+      }
+    };
     auto commit = [&](const u32x4 (&from)[kLoads], uint8_t* to, bool is_v) {
       constexpr int kPer = kDp / kLoadElems;
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const int row = (tid + 256 * i) / kPer, ch = (tid + 256 * i) % kPer;
-        const int swz = is_v ? vswz(row) : kswz(row);
-        if constexpr (kSrc == kCodes) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x2 lo = widen4<kBF16>(from[i][2 * h]), hi = widen4<kBF16>(from[i][2 * h + 1]);
-            *reinterpret_cast<u32x4*>(to + row * kRow + (((2 * ch + h) ^ swz) << 4)) = u32x4{lo[0], lo[1], hi[0], hi[1]};
-          }
-        } else {
-          *reinterpret_cast<u32x4*>(to + row * kRow + ((ch ^ swz) << 4)) = from[i];
-        }
+        put(from[i], to + row * kRow, ch, is_v ? vswz(row) : kswz(row));
       }
     };
     auto k_stage = [&](int s) { return smem + s * kStageB; };
@@ -580,6 +526,228 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
 #pragma unroll
     for (int cc = 0; cc < kPN; ++cc) pa[cc] = pb[cc] = u32x4{0u, 0u, 0u, 0u};
 
+    auto softmax_block = [&](int j, auto masked, uint64_t there, f32x16 (&s)[kST], u32x4 (&pnew)[kPN]) {
+      constexpr bool kMasked = decltype(masked)::value;
+      if constexpr (kMasked) {
+        const int e = b0 + j;
+        const int kb = (e < b1 ? block_of(e) * kNK : 0x40000000) + 4 * g;
+        const int hi = p - kb;             // key offsets > hi are not seen
+        const int lo = p - win - kb;       // <= lo neither, unless
+        const int sk = sinks - kb;         // below sk
+        const uint64_t mine = there >> (4 * g);
+#pragma unroll
+        for (int st = 0; st < kST; ++st)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int off = 32 * st + 8 * (i >> 2) + (i & 3);
+            const bool in = off <= hi && (off > lo || off < sk) && ((mine >> off) & 1);
+            s[st][i] = in ? s[st][i] : -__builtin_inff();
+          }
+      }
+      // fast path: P_j against the running max; a lane whose block sum is larger than the limit, or
+      // NaN, sends the wave to the block-max update
+      auto probs = [&](float mc) {
+        float rs = 0.0f;
+#pragma unroll
+        for (int st = 0; st < kST; ++st)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            u32x4 w;
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const float x0 = exp2_fast(__builtin_fmaf(s[st][8 * h + 2 * jj], c, -mc));
+              const float x1 = exp2_fast(__builtin_fmaf(s[st][8 * h + 2 * jj + 1], c, -mc));
+              w[jj] = pack2<kBF16>(x0, x1);
+              rs = pair_sum<kBF16>(w[jj], rs);
+            }
+            pnew[2 * st + h] = w;
+          }
+        return rs;
+      };
+      float rs = probs(m_run * c - kLift<kBF16>);
+      if (__builtin_amdgcn_ballot_w64(!(rs <= kBlockSumLimit<kBF16>)) != 0) {
+#pragma unroll
+        for (int st = 0; st < kST; ++st) asm volatile("" : "+v"(s[st]));
+        float m = s[0][0];
+#pragma unroll
+        for (int st = 0; st < kST; ++st)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) m = __builtin_fmaxf(m, s[st][i]);
+        const float mx = pair32_max(m);
+        const bool grow = __builtin_amdgcn_ballot_w64((mx - m_run) * c > kRescaleLog2) != 0;
+        const float m_new = grow ? __builtin_fmaxf(m_run, mx) : m_run;
+        // a row may have masked keys only so far: then every p is 0
+        const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
+        const float alpha = exp2_fast((m_run - m_use) * c);
+        m_run = m_new;
+        rs = probs(m_use * c - kLift<kBF16>);
+        l_run *= alpha;
+        if (grow) {
+#pragma unroll
+          for (int dt = 0; dt < kDT; ++dt) oacc[dt] *= alpha;
+        }
+      }
+      l_run += rs;
+    };
+
+    // ---- at most 32 rows: a wave takes every fourth block, in a K and a V tile of its own, and waits for
+    // no other; the waves' results are joined through LDS.  (One wave with all blocks, the others
+    // loading for it, as with more rows, was held up by its products and softmax: with e4m3
+    // codes 32 pieces of 8 over up to 8192 keys took 108 us, now 90; 3 pieces of up to 700 and 48 single
+    // tokens 164, now 146.  16-bit keys come at 5.1 TB/s either way.) ----
+    if constexpr (kNarrow) {
+      constexpr int kN = kTileB / 1024;                          // DMAs of a tile
+      constexpr int kOwn = kNK * kDp / kLoadElems / 64;          // or loads of a lane
+      constexpr int kPer = kDp / kLoadElems;                     // loads of a row
+      u32x4 own_k[kSrc == kDma ? 1 : kOwn], own_v[kSrc == kDma ? 1 : kOwn];
+      // past the part nothing is read
+      auto own_dma = [&](const uint8_t* from, uint8_t* to, bool is_v, int e, const Keys& k) {
+        const int end = e < b1 ? len - block_of(e) * kNK : 0;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const int row0 = kDmaRows * i, row = row0 + lane / kChunks;
+          const int ch = lane % kChunks ^ (is_v ? vswz(row) : kswz(row));
+          const int off = ch < chunks_g ? lane / kChunks * row_b + ch * 16 : 0x7fff0000;
+          const int hi = __builtin_amdgcn_readlane(k.hi, row0);
+          const uint64_t at = (uint64_t)(uint32_t)hi << 32 | (uint32_t)__builtin_amdgcn_readlane((int)k.lo, row0);
+          const int rows_in = sgpr(min(max(end - row0, 0), kDmaRows));
+          const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)(from + at), (short)0, hi < 0 ? 0 : rows_in * row_b, 0x00020000);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(to + i * 1024), 16, off, 0, 0, 0);
+        }
+      };
+      auto own_fetch = [&](const uint8_t* from, u32x4* to, int e, const Keys& k) {
+        const int end = e < b1 ? len - block_of(e) * kNK : 0;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int row = (lane + 64 * i) / kPer, ch = (lane + 64 * i) % kPer;
+          const int hi = __shfl(k.hi, row);
+          const uint64_t at = (uint64_t)(uint32_t)hi << 32 | (uint32_t)__shfl((int)k.lo, row);
+          u32x4 w = {0u, 0u, 0u, 0u};
+          if (hi >= 0 && row < end && ch * kLoadElems < d) w = *reinterpret_cast<const u32x4*>(from + at + ch * 16);
+          to[i] = w;
+        }
+      };
+      auto own_commit = [&](const u32x4* from, uint8_t* to, bool is_v) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          const int row = (lane + 64 * i) / kPer, ch = (lane + 64 * i) % kPer;
+          put(from[i], to + row * kRow, ch, is_v ? vswz(row) : kswz(row));
+        }
+      };
+      auto load_k = [&](int e, const Keys& k) {
+        if constexpr (kSrc == kDma) own_dma(K, k_stage(wave), false, e, k);
+        else own_fetch(K, own_k, e, k);
+      };
+      auto load_v = [&](int e, const Keys& k) {
+        if constexpr (kSrc == kDma) own_dma(V, v_stage(wave), true, e, k);
+        else own_fetch(V, own_v, e, k);
+      };
+      // the tile whose loads are older than those of the last kN DMAs is there; reads before have ended
+      auto arrived = [&] {
+        static_assert(kN <= 63, "vmcnt");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((kN & 15) | (7 << 4) | (15 << 8) | ((kN >> 4) << 14));
+        asm volatile("" ::: "memory");
+      };
+      auto reads_done = [&] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+        asm volatile("" ::: "memory");
+      };
+      if (b0 + wave < b1) {
+        const int e0 = b0 + wave;
+        const int32_t id0 = ids_of(e0), id1 = ids_of(e0 + 4);
+        int32_t id2 = ids_of(e0 + 8);
+        Keys keys0 = keys_at(e0, id0), keys1 = keys_at(e0 + 4, id1);
+        load_k(e0, keys0);
+        load_v(e0, keys0);
+        for (int e = e0; e < b1; e += 4) {
+          const uint64_t there = pages_there(keys0);
+          keys0 = keys1;
+          if constexpr (kSrc == kDma) arrived();
+          else {
+            own_commit(own_k, k_stage(wave), false);
+            load_k(e + 4, keys0);
+          }
+          f32x16 s[kST];
+          s_block(wave, s);
+          if constexpr (kSrc == kDma) {
+            reads_done();
+            load_k(e + 4, keys0);
+          }
+          softmax_block(e - b0, std::true_type{}, there, s, pa);
+          if constexpr (kSrc == kDma) arrived();
+          else {
+            own_commit(own_v, v_stage(wave), true);
+            load_v(e + 4, keys0);
+          }
+          pv_block(wave, pa, oacc);
+          if constexpr (kSrc == kDma) {
+            reads_done();
+            load_v(e + 4, keys0);
+          }
+          keys1 = keys_at(e + 8, id2);
+          id2 = ids_of(e + 12);
+        }
+      }
+      // the four waves' results: in their own tiles' place, then a wave a quarter of the dims
+      static_assert(kDT * 4096 <= kStageB, "O in the place of K and V");
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));   // vmcnt(0) lgkmcnt(0): nothing more is written there
+      asm volatile("" ::: "memory");
+      int el = lane;   // (through an empty asm: addresses worked out here are not kept in registers through the blocks)
+      asm volatile("" : "+v"(el));
+#pragma unroll
+      for (int t = 0; t < 4 * kDT; ++t) {
+        const int e = 4 * (t % 4);
+        *reinterpret_cast<f32x4*>(smem + wave * kStageB + 1024 * t + 16 * el) =
+            f32x4{oacc[t / 4][e], oacc[t / 4][e + 1], oacc[t / 4][e + 2], oacc[t / 4][e + 3]};
+      }
+      deal->acc[wave][el] = m_run;
+      deal->acc[wave][64 + el] = pair32_sum(l_run);
+      __syncthreads();
+      float m = deal->acc[0][el], l = 0.0f;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) m = __builtin_fmaxf(m, deal->acc[w][el]);
+      const float m_use = m == -__builtin_inff() ? 0.0f : m;   // no key seen
+      f32x4 o[kDT];
+#pragma unroll
+      for (int t = 0; t < kDT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = exp2_fast((deal->acc[w][el] - m_use) * c);
+        l += f * deal->acc[w][64 + el];
+#pragma unroll
+        for (int t = 0; t < kDT; ++t)
+          o[t] += *reinterpret_cast<const f32x4*>(smem + w * kStageB + 1024 * (kDT * wave + t) + 16 * el) * f;
+      }
+      if (!whole) {
+        const int32_t w = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+        float* part = a.parts + (int64_t)(2 * w + (b0 == 0 ? 1 : 0)) * kPartFloats<kDh> + 4 * el;
+#pragma unroll
+        for (int t = 0; t < kDT; ++t) *reinterpret_cast<f32x4*>(part + 256 * (kDT * wave + t)) = o[t];
+        if (wave == 0) *reinterpret_cast<f32x4*>(part + 256 * 4 * kDT) = f32x4{m, l, 0.0f, 0.0f};
+      } else if ((el & 31) < rows) {
+        const bool none = p < 0;   // no key: zeros
+        const float inv = none ? 0.0f : a.v_scale / l;
+        float z = none ? 0.0f : l * inv * 0.0f;
+        uint16_t* orow = O + (int64_t)(u.seq.start + token) * a.ldo + (int64_t)(kvh * G + head) * d;
+#pragma unroll
+        for (int t = 0; t < kDT; ++t) {
+          const int tt = kDT * wave + t, dim = 32 * (tt / 4) + 8 * (tt % 4) + 4 * (el >> 5);
+          if (dim >= d) continue;
+          const f32x4 f = o[t] * inv;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z = __builtin_fmaf(f[i], 0.0f, z);
+          *reinterpret_cast<u32x2*>(orow + dim) = u32x2{pack2<kBF16>(f[0], f[1]), pack2<kBF16>(f[2], f[3])};
+        }
+        if (!(z == 0.0f)) deal->again = 1;
+      }
+      __syncthreads();   // (the next unit's tiles go to the same place)
+      continue;
+    }
+
     int nb = b1 - b0;
     nb += nb & 1;
     if (nb > 0 && n_blocks > 0) {
@@ -615,70 +783,6 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
           __syncthreads();
         }
       } else {
-      auto softmax_block = [&](int j, auto masked, uint64_t there, f32x16 (&s)[kST], u32x4 (&pnew)[kPN]) {
-        constexpr bool kMasked = decltype(masked)::value;
-        if constexpr (kMasked) {
-          const int e = b0 + j;
-          const int kb = (e < b1 ? block_of(e) * kNK : 0x40000000) + 4 * g;
-          const int hi = p - kb;             // key offsets > hi are not seen
-          const int lo = p - win - kb;       // <= lo neither, unless
-          const int sk = sinks - kb;         // below sk
-          const uint64_t mine = there >> (4 * g);
-#pragma unroll
-          for (int st = 0; st < kST; ++st)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int off = 32 * st + 8 * (i >> 2) + (i & 3);
-              const bool in = off <= hi && (off > lo || off < sk) && ((mine >> off) & 1);
-              s[st][i] = in ? s[st][i] : -__builtin_inff();
-            }
-        }
-        // fast path: P_j against the running max; a lane whose block sum is larger than the limit, or
-        // NaN, sends the wave to the block-max update
-        auto probs = [&](float mc) {
-          float rs = 0.0f;
-#pragma unroll
-          for (int st = 0; st < kST; ++st)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              u32x4 w;
-#pragma unroll
-              for (int jj = 0; jj < 4; ++jj) {
-                const float x0 = exp2_fast(__builtin_fmaf(s[st][8 * h + 2 * jj], c, -mc));
-                const float x1 = exp2_fast(__builtin_fmaf(s[st][8 * h + 2 * jj + 1], c, -mc));
-                w[jj] = pack2<kBF16>(x0, x1);
-                rs = pair_sum<kBF16>(w[jj], rs);
-              }
-              pnew[2 * st + h] = w;
-            }
-          return rs;
-        };
-        float rs = probs(m_run * c - kLift<kBF16>);
-        if (__builtin_amdgcn_ballot_w64(!(rs <= kBlockSumLimit<kBF16>)) != 0) {
-#pragma unroll
-          for (int st = 0; st < kST; ++st) asm volatile("" : "+v"(s[st]));
-          float m = s[0][0];
-#pragma unroll
-          for (int st = 0; st < kST; ++st)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = __builtin_fmaxf(m, s[st][i]);
-          const float mx = pair32_max(m);
-          const bool grow = __builtin_amdgcn_ballot_w64((mx - m_run) * c > kRescaleLog2) != 0;
-          const float m_new = grow ? __builtin_fmaxf(m_run, mx) : m_run;
-          // a row may have masked keys only so far: then every p is 0
-          const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;
-          const float alpha = exp2_fast((m_run - m_use) * c);
-          m_run = m_new;
-          rs = probs(m_use * c - kLift<kBF16>);
-          l_run *= alpha;
-          if (grow) {
-#pragma unroll
-            for (int dt = 0; dt < kDT; ++dt) oacc[dt] *= alpha;
-          }
-        }
-        l_run += rs;
-      };
-
       auto iteration = [&](int j, auto stage_c, auto masked, f32x16 (&scur)[kST], f32x16 (&snext)[kST],
                            const u32x4 (&pprev)[kPN], u32x4 (&pnew)[kPN]) {
         constexpr int kS = decltype(stage_c)::value;
@@ -770,32 +874,131 @@ __device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* _
     }
     __syncthreads();   // (the next unit's tiles go to the same place)
   }
+  return others;
+}
+
+template <bool kBF16, Source kSrc, int kNK, int kDh, int kDp>
+__device__ __forceinline__ void chunk_attn(const ChunkArgs& a, const uint16_t* __restrict__ Q, const uint8_t* __restrict__ K,
+                                           const uint8_t* __restrict__ V, uint16_t* __restrict__ O, uint8_t* smem,
+                                           ChunkLds* deal) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // ---- this workgroup's blocks: x .. x1 - 1 of the list, in tile `tile` of key head kvh, which
+  // begins at `base` ----
+  int32_t tile, kvh, seq;
+  int32_t x, x1, base, first_rows;
+  if (a.direct) {
+    // (an XCD takes a contiguous run of units; the last tiles of a piece see the most keys: first)
+    const int units = a.tiles * a.kv_heads, per_xcd = (units + 7) / 8;
+    const int unit = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (unit >= units) return;
+    kvh = sgpr(unit / a.tiles);
+    tile = a.tiles - 1 - (unit - kvh * a.tiles);
+    seq = __builtin_amdgcn_readfirstlane(seq_of_tile(a, tile));
+    const ChunkTile t = chunk_tile(a.shape, load_seq(a, seq),
+                                   tile - chunk_base(a.shape, chunk_clamp(a.starts[seq], a.shape.n_tokens), seq));
+    base = x = 0;
+    x1 = sgpr(chunk_size(t));
+    if (x1 == 0) return;
+    first_rows = sgpr(t.rows);
+  } else {
+    const int per = (a.tiles + 255) / 256;
+    const int32_t c0 = min(tid * per, a.tiles), c1 = min(c0 + per, a.tiles);
+    // the sizes of a run of tiles, in order
+    auto run = [&](auto visit) { chunk_run(a, c0, c1, visit); };
+    int64_t mine = 0;
+    run([&](int32_t, int32_t size, int32_t, int32_t, int32_t) { mine += size; });
+    int64_t incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t up = __shfl_up((long long)incl, off);
+      if (lane >= off) incl += up;
+    }
+    if (lane == 63) deal->wave_sum[wave] = incl;
+    __syncthreads();
+    int64_t before = incl - mine, head_total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += deal->wave_sum[w];
+      head_total += deal->wave_sum[w];
+    }
+    // (at most 2^31 - 1 by the host's bound)
+    const int32_t per_head = __builtin_amdgcn_readfirstlane((int32_t)head_total);
+    const int64_t total = (int64_t)per_head * a.kv_heads;
+    const int64_t share = chunk_share(total, a.groups);
+    // an XCD (workgroup i runs on XCD i % 8) takes a contiguous run of shares
+    const int32_t w = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    x = sgpr((int32_t)min((int64_t)w * share, total));
+    x1 = sgpr((int32_t)min(x + share, total));
+    if (w != 0 && x >= x1) return;
+    kvh = per_head == 0 ? 0 : sgpr(x / per_head);
+    const int32_t in_head = x - kvh * per_head;
+    if (w == 0 || (in_head >= before && in_head < before + mine)) {
+      int64_t at = before;
+      run([&](int32_t t, int32_t size, int32_t r, int32_t first, int32_t rows) {
+        if (w == 0) a.plan[t] = {(int32_t)at, r, first, rows};
+        if (in_head >= at && in_head < at + size) {
+          deal->tile = t;
+          deal->before = (int32_t)at;
+          deal->seq = r;
+          deal->rows = rows;
+        }
+        at += size;
+      });
+    }
+    if (w == 0 && tid == 0) a.plan[a.tiles].at = per_head;
+    if (x >= x1) return;
+    __syncthreads();
+    tile = __builtin_amdgcn_readfirstlane(deal->tile);
+    seq = __builtin_amdgcn_readfirstlane(deal->seq);
+    first_rows = sgpr(deal->rows);
+    base = kvh * per_head + sgpr(deal->before);
+  }
+
+  if (tid == 0) {
+    deal->x = x;
+    deal->x1 = x1;
+    deal->base = base;
+    deal->first_tile = tile;
+    deal->kvh = kvh;
+    deal->seq = seq;
+    deal->again = 0;
+  }
+  __syncthreads();
+  if constexpr (kOwnTiles<kSrc>) {
+    // those like the share's first unit first: most shares have no others to look for
+    bool narrow = first_rows <= 32, more = true;
+    for (int i = 0; i < 2 && more; ++i, narrow = !narrow)
+      more = narrow ? chunk_units<kBF16, kSrc, kNK, kDh, kDp, true>(a, Q, K, V, O, smem, deal)
+                    : chunk_units<kBF16, kSrc, kNK, kDh, kDp, false>(a, Q, K, V, O, smem, deal);
+  } else {
+    chunk_units<kBF16, kSrc, kNK, kDh, kDp, false>(a, Q, K, V, O, smem, deal);
+  }
   __syncthreads();   // (a share may have no unit and so no barrier since the flag was cleared)
   if (__builtin_amdgcn_readfirstlane(deal->again) != 0) chunk_again<kBF16, kSrc == kCodes>(a, deal);
 }
 
-// Joins the parts of unit blockIdx.x (key head, tile), 32 rows a workgroup (blockIdx.y); a wave takes
-// every fourth 4-dim column, eight parts' loads in flight.
-template <bool kBF16, bool kFp8, int kDh>
+// Joins the parts of unit blockIdx.x (key head, tile), 32 rows a workgroup (blockIdx.y); each wave has
+// kQ 4-dim columns of every lane, all of a row's in one workgroup, or (kQ 1) over blockIdx.z.
+template <bool kBF16, bool kFp8, int kDh, int kQ>
 __device__ __forceinline__ void chunk_join(const ChunkArgs& a, ChunkLds* deal) {
   constexpr int kDT = kDh / 32;
   const int kvh = blockIdx.x / a.tiles, tile = blockIdx.x - kvh * a.tiles;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 5, l32 = lane & 31, rw = blockIdx.y, d = a.d, G = a.shape.group;
-  const int32_t at = a.plan[tile], size = a.plan[tile + 1] - at;
-  if (size <= kChunkUnit) return;   // empty, or without keys
-  const int64_t total = (int64_t)a.plan[a.tiles] * a.kv_heads;
-  const int64_t share = chunk_share(total, a.groups);
-  const int64_t x0 = (int64_t)kvh * a.plan[a.tiles] + at + kChunkUnit;
+  const int col0 = kQ * (4 * blockIdx.z + wave);   // the wave's first column, of 8 dims
+  const ChunkRec rec = a.plan[tile];
+  const int32_t at = rec.at, size = a.plan[tile + 1].at - at, per_head = a.plan[a.tiles].at;
+  if (size <= kChunkUnit || 32 * rw >= rec.rows) return;   // without keys, or rows
+  const int64_t share = chunk_share((int64_t)per_head * a.kv_heads, a.groups);
+  const int64_t x0 = (int64_t)kvh * per_head + at + kChunkUnit;
   const int32_t g0 = (int32_t)(x0 / share), g1 = (int32_t)((x0 + size - kChunkUnit - 1) / share);
   if (g0 == g1) return;   // one workgroup had it whole
-  const int32_t seq = seq_of_tile(a, tile);
+  const int32_t seq = rec.seq, rows = rec.rows;
   const ChunkSeq q_seq = load_seq(a, seq);
-  const int32_t seq_base = chunk_base(a.shape, q_seq.start, seq);
-  const ChunkTile tl = chunk_tile(a.shape, q_seq, tile - seq_base);
-  if (32 * rw >= tl.rows) return;
-  const int m_row = min(32 * rw + l32, tl.rows - 1);
-  const int64_t packed = (int64_t)(tile - seq_base) * kChunkRows + m_row;
+  const int64_t packed0 = (int64_t)(tile - rec.first) * kChunkRows + 32 * rw;   // the first row's
+  const int64_t packed = packed0 + min(l32, rows - 1 - 32 * rw);
   const int32_t token = (int32_t)(packed / G), head = (int32_t)(packed - (int64_t)token * G);
   const int32_t p = q_seq.len - q_seq.tokens + token;
   auto part = [&](int32_t w) {
@@ -803,65 +1006,66 @@ __device__ __forceinline__ void chunk_join(const ChunkArgs& a, ChunkLds* deal) {
   };
   if (threadIdx.x == 0) deal->again = 0;
   __syncthreads();
-  f32x4 acc[kDT];
+  f32x4 acc[kQ];
 #pragma unroll
-  for (int t = 0; t < kDT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < kQ; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = -__builtin_inff(), l = 0.0f;
-  for (int32_t w0 = g0; w0 <= g1; w0 += 4) {
-    f32x4 ml[4], o[4][kDT];
+  constexpr int kTake = kQ == 1 ? 16 : 4;   // parts whose loads are in flight
+  for (int32_t w0 = g0; w0 <= g1; w0 += kTake) {
+    f32x4 ml[kTake], o[kTake][kQ];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kTake; ++u) {
       const float* from = part(min(w0 + u, g1));
       ml[u] = *reinterpret_cast<const f32x4*>(from + 256 * 4 * kDT);
 #pragma unroll
-      for (int t = 0; t < kDT; ++t) o[u][t] = *reinterpret_cast<const f32x4*>(from + 256 * (kDT * wave + t));
+      for (int t = 0; t < kQ; ++t) o[u][t] = *reinterpret_cast<const f32x4*>(from + 256 * (col0 + t));
       if (w0 + u > g1) ml[u] = f32x4{-__builtin_inff(), 0.0f, 0.0f, 0.0f};
     }
     float m_new = m;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) m_new = __builtin_fmaxf(m_new, ml[u][0]);
+    for (int u = 0; u < kTake; ++u) m_new = __builtin_fmaxf(m_new, ml[u][0]);
     const float m_use = m_new == -__builtin_inff() ? 0.0f : m_new;   // no key seen so far
     const float alpha = exp2_fast((m - m_use) * a.scale_log2);
     m = m_new;
     l *= alpha;
 #pragma unroll
-    for (int t = 0; t < kDT; ++t) acc[t] *= alpha;
+    for (int t = 0; t < kQ; ++t) acc[t] *= alpha;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kTake; ++u) {
       if (w0 + u > g1) continue;
       const float f = exp2_fast((ml[u][0] - m_use) * a.scale_log2);   // (a part without seen keys: 0)
       l += f * ml[u][1];
 #pragma unroll
-      for (int t = 0; t < kDT; ++t) acc[t] += o[u][t] * f;
+      for (int t = 0; t < kQ; ++t) acc[t] += o[u][t] * f;
     }
   }
   const bool none = p < 0;
   const float inv = none ? 0.0f : a.v_scale / l;
   float z = none ? 0.0f : l * 0.0f;
 #pragma unroll
-  for (int t = 0; t < kDT; ++t)
+  for (int t = 0; t < kQ; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) z = __builtin_fmaf(acc[t][i] * inv, 0.0f, z);
-  const uint64_t bad = __builtin_amdgcn_ballot_w64((!(z == 0.0f) || (!none && l == 0.0f)) && 32 * rw + l32 < tl.rows);
+  const uint64_t bad = __builtin_amdgcn_ballot_w64((!(z == 0.0f) || (!none && l == 0.0f)) && 32 * rw + l32 < rows);
   if (lane == 0 && bad != 0) atomicOr(&deal->again, (int)((uint32_t)bad | (uint32_t)(bad >> 32)));
   __syncthreads();
   const uint32_t again = (uint32_t)__builtin_amdgcn_readfirstlane(deal->again);
-  if (32 * rw + l32 < tl.rows && !((again >> l32) & 1)) {
+  if (32 * rw + l32 < rows && !((again >> l32) & 1)) {
     uint16_t* orow = a.o + (int64_t)(q_seq.start + token) * a.ldo + (int64_t)(kvh * G + head) * d;
 #pragma unroll
-    for (int t = 0; t < kDT; ++t) {
-      const int tt = kDT * wave + t, dim = 32 * (tt / 4) + 8 * (tt % 4) + 4 * g;
+    for (int t = 0; t < kQ; ++t) {
+      const int dim = 8 * (col0 + t) + 4 * g;
       if (dim >= d) continue;
       const u32x2 w = {pack2<kBF16>(acc[t][0] * inv, acc[t][1] * inv), pack2<kBF16>(acc[t][2] * inv, acc[t][3] * inv)};
       *reinterpret_cast<u32x2*>(orow + dim) = w;
     }
   }
   for (uint32_t left = again; left != 0; left &= left - 1) {
-    const int64_t r = (int64_t)(tile - seq_base) * kChunkRows + 32 * rw + __builtin_ctz(left);
+    const int64_t r = packed0 + __builtin_ctz(left);
     const int32_t tk = (int32_t)(r / G), hd = kvh * G + (int32_t)(r - (int64_t)tk * G);
     const int64_t t = q_seq.start + tk;
     chunk_row<kBF16, kFp8>(a, seq, kvh, q_seq.len - q_seq.tokens + tk, a.q + t * a.ldq + (int64_t)hd * d,
-                           a.o + t * a.ldo + (int64_t)hd * d, deal);
+                           a.o + t * a.ldo + (int64_t)hd * d, 32 * kQ * blockIdx.z, 32 * kQ * (blockIdx.z + 1), deal);
   }
 }
 
@@ -873,20 +1077,22 @@ __device__ __forceinline__ void chunk_join(const ChunkArgs& a, ChunkLds* deal) {
 // d<D>: head dimensions up to D; s: pages below a DMA instruction's keys
 #define SILE_CHUNK_KERNEL(NAME, BF, SRC, EU, NK, DH, DP)                                  \
   extern "C" __global__ __launch_bounds__(256, EU) void NAME(ChunkArgs a) {               \
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * 2 * NK * 2 * DP + sizeof(ChunkLds)]; \
-    chunk_attn<BF, SRC, NK, DH, DP>(a, a.q, a.k, a.v, a.o, smem, reinterpret_cast<ChunkLds*>(smem + 2 * 2 * NK * 2 * DP)); \
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[4 * 2 * NK * 2 * DP + sizeof(ChunkLds)]; \
+    chunk_attn<BF, SRC, NK, DH, DP>(a, a.q, a.k, a.v, a.o, smem, reinterpret_cast<ChunkLds*>(smem + 4 * 2 * NK * 2 * DP)); \
   }
-#define SILE_CHUNK_JOIN(NAME, BF, F8, DH)                                     \
+#define SILE_CHUNK_JOIN(NAME, BF, F8, DH, Q)                                     \
   extern "C" __global__ __launch_bounds__(256) void NAME(ChunkArgs a) {       \
     __shared__ ChunkLds deal;                                                 \
-    chunk_join<BF, F8, DH>(a, &deal);                                         \
+    chunk_join<BF, F8, DH, Q>(a, &deal);                                         \
   }
 #define SILE_CHUNK_TYPES(T, BF, EU, NK, DH, DP)                                  \
   SILE_CHUNK_KERNEL(sile_paged_chunk_##T##_d##DH, BF, kDma, EU, NK, DH, DP)      \
   SILE_CHUNK_KERNEL(sile_paged_chunk_##T##_s##DH, BF, kStaged, EU, NK, DH, DP)   \
   SILE_CHUNK_KERNEL(sile_paged_chunk_##T##_fp8_d##DH, BF, kCodes, EU, NK, DH, DP) \
-  SILE_CHUNK_JOIN(sile_paged_chunk_join_##T##_d##DH, BF, false, DH)              \
-  SILE_CHUNK_JOIN(sile_paged_chunk_join_##T##_fp8_d##DH, BF, true, DH)
+  SILE_CHUNK_JOIN(sile_paged_chunk_join_##T##_d##DH, BF, false, DH, DH / 32)     \
+  SILE_CHUNK_JOIN(sile_paged_chunk_join_##T##_fp8_d##DH, BF, true, DH, DH / 32)  \
+  SILE_CHUNK_JOIN(sile_paged_chunk_join1_##T##_d##DH, BF, false, DH, 1)          \
+  SILE_CHUNK_JOIN(sile_paged_chunk_join1_##T##_fp8_d##DH, BF, true, DH, 1)
 #define SILE_CHUNK_DIM(EU, NK, DH, DP)          \
   SILE_CHUNK_TYPES(f16, false, EU, NK, DH, DP)  \
   SILE_CHUNK_TYPES(bf16, true, EU, NK, DH, DP)

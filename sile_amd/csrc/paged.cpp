@@ -55,7 +55,7 @@ struct ChunkArgs {
   const void *q, *k, *v;
   void* o;
   const int32_t *starts, *tables, *lengths;
-  int32_t* plan;
+  sile::ChunkRec* plan;
   float* parts;
   int64_t ldq, ldo, page_stride, ld_table;
   sile::ChunkShape shape;
@@ -154,7 +154,7 @@ int chunk_plan(int64_t n_rows, int64_t n_tokens, int64_t q_heads, int64_t kv_hea
   const int rc = device_cus(&cus);
   if (rc != SILE_OK) return rc;
   p->groups = std::max<int64_t>(8, (int64_t)(p->dp == 256 ? 1 : 2) * cus / 8 * 8);
-  p->plan_ints = ints16(p->tiles + 1);
+  p->plan_ints = ints16(4 * (p->tiles + 1));   // a ChunkRec each
   // O and (m, l) of a tile's 128 rows, two parts a workgroup
   p->bytes = 4 * (p->plan_ints + 2 * p->groups * 4 * (p->dp / 8 + 1) * 256);
   return SILE_OK;
@@ -566,8 +566,8 @@ int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n
   a.starts = starts;
   a.tables = tables;
   a.lengths = lengths;
-  a.plan = static_cast<int32_t*>(workspace);
-  a.parts = reinterpret_cast<float*>(a.plan + plan.plan_ints);
+  a.plan = static_cast<sile::ChunkRec*>(workspace);
+  a.parts = static_cast<float*>(workspace) + plan.plan_ints;
   a.ldq = ldq;
   a.ldo = ldo;
   a.page_stride = page_stride;
@@ -601,8 +601,11 @@ int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n
   }
   rc = launch(Module::kPagedChunk, name, dim3((unsigned)grid), dim3(256), params, s);
   if (rc != SILE_OK || a.direct) return rc == SILE_OK ? ok() : rc;
-  snprintf(name, sizeof name, "sile_paged_chunk_join_%s%s_d%d", dt, fp8 ? "_fp8" : "", plan.dp);
-  rc = launch(Module::kPagedChunk, name, dim3((unsigned)units, sile::kChunkRows / 32), dim3(256), params, s);
+  // with few units, of many parts, the dims of a row go to several workgroups (8 tokens over 131072 keys, 8 units
+  // of 64 parts: 132 -> 121 us; 568 units of one to three: 145 -> 161)
+  const int split = units <= 64 ? plan.dp / 32 : 1;
+  snprintf(name, sizeof name, "sile_paged_chunk_join%s_%s%s_d%d", split > 1 ? "1" : "", dt, fp8 ? "_fp8" : "", plan.dp);
+  rc = launch(Module::kPagedChunk, name, dim3((unsigned)units, sile::kChunkRows / 32, split), dim3(256), params, s);
   return rc == SILE_OK ? ok() : rc;
 }
 

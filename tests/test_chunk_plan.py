@@ -27,7 +27,7 @@ int32_t walk(const int32_t* starts, const int32_t* lengths, const int64_t* s, in
              int32_t* seen, int32_t* parts, int32_t* zeros, int32_t* at_of) {
   const Args a = args(starts, lengths, s);
   int64_t per_head = 0;
-  chunk_run(a, 0, a.tiles, [&](int32_t t, int32_t size) { at_of[t] = (int32_t)per_head; per_head += size; });
+  chunk_run(a, 0, a.tiles, [&](int32_t t, int32_t size, auto...) { at_of[t] = (int32_t)per_head; per_head += size; });
   at_of[a.tiles] = (int32_t)per_head;
   const int64_t total = per_head * a.kv_heads, share = chunk_share(total, groups);
   for (int32_t w = 0; w < groups; ++w) {

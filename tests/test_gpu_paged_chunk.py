@@ -215,6 +215,32 @@ def test_chunk_nan_ahead(hip, dtype, fp8, d):
     case.check(case.do.download(np.uint16, (case.n + 1, case.ldo))[:case.n, :case.hq * d].reshape(case.n, case.hq, d), "nan ahead")
 
 
+@pytest.mark.parametrize("dtype,fp8", [("f16", False), ("bf16", False), ("bf16", True)])
+@pytest.mark.parametrize("d,window", [(64, 0), (80, 0), (128, 0), (128, 700), (208, 0), (256, 500)])
+def test_chunk_drafts(hip, dtype, fp8, d, window):
+    """A few tokens behind many: the keys of all workgroups' waves joined, with pages that are missing and a NaN that
+    only the last token sees (the rows before it are taken again, in parts of their dims)."""
+    case = Case(11, dtype, [(6, 3001), (1, 900), (8, 8000), (4, 4)], 4, 1, d, 16, fp8=fp8, window=window, sinks=5 if window else 0)
+    gone = {0: {180, 186}, 2: {0, 470, 495}}
+    for i, entries in gone.items():
+        for e in entries:
+            case.tables[i, e] = (-1, case.num)[e % 2]
+    for i in (0, 2, 3):
+        n = case.seqs[i][1] - 1
+        for pool in case.pools:
+            view = pool[:, :case.hkv * case.page * d].reshape(case.num, case.hkv, case.page, d)
+            view[case.tables[i, n // case.page], :, n % case.page] = 0x7F if fp8 else NAN16[dtype]
+    say(f"chunk drafts {dtype} fp8={fp8} d {d} window {window}")
+    case.upload(hip)
+    case.run(hip)
+    got = as_f32(case.result(hip), dtype)
+    for i in (0, 2, 3):
+        assert np.isnan(got[case.starts[i + 1] - 1]).all(), "the token of the NaN key"
+    case.seqs = [(new - (i != 1), n - (i != 1)) for i, (new, n) in enumerate(case.seqs)]
+    case.check(case.do.download(np.uint16, (case.n + 1, case.ldo))[:case.n, :case.hq * d].reshape(case.n, case.hq, d),
+               "drafts", gone=gone)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
 def test_chunk_scales(hip, scale):
     """No scale (every key alike), a negative one, sharp ones."""
