@@ -97,18 +97,18 @@ struct SlotsArgs {
 };
 constexpr int kSlotTokens = 1024;   // of the list, a workgroup
 
-// One launch for a list of any length: every workgroup of 256 adds up the rows' tokens (a
-// run of rows a thread, a scan over the threads; rows up to 65536 are in the L2), marks
-// where the rows of its own 1024 tokens begin, and a running maximum over the marks names
-// each token's row.  Every 256th run of rows (or all, where there is one workgroup) also
-// goes to starts and lengths_out.  Bound by the launch and three dependent reads: 256 rows
-// and 1800 tokens 4 us, 4000 rows and 134000 tokens 8.
+// One launch for a list of any length: every workgroup adds up the rows' tokens (a run of rows a
+// thread, a scan over the threads; rows up to 65536 are in the L2), marks where the rows of its own
+// 1024 tokens begin, and a running maximum over the marks names each token's row.  Every 1024th
+// run of rows (or all, where there is one workgroup) also goes to starts and lengths_out.  Bound by the
+// launch and three dependent reads: 256 rows and 1800 tokens 5 us, 4000 rows and 134000 tokens
+// 8.7 (14.5 with a quarter of the threads, and four times the rows in each).
 SILE_DEV void slots(const SlotsArgs& a) {
-  __shared__ int64_t wave_sum[4];
+  __shared__ int64_t wave_sum[kSlotTokens / 64];
   __shared__ int32_t mark_row[kSlotTokens], mark_base[kSlotTokens];   // by token: row + 1 that begins there, length - start
-  __shared__ int32_t wave_top[4], first_row, first_base;
+  __shared__ int32_t wave_top[kSlotTokens / 64], first_row, first_base;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (a.n_rows + 255) / 256;
+  const int per = (a.n_rows + kSlotTokens - 1) / kSlotTokens;
   const int r0 = min(tid * per, a.n_rows), r1 = min(r0 + per, a.n_rows);
   const int32_t t0 = blockIdx.x * kSlotTokens;
   // a row's length, and how many tokens it asks for: no position passes 2^31 - 1
@@ -117,7 +117,7 @@ SILE_DEV void slots(const SlotsArgs& a) {
     *length = len;
     return min(n, 0x7fffffff - len);
   };
-  for (int i = tid; i < kSlotTokens; i += 256) mark_row[i] = 0;
+  mark_row[tid] = 0;
   int64_t mine = 0;
   int32_t length;
   for (int r = r0; r < r1; ++r) mine += row(r, &length);
@@ -131,7 +131,7 @@ SILE_DEV void slots(const SlotsArgs& a) {
   __syncthreads();
   int64_t at = incl - mine, total = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < kSlotTokens / 64; ++w) {
     if (w < wave) at += wave_sum[w];
     total += wave_sum[w];
   }
@@ -156,34 +156,22 @@ SILE_DEV void slots(const SlotsArgs& a) {
     }
   if (blockIdx.x == 0 && tid == 0) a.starts[a.n_rows] = (int32_t)min(total, (int64_t)a.tokens);
   __syncthreads();
-  // the last mark at or before each of the thread's four tokens
-  int top[4], run = -1;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (mark_row[4 * tid + i] != 0) run = 4 * tid + i;
-    top[i] = run;
-  }
+  // the last mark at or before the thread's token
+  int mark = mark_row[tid] != 0 ? tid : -1;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int up = __shfl_up(run, off);
-    if (lane >= off) run = max(run, up);
+    const int up = __shfl_up(mark, off);
+    if (lane >= off) mark = max(mark, up);
   }
-  if (lane == 63) wave_top[wave] = run;
-  int before = __shfl_up(run, 1);
-  if (lane == 0) before = -1;
+  if (lane == 63) wave_top[wave] = mark;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 3; ++w)
-    if (w < wave) before = max(before, wave_top[w]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int32_t left = a.tokens - t0, k = 4 * tid + i;
-    if (k >= left) break;
-    const int m = max(top[i], before);
-    const bool there = (int64_t)t0 + k < total;
-    a.rows[t0 + k] = !there ? -1 : m < 0 ? first_row : mark_row[m] - 1;
-    a.positions[t0 + k] = !there ? -1 : t0 + k + (m < 0 ? first_base : mark_base[m]);
-  }
+  for (int w = 0; w < kSlotTokens / 64 - 1; ++w)
+    if (w < wave) mark = max(mark, wave_top[w]);
+  if (tid >= a.tokens - t0) return;
+  const bool there = (int64_t)t0 + tid < total;
+  a.rows[t0 + tid] = !there ? -1 : mark < 0 ? first_row : mark_row[mark] - 1;
+  a.positions[t0 + tid] = !there ? -1 : t0 + tid + (mark < 0 ? first_base : mark_base[mark]);
 }
 
 // ---- page contents ----
@@ -281,7 +269,7 @@ SILE_DEV bool wanted(const ReserveArgs& a, int row, int64_t* first, int64_t* las
 
 }  // namespace
 
-extern "C" __global__ __launch_bounds__(256) void sile_kv_slots(SlotsArgs a) { slots(a); }
+extern "C" __global__ __launch_bounds__(1024) void sile_kv_slots(SlotsArgs a) { slots(a); }
 extern "C" __global__ __launch_bounds__(256) void sile_kv_append(AppendArgs a) { append<0>(a); }
 extern "C" __global__ __launch_bounds__(256) void sile_kv_append_f16_fp8(AppendArgs a) { append<1>(a); }
 extern "C" __global__ __launch_bounds__(256) void sile_kv_append_bf16_fp8(AppendArgs a) { append<2>(a); }

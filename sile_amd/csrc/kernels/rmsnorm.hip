@@ -282,9 +282,7 @@ SILE_DEV void norm_any(const NormArgs& a) {
   SILE_NORM(NAME, TYPE, F8, 256, 1, 256)                                                       \
   SILE_NORM(NAME, TYPE, F8, 256, 2, 256)                                                       \
   SILE_NORM(NAME, TYPE, F8, 256, 4, 256)                                                       \
-  SILE_NORM(NAME, TYPE, F8, 1024, 1, 1024)                                                     \
   SILE_NORM(NAME, TYPE, F8, 1024, 2, 1024)                                                     \
-  SILE_NORM(NAME, TYPE, F8, 1024, 4, 1024)                                                     \
   extern "C" __global__ __launch_bounds__(256) void sile_rmsnorm_##NAME##_any(NormArgs a) {    \
     norm_any<TYPE, F8>(a);                                                                     \
   }

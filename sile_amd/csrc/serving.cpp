@@ -158,7 +158,7 @@ int sile_hip_kv_slots(int64_t n_rows, const int32_t* lengths, const int32_t* nee
   SlotsArgs a{lengths, need, granted, starts, rows, positions, lengths_out, (int32_t)n_rows, (int32_t)max_tokens};
   void* params[] = {&a};
   const int64_t groups = std::max<int64_t>(1, (max_tokens + kSlotTokens - 1) / kSlotTokens);
-  rc = launch(Module::kKvCache, "sile_kv_slots", dim3((unsigned)groups), dim3(256), params,
+  rc = launch(Module::kKvCache, "sile_kv_slots", dim3((unsigned)groups), dim3(1024), params,
               static_cast<hipStream_t>(stream));
   return rc == SILE_OK ? ok() : rc;
 }
