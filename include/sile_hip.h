@@ -473,8 +473,8 @@ int sile_hip_flash_attn_fwd(sile_dtype dtype, int64_t batch, int64_t heads, int6
  * taken again row by row: right, but slow.  q_start + q_len and kv_len <= 2^29, one head's
  * K at most 2^31 - 1 bytes, batch * q_heads * q_len < 2^31 (on the matrix cores some 2^24 blocks
  * of 32 to 128 query rows of one key head; more key heads take more launches).  Its form for
- * single tokens: sile_hip_paged_attn_decode.  It reads contiguous keys only: a prompt taken in
- * pieces keeps its keys contiguous beside the pages.
+ * single tokens: sile_hip_paged_attn_decode.  It reads contiguous keys only: for a prompt
+ * taken in pieces, whose earlier keys lie in pages, sile_hip_paged_attn_chunk.
  * No reference counterpart, as sile_hip_flash_attn_fwd. */
 int sile_hip_flash_attn_window_fwd(sile_dtype dtype, int64_t batch, int64_t q_heads,
                                    int64_t kv_heads, int64_t q_len, int64_t kv_len,

