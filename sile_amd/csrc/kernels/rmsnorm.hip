@@ -14,7 +14,7 @@
 //
 // Measured, bf16 with residual and stored sum: 8000 rows of 8192 100 us (5.2 TB/s), into e4m3 codes in groups
 // 106 (4.3 TB/s: the codes' conversion is 35 % of the vector units' cycles), 64 rows of 8192 5; rows of
-// 8191, which are no whole vectors, 277.
+// 8191, which are no whole vectors, 136.
 #include "common.h"
 #include "e4m3.h"
 
@@ -48,14 +48,30 @@ SILE_DEV void store1(void* p, int64_t i, float v) {
     static_cast<uint16_t*>(p)[i] = kType == 1 ? f16_rne(v) : bf16_rne(v);
 }
 
-// 8 elements as they lie in memory
+// rows may begin anywhere: whole vectors all the same, which the memory takes at any element
+typedef uint32_t raw_16 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t raw_8 __attribute__((ext_vector_type(2), aligned(1)));
+
+// 8 elements as they lie in memory, of which the first n are there (the others: zeros)
 template <int kType>
 struct Vec {
   u32x4 w[kType == 0 ? 2 : 1];
-  SILE_DEV void load(const void* p, int64_t i) {
-    const u32x4* q = reinterpret_cast<const u32x4*>(static_cast<const uint8_t*>(p) + i * (kType == 0 ? 4 : 2));
-    w[0] = q[0];
-    if constexpr (kType == 0) w[1] = q[1];
+  SILE_DEV void load(const void* p, int64_t i, int n) {
+    if (n >= 8) {
+      const raw_16* q = reinterpret_cast<const raw_16*>(static_cast<const uint8_t*>(p) + i * (kType == 0 ? 4 : 2));
+      w[0] = q[0];
+      if constexpr (kType == 0) w[1] = q[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (kType == 0) {
+          w[j >> 2][j & 3] = j < n ? static_cast<const uint32_t*>(p)[i + j] : 0u;
+        } else {
+          const uint32_t h = j < n ? static_cast<const uint16_t*>(p)[i + j] : 0u;
+          w[0][j >> 1] = (j & 1) ? w[0][j >> 1] | h << 16 : h;
+        }
+      }
+    }
   }
   SILE_DEV void unpack(float* f) const {
 #pragma unroll
@@ -74,17 +90,21 @@ struct Vec {
   }
 };
 template <int kType>
-SILE_DEV void store8(void* p, int64_t i, const float* f) {
-  if constexpr (kType == 0) {
-    f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + i);
-    q[0] = f32x4{f[0], f[1], f[2], f[3]};
-    q[1] = f32x4{f[4], f[5], f[6], f[7]};
+SILE_DEV void store8(void* p, int64_t i, int n, const float* f) {
+  if (n < 8) {
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+      if (j < n) store1<kType>(p, i + j, f[j]);
+  } else if constexpr (kType == 0) {
+    raw_16* q = reinterpret_cast<raw_16*>(static_cast<float*>(p) + i);
+    q[0] = raw_16{f32_bits(f[0]), f32_bits(f[1]), f32_bits(f[2]), f32_bits(f[3])};
+    q[1] = raw_16{f32_bits(f[4]), f32_bits(f[5]), f32_bits(f[6]), f32_bits(f[7])};
   } else {
-    u32x4 w;
+    raw_16 w;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       w[j] = kType == 1 ? pack_f16x2(f[2 * j], f[2 * j + 1]) : pack_bf16x2(f[2 * j], f[2 * j + 1]);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) = w;
+    *reinterpret_cast<raw_16*>(static_cast<uint16_t*>(p) + i) = w;
   }
 }
 
@@ -116,9 +136,10 @@ SILE_DEV float lanes_max(float v, int lanes) {
 SILE_DEV float scale_of(float top) { return __builtin_fmaxf(top, kLeast) / kTop; }
 SILE_DEV float rcp_of(float scale) { return scale >= 0x1p-60f && scale <= 0x1p60f ? 1.0f / scale : 0.0f; }
 
-// Columns in vectors of 8, all of them aligned: a row takes kThreads threads of kV vectors.
-// kF8: codes out.  kWg: threads of the workgroup.
-template <int kType, bool kF8, int kThreads, int kV, int kWg>
+// Columns in vectors of 8, the last one (kPart) perhaps in part: a row takes kThreads threads of kV vectors.
+// kF8: codes out.  kWg: threads of the workgroup.  (With the parts' code in the way, 8000 x 8192 into codes took 125
+// us, 106 without; 8000 x 8191 through the form for any width 277, 136 here.)
+template <int kType, bool kF8, int kThreads, int kV, int kWg, bool kPart>
 SILE_DEV void norm_rows(const NormArgs& a) {
   __shared__ float lds[2][2][16];
   const int tid = threadIdx.x % kThreads, cols = a.cols;
@@ -126,7 +147,10 @@ SILE_DEV void norm_rows(const NormArgs& a) {
   Vec<kType> wv[kV];
 #pragma unroll
   for (int v = 0; v < kV; ++v)
-    if (a.weight && 8 * (v * kThreads + tid) < cols) wv[v].load(a.weight, 8 * (v * kThreads + tid));
+    if (a.weight && 8 * (v * kThreads + tid) < cols) {
+      const int c = 8 * (v * kThreads + tid);
+      wv[v].load(a.weight, c, kPart ? cols - c : 8);
+    }
   int turn = 0;
   constexpr int kRows = kWg / kThreads;
   const int groups = a.group > 0 ? cols / a.group : 0;
@@ -137,8 +161,8 @@ SILE_DEV void norm_rows(const NormArgs& a) {
     for (int v = 0; v < kV; ++v) {
       const int c = 8 * (v * kThreads + tid);
       if (c < cols) {
-        xv[v].load(a.x, r * a.ldx + c);
-        if (a.residual) rv[v].load(a.residual, r * a.ldr + c);
+        xv[v].load(a.x, r * a.ldx + c, kPart ? cols - c : 8);
+        if (a.residual) rv[v].load(a.residual, r * a.ldr + c, kPart ? cols - c : 8);
       }
     }
     float s[kV][8], ss = 0.0f;
@@ -153,7 +177,7 @@ SILE_DEV void norm_rows(const NormArgs& a) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) s[v][j] += f[j];
         }
-        if (a.sum) store8<kType>(a.sum, r * a.lds + c, s[v]);
+        if (a.sum) store8<kType>(a.sum, r * a.lds + c, kPart ? cols - c : 8, s[v]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[v][j] = 0.0f;
@@ -179,7 +203,7 @@ SILE_DEV void norm_rows(const NormArgs& a) {
 #pragma unroll
       for (int v = 0; v < kV; ++v) {
         const int c = 8 * (v * kThreads + tid);
-        if (c < cols) store8<kType>(a.y, r * a.ldy + c, s[v]);
+        if (c < cols) store8<kType>(a.y, r * a.ldy + c, kPart ? cols - c : 8, s[v]);
       }
     } else {
       float scale = a.scale, rcp = a.rcp;
@@ -212,15 +236,22 @@ SILE_DEV void norm_rows(const NormArgs& a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) f[j] = e4m3_in(s[v][j], scale, rcp);
           }
-          const u32x2 out = {e4m3_pack4(f), e4m3_pack4(f + 4)};
-          __builtin_nontemporal_store(out, reinterpret_cast<u32x2*>(static_cast<uint8_t*>(a.y) + r * a.ldy + c));
+          const raw_8 out = {e4m3_pack4(f), e4m3_pack4(f + 4)};
+          uint8_t* y = static_cast<uint8_t*>(a.y) + r * a.ldy + c;
+          if (!kPart || cols - c >= 8) {
+            __builtin_nontemporal_store(out, reinterpret_cast<raw_8*>(y));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 7; ++j)
+              if (j < cols - c) y[j] = (uint8_t)(out[j >> 2] >> (8 * (j & 3)));
+          }
         }
       }
     }
   }
 }
 
-// Any width, alignment and group: a workgroup of 256 a row, which reads it once for the sum and
+// Any width and group: a workgroup of 256 a row, which reads it once for the sum and
 // once more for each pass behind it.  s is kept nowhere: `sum` may be x or the residual itself,
 // so it is written by the last pass, each element by the thread that reads it there.
 template <int kType, bool kF8>
@@ -276,10 +307,13 @@ SILE_DEV void norm_any(const NormArgs& a) {
 
 }  // namespace
 
-// t<threads of a row>_v<vectors of a thread>; w: four rows a workgroup, a wave each
-#define SILE_NORM(NAME, TYPE, F8, T, V, WG)                                                       \
-  extern "C" __global__ __launch_bounds__(WG) void sile_rmsnorm_##NAME##_t##T##_v##V(NormArgs a) { \
-    norm_rows<TYPE, F8, T, V, WG>(a);                                                             \
+// t<threads of a row>_v<vectors of a thread>, p: columns that are no whole vectors
+#define SILE_NORM(NAME, TYPE, F8, T, V, WG)                                                         \
+  extern "C" __global__ __launch_bounds__(WG) void sile_rmsnorm_##NAME##_t##T##_v##V(NormArgs a) {  \
+    norm_rows<TYPE, F8, T, V, WG, false>(a);                                                        \
+  }                                                                                                 \
+  extern "C" __global__ __launch_bounds__(WG) void sile_rmsnorm_##NAME##_t##T##_v##V##p(NormArgs a) { \
+    norm_rows<TYPE, F8, T, V, WG, true>(a);                                                         \
   }
 #define SILE_NORM_TYPES(NAME, TYPE, F8)                                                        \
   SILE_NORM(NAME, TYPE, F8, 64, 1, 256)                                                        \

@@ -341,12 +341,9 @@ int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows,
     return fail(SILE_ERR_SHAPE, "an output overlaps another operand without being its rows");
   NormArgs a{x, residual, weight, sum, y, scales, rows, ldx, ldr, lds, ldy, (int32_t)cols, (int32_t)group,
              eps, 1.0f / (float)cols, scale, reciprocal(scale)};
-  const int64_t e16 = 16 / es;
+  // a row in registers, and a group in a lane, lanes of one wave or all of the row
   const bool vectors =
-      cols % 8 == 0 && cols <= 16384 && ldx % e16 == 0 && (!residual || ldr % e16 == 0) && (!sum || lds % e16 == 0) &&
-      ldy % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(sum) && aligned16(weight) &&
-      (fp8 ? aligned_to(y, 8) : aligned16(y)) &&
-      (group == 0 || group == cols || (group <= 512 && group >= 8 && (group & (group - 1)) == 0));
+      cols <= 16384 && (group == 0 || group == cols || (group <= 512 && group >= 8 && (group & (group - 1)) == 0));
   int cus = 0;
   int rc = device_cus(&cus);
   if (rc != SILE_OK) return rc;
@@ -357,7 +354,7 @@ int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows,
     per = cols <= 512 ? 1 : (int)((cols + threads * 8 - 1) / (threads * 8));
     per = per == 3 ? 4 : per;
     wg = threads == 64 ? 256 : threads;
-    snprintf(form, sizeof form, "t%d_v%d", threads, per);
+    snprintf(form, sizeof form, "t%d_v%d%s", threads, per, cols % 8 != 0 ? "p" : "");
   } else {
     snprintf(form, sizeof form, "any");
   }
