@@ -35,8 +35,8 @@
 // maximum allows, so that those far below the maximum keep their bits.
 //
 // Measured, 32 query heads of 128 over 8 key heads: 2048 tokens behind 30000 keys 1.19 ms (875 TFLOP/s, the
-// matrix cores and their power), 8192 from none 0.71 ms; 32 pieces of 8 tokens over up to 8192 keys 130 us
-// (4.3 TB/s; a key more costs its bytes at 5.1 TB/s), as e4m3 codes 90 us; 1 piece of 4 over 300 13 us.
+// matrix cores and their power), 8192 from none 0.71 ms; 32 pieces of 8 tokens over up to 8192 keys 115 us
+// (4.8 TB/s), as e4m3 codes 86 us; 1 piece of 4 over 300 13 us.
 #include <type_traits>
 
 #include "common.h"
@@ -594,13 +594,15 @@ __device__ __forceinline__ bool chunk_units(const ChunkArgs& a, const uint16_t* 
     // no other; the waves' results are joined through LDS.  (One wave with all blocks, the others
     // loading for it, as with more rows, was held up by its products and softmax: with e4m3
     // codes 32 pieces of 8 over up to 8192 keys took 108 us, now 90; 3 pieces of up to 700 and 48 single
-    // tokens 164, now 146.  16-bit keys come at 5.1 TB/s either way.) ----
+    // tokens 164, now 146.) ----
     if constexpr (kNarrow) {
       constexpr int kN = kTileB / 1024;                          // DMAs of a tile
       constexpr int kOwn = kNK * kDp / kLoadElems / 64;          // or loads of a lane
       constexpr int kPer = kDp / kLoadElems;                     // loads of a row
       u32x4 own_k[kSrc == kDma ? 1 : kOwn], own_v[kSrc == kDma ? 1 : kOwn];
-      // past the part nothing is read
+      // past the part nothing is read; the loads are non-temporal, as no other tile of the sequence, or at most
+      // the larger ones before it, reads these keys (32 pieces of 8: 129 -> 115 us, of e4m3 90 -> 86)
+      constexpr int kOnce = 2;
       auto own_dma = [&](const uint8_t* from, uint8_t* to, bool is_v, int e, const Keys& k) {
         const int end = e < b1 ? len - block_of(e) * kNK : 0;
 #pragma unroll
@@ -613,7 +615,7 @@ __device__ __forceinline__ bool chunk_units(const ChunkArgs& a, const uint16_t* 
           const int rows_in = sgpr(min(max(end - row0, 0), kDmaRows));
           const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
               (void*)(from + at), (short)0, hi < 0 ? 0 : rows_in * row_b, 0x00020000);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(to + i * 1024), 16, off, 0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(to + i * 1024), 16, off, 0, 0, kOnce);
         }
       };
       auto own_fetch = [&](const uint8_t* from, u32x4* to, int e, const Keys& k) {
@@ -624,7 +626,8 @@ __device__ __forceinline__ bool chunk_units(const ChunkArgs& a, const uint16_t* 
           const int hi = __shfl(k.hi, row);
           const uint64_t at = (uint64_t)(uint32_t)hi << 32 | (uint32_t)__shfl((int)k.lo, row);
           u32x4 w = {0u, 0u, 0u, 0u};
-          if (hi >= 0 && row < end && ch * kLoadElems < d) w = *reinterpret_cast<const u32x4*>(from + at + ch * 16);
+          if (hi >= 0 && row < end && ch * kLoadElems < d) 
+            w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from + at + ch * 16));
           to[i] = w;
         }
       };
