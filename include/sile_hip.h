@@ -608,7 +608,7 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
                                size_t workspace_bytes, sile_hip_stream stream);
 
 /* Workspace bytes that sile_hip_paged_attn_chunk needs on the current device (for any lengths;
- * at most some 71 MB beside 4 for each 128 rows of tokens x query heads a key head). */
+ * at most some 71 MB beside 16 for each 128 rows of tokens x query heads a key head). */
 int sile_hip_paged_attn_chunk_workspace(int64_t n_rows, int64_t n_tokens, int64_t q_heads,
                                         int64_t kv_heads, int64_t head_dim, size_t *bytes);
 

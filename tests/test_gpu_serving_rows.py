@@ -169,6 +169,17 @@ def test_norm_unaligned(hip, shift):
             c.check()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols", [3, 511, 513, 2047, 5001, 8193, 16383])
+def test_norm_of_part_vectors(hip, dtype, cols):
+    """Rows that end inside a vector and begin anywhere; nothing behind them is written."""
+    for shift, pad in ((0, 1), (1, 5), (3, 0)):
+        for out, group in ((dtype, 0), ("fp8", 0), ("fp8", cols)):
+            c = Norm(hip, shift + cols, dtype, out, 3, cols, group=group, pad=pad, shift=shift)
+            c.run()
+            c.check()
+
+
 def test_norm_of_zeros_and_extremes(hip):
     """A row of zeros, one whose maximum is below the least, rows with Inf and NaN."""
     for cols in (256, 255):
