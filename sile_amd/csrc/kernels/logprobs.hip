@@ -17,9 +17,11 @@
 //
 // Few long rows: a row's chunks go to several workgroups, and a second launch joins their parts.
 //
+// The loads are non-temporal (below 54 -> 52, without top ones 45 -> 41 and 27 -> 25).
+//
 // Measured: 64 rows of 131072 in bf16, 20 top ones, 20 us (14 and the join 6; without top ones 9), one
-// row 14; 2000 rows of 32001 in f32, 5 top ones, 54 (4.8 TB/s; without 45), of 32000 in bf16, 20 top ones,
-// 50 (without 27).  What holds them is the latency of the list's steps, then instructions: a quarter
+// row 14; 2000 rows of 32001 in f32, 5 top ones, 52 (4.9 TB/s; without 41), of 32000 in bf16, 20 top ones,
+// 51 (without 25).  What holds them is the latency of the list's steps, then instructions: a quarter
 // of the time without top ones is exp2's.
 #include <type_traits>
 
@@ -253,7 +255,7 @@ SILE_DEV void logprobs(const LogprobArgs& a, List* s) {
       const int64_t at = (int64_t)chunk * kChunk + (i * kThreads + tid) * kPer;
       constexpr uint32_t kNone = kType == 0 ? 0xff800000u : kType == 1 ? 0xfc00fc00u : 0xff80ff80u;   // -inf
       u32x4 w = {kNone, kNone, kNone, kNone};
-      if (at < whole) w = *reinterpret_cast<const raw_t*>(base + at * (kType == 0 ? 4 : 2));
+      if (at < whole) w = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(base + at * (kType == 0 ? 4 : 2)));
       next[i] = w;
     }
   };

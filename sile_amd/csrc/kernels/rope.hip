@@ -16,9 +16,9 @@
 // up to four items (two vectors, of E pairs or of E dims and the E next), then work out each
 // angle of the tokens once, for all heads, into LDS, and then rotate and store.
 //
-// Measured: 16382 tokens of 32 + 2 x 8 heads of 128, bf16, with append 96 us (4.2 TB/s; 88 with nothing rotated), into
-// e4m3 pages 100 (3.7 TB/s: the vector units are busy for 57 % of it); 5000 tokens of f16, 32 of 128 dims
-// rotated, 40 (4.1 TB/s); 64 tokens 5.
+// Measured: 16382 tokens of 32 + 2 x 8 heads of 128, bf16, with append 90 us (4.5 TB/s), into e4m3 pages
+// 97 (3.8 TB/s: the vector units are busy for 57 % of it); 5000 tokens of f16, 32 of 128 dims rotated, 38.5
+// (4.3 TB/s); 64 tokens 5.  The loads are non-temporal: 96, 100 and 41 us without.
 #include "common.h"
 #include "e4m3.h"
 
@@ -175,8 +175,8 @@ SILE_DEV void rope(const RopeArgs& a) {
     if (i >= n) break;
     const Item m = item(i);
     const uint8_t* p = source(m);
-    raw[u][0] = *reinterpret_cast<const V*>(p + m.o0 * kEs);
-    if (m.two) raw[u][1] = *reinterpret_cast<const V*>(p + m.o1 * kEs);
+    raw[u][0] = __builtin_nontemporal_load(reinterpret_cast<const V*>(p + m.o0 * kEs));
+    if (m.two) raw[u][1] = __builtin_nontemporal_load(reinterpret_cast<const V*>(p + m.o1 * kEs));
   }
 
   // ---- the tokens' angles, positions and slots ----
