@@ -709,12 +709,13 @@ int sile_hip_logprobs_workspace(int64_t rows, int64_t cols, int64_t top_k, size_
  *   entropy[r]   - sum p log p
  *   top_ids[r], top_logp[r]   [top_k], the columns of the largest x, largest first, of equal
  *                ones the lowest first, and their log p; top_k at most 64
- * logp and entropy may be NULL, and top_k 0.  Columns of -inf have log p -inf and are never among
- * the top ones: where fewer than top_k are left the rest is -1 with -inf.  A row of nothing else:
- * logp and top_logp -inf, entropy 0.  A NaN or +inf makes the row's numbers NaN; its top_ids are
- * those of the comparisons (+inf first, NaN never).  A row's chunks may be shared out over
- * workgroups, by rows and cols, so its rounding can depend on both; the same call gives the same
- * bits. */
+ * logp, top_logp and entropy keep their digits where one column has nearly all of the mass (the
+ * rest is summed apart).  logp and entropy may be NULL, and top_k 0.  Columns of -inf have log p
+ * -inf and are never among the top ones: where fewer than top_k are left the rest is -1 with -inf.
+ * A row of nothing else: logp and top_logp -inf, entropy 0.  A NaN or +inf makes the row's numbers
+ * NaN; its top_ids are those of the comparisons (+inf first, NaN never).  A row's chunks may be
+ * shared out over workgroups, by rows and cols, so its rounding can depend on both; the same call
+ * gives the same bits. */
 int sile_hip_logprobs_rows(sile_dtype in_type, int64_t rows, int64_t cols, const void *x,
                            int64_t ldx, float scale, const int32_t *targets, float *logp,
                            float *entropy, int64_t top_k, float *top_logp, int32_t *top_ids,

@@ -7,21 +7,32 @@
 // Memory bounds it: every logit is read once (16 bytes a load, two chunks of 8192 in flight) and
 // kept in registers while a lane folds it into its own running (max m, sum l of p = 2^(c (x - m)),
 // sum e of p (x - m)), c = scale log2 e.  The difference comes first, so that logits at the type's
-// lowest value stay numbers; e keeps the entropy's digits where one token has nearly all the mass.  What the top ones cost
-// beside that: every wave keeps the k best of its columns in order, an entry a lane, and a chunk's largest
-// value of a lane is compared with the k-th; where one passes (rarely, after the first chunk) its
-// elements are, and what passes is put in its place by a shift of the lanes behind it.  In the first
-// chunk the ceil(k / 4)-th largest of the lanes' maxima, the least of the four waves', stands for the k-th best:
-// k elements reach it.  After that no wave waits for another before its last column.  (Candidates of the workgroup in LDS, ranked by counting
-// after each chunk: 77 us both below; sorted and merged by one wave: 24 and 82.)
+// lowest value stay numbers.
+//
+// One token often has nearly all the mass, and what counts is then the rest: with u = l less the p = 1
+// of one column that has the maximum, log l = log1p(u) and the entropy log1p(u) - scale e / (1 + u), of
+// two terms of one sign, keep their digits however small u is (from l itself, a u of 1e-8 is gone and
+// one of 1e-3 good to 1e-4).  A wave whose l is below 1.25 works its u out anew: the other lanes' l, and the
+// columns of one lane that has the maximum again, a 64th of the wave's, without it; above, l - 1 has
+// lost two or three bits at most.  (Of the rows of 32000 below a quarter has such a wave: without top
+// ones 25.5 -> 27.5 us in bf16 and 41.2 -> 42 in f32.  In every wave it took 29.5 and 46, a sum of its own
+// of what is below the maximum, in every lane, 30 and 44.)
+//
+// What the top ones cost beside that: every wave keeps the k best of its columns in order, an
+// entry a lane, and a chunk's largest value of a lane is compared with the k-th; where one passes
+// (rarely, after the first chunk) its elements are, and what passes is put in its place by a shift
+// of the lanes behind it.  In the first chunk the ceil(k / 4)-th largest of the lanes' maxima, the
+// least of the four waves', stands for the k-th best: k elements reach it.  After that no wave waits
+// for another before its last column.  (Candidates of the workgroup in LDS, ranked by counting after
+// each chunk: 77 us both below; sorted and merged by one wave: 24 and 82.)
 //
 // Few long rows: a row's chunks go to several workgroups, and a second launch joins their parts.
 //
 // The loads are non-temporal (below 54 -> 52, without top ones 45 -> 41 and 27 -> 25).
 //
 // Measured: 64 rows of 131072 in bf16, 20 top ones, 20 us (14 and the join 6; without top ones 9), one
-// row 14; 2000 rows of 32001 in f32, 5 top ones, 52 (4.9 TB/s; without 41), of 32000 in bf16, 20 top ones,
-// 51 (without 25).  What holds them is the latency of the list's steps, then instructions: a quarter
+// row 14; 2000 rows of 32001 in f32, 5 top ones, 55 (4.6 TB/s; without 42), of 32000 in bf16, 20 top ones,
+// 50 (without 27).  What holds them is the latency of the list's steps, then instructions: a quarter
 // of the time without top ones is exp2's.
 #include <type_traits>
 
@@ -42,7 +53,7 @@ struct LogprobArgs {
   const int32_t* targets;
   float *logp, *entropy, *top_logp;           // each may be NULL (top_logp with top_ids)
   int32_t* top_ids;
-  float* part_sums;                           // [rows][parts][4]: m, l, e
+  float* part_sums;                           // [rows][parts][4]: m, u, e
   float* part_top;                            // [rows][parts][top]: values
   int32_t* part_ids;                          // their columns
   int64_t ldx;
@@ -172,34 +183,42 @@ SILE_DEV void merge_waves(List* s, Entry t, int top) {
   __syncthreads();
 }
 
-// the lane's sums as those of a maximum of `top`, which is at least m (both -inf: nothing to scale)
+// the sums l and e of a maximum m as those of a maximum of `top`, which is at least m (both -inf:
+// nothing to scale)
 SILE_DEV void rescale(const LogprobArgs& a, float m, float& l, float& e, float top) {
   const float d = m == top ? 0.0f : m - top, f = exp2_fast(d * a.scale_log2);
   e = f * (e + l * __builtin_fmaxf(d, a.floor));
   l *= f;
 }
-// the sums of all threads, joined
-SILE_DEV void all_sums(const LogprobArgs& a, List* s, float& m, float& l, float& e) {
-  const float top = wave_max(m);
-  rescale(a, m, l, e, top);
-  l = wave_sum(l);
-  e = wave_sum(e);
+// The same with u, l less the 1 of a maximum of its own: where m is less than `top` that one counts with
+// the rest; where not, u stays as it is, and the function is 1.  (m = -inf, no column: u means nothing, and
+// becomes 0 under a larger maximum.)
+SILE_DEV float rescale_rest(const LogprobArgs& a, float m, float& u, float& e, float top) {
+  if (m == top) return 1.0f;
+  u += 1.0f;
+  rescale(a, m, u, e, top);
+  return 0.0f;
+}
+// the waves' sums (m, u, e), joined
+SILE_DEV void waves_sums(const LogprobArgs& a, List* s, float& m, float& u, float& e) {
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) == 0) {
-    s->sums[wave][0] = top;
-    s->sums[wave][1] = l;
+    s->sums[wave][0] = m;
+    s->sums[wave][1] = u;
     s->sums[wave][2] = e;
   }
   __syncthreads();
   m = __builtin_fmaxf(__builtin_fmaxf(s->sums[0][0], s->sums[1][0]), __builtin_fmaxf(s->sums[2][0], s->sums[3][0]));
-  l = e = 0.0f;
+  u = e = 0.0f;
+  float largest = -1.0f;   // waves that have the maximum, but one
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    float lw = s->sums[w][1], ew = s->sums[w][2];
-    rescale(a, s->sums[w][0], lw, ew, m);
-    l += lw;
+    float uw = s->sums[w][1], ew = s->sums[w][2];
+    largest += rescale_rest(a, s->sums[w][0], uw, ew, m);
+    u += uw;
     e += ew;
   }
+  u += largest;
 }
 
 // the logit of the row's target, asked for ahead of its use; thread 0
@@ -212,17 +231,14 @@ SILE_DEV float target_logit(const LogprobArgs& a, int row, bool* there) {
   return *there ? logit<kType>(a.x, row * a.ldx + t) : 0.0f;
 }
 // the results of a row from its sums and the list
-SILE_DEV void finish(const LogprobArgs& a, const List* s, int row, float target, bool there, float m, float l, float e) {
+SILE_DEV void finish(const LogprobArgs& a, const List* s, int row, float target, bool there, float m, float u, float e) {
   const int tid = threadIdx.x;
-  const float log_l = logf(l);
-  const bool none = m == -__builtin_inff() && l == 0.0f;   // every logit is -inf
+  const float log_l = log1pf(u);
+  const bool none = m == -__builtin_inff() && u == u;   // every logit is -inf
   auto logp_of = [&](float x) { return none ? -__builtin_inff() : (x - m) * a.scale - log_l; };
   if (tid == 0) {
     if (a.logp) a.logp[row] = there ? logp_of(target) : 0.0f;
-    if (a.entropy) {
-      const float h = none ? 0.0f : log_l - e / l * a.scale;
-      a.entropy[row] = h < 0.0f ? 0.0f : h;   // (by rounding; NaN stays)
-    }
+    if (a.entropy) a.entropy[row] = none ? 0.0f : log_l - e / (1.0f + u) * a.scale;
   }
   if (a.top_ids && tid < a.top) {
     const float v = s->value[0][tid];
@@ -340,20 +356,54 @@ SILE_DEV void logprobs(const LogprobArgs& a, List* s) {
     const float some = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(best.v), few - 1));
     if (lane == 0 && chunk != c_first) __hip_atomic_store(&s->quarter[wave], some, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
+  float tail = -__builtin_inff();
   if (part == a.parts - 1 && whole < a.cols && wave == 0) {   // the row's last few: a lane one
-    const float v = tid < a.cols - whole ? logit<kType>(base, whole + tid) : -__builtin_inff();
-    grow(v);
-    add(v, m == -__builtin_inff() ? 0.0f : m);
-    if (a.top != 0) place(v, whole + tid);
+    if (tid < a.cols - whole) tail = logit<kType>(base, whole + tid);
+    grow(tail);
+    add(tail, m == -__builtin_inff() ? 0.0f : m);
+    if (a.top != 0) place(tail, whole + tid);
   }
+  // ---- the wave's sums, its maximum's 1 apart ----
+  const float top_m = wave_max(m);
+  rescale(a, m, l, e, top_m);
+  float u = wave_sum(l) - 1.0f;
+  if (top_m > -__builtin_inff() && !(u >= 0.25f)) {
+    // the columns of a lane that has the maximum again, but for the first at it (m is no NaN)
+    const int owner = __builtin_ctzll(__builtin_amdgcn_ballot_w64(m == top_m));
+    u = lane == owner ? 0.0f : l;
+    bool found = false;
+    const int n = (c_last - c_first) * kElems, first = (wave * 64 + owner) * kPer;
+    for (int j0 = 0; j0 < n; j0 += 256) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 64 * i + lane;
+        const int64_t at = (int64_t)(c_first + j / kElems) * kChunk + first + j % kElems / kPer * (kThreads * kPer) + j % kPer;
+        v[i] = j < n && at < whole ? logit<kType>(base, at) : -__builtin_inff();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t at_top = __builtin_amdgcn_ballot_w64(v[i] == top_m);
+        const bool out = !found && at_top != 0 && lane == __builtin_ctzll(at_top);
+        found |= at_top != 0;
+        const float d = v[i] - top_m;   // (of a +inf NaN, also where it is left out)
+        u += out ? d : exp2_fast(d * c);
+      }
+    }
+    const float d = bits_f32((uint32_t)__builtin_amdgcn_readlane((int)f32_bits(tail), owner)) - top_m;
+    if (lane == 0) u += found ? exp2_fast(d * c) : d;
+    u = wave_sum(u);
+  }
+  e = wave_sum(e);
+  m = top_m;
   if (a.top != 0) merge_waves(s, best, a.top);
-  all_sums(a, s, m, l, e);
+  waves_sums(a, s, m, u, e);
   if (a.parts == 1) {
-    finish(a, s, row, target, there, m, l, e);
+    finish(a, s, row, target, there, m, u, e);
     return;
   }
   const int64_t at = (int64_t)row * a.parts + part;
-  if (tid == 0) *reinterpret_cast<f32x4*>(a.part_sums + 4 * at) = f32x4{m, l, e, 0.0f};
+  if (tid == 0) *reinterpret_cast<f32x4*>(a.part_sums + 4 * at) = f32x4{m, u, e, 0.0f};
   if (tid < a.top) {
     a.part_top[at * a.top + tid] = s->value[0][tid];
     a.part_ids[at * a.top + tid] = s->column[0][tid];
@@ -367,35 +417,39 @@ SILE_DEV void logprobs_join(const LogprobArgs& a, List* s) {
   const int64_t first = (int64_t)row * a.parts;
   bool there;
   const float target = target_logit<kType>(a, row, &there);
-  float m = -__builtin_inff(), l = 0.0f, e = 0.0f;
+  float m = -__builtin_inff(), u = 0.0f, e = 0.0f;
   for (int p = tid; p < a.parts; p += kThreads) {
     const f32x4 w = *reinterpret_cast<const f32x4*>(a.part_sums + 4 * (first + p));
     const float top = __builtin_fmaxf(m, w[0]);
-    float lw = w[1], ew = w[2];
-    rescale(a, m, l, e, top);
-    rescale(a, w[0], lw, ew, top);
+    float uw = w[1], ew = w[2];
+    const float both = rescale_rest(a, m, u, e, top) * rescale_rest(a, w[0], uw, ew, top);
     m = top;
-    l += lw;
+    u += uw + both;
     e += ew;
   }
   if (a.top) {
     // a part's list is in order; the next one is on its way
     auto list = [&](int p) {
-      Entry u = no_entry();
-      if (lane < a.top && p < a.parts) u = {a.part_top[(first + p) * a.top + lane], a.part_ids[(first + p) * a.top + lane]};
-      return u;
+      Entry some = no_entry();
+      if (lane < a.top && p < a.parts) some = {a.part_top[(first + p) * a.top + lane], a.part_ids[(first + p) * a.top + lane]};
+      return some;
     };
-    Entry t = list(wave), u = list(wave + 4);
+    Entry t = list(wave), next = list(wave + 4);
 #pragma unroll 1
     for (int p = wave + 4; p < a.parts; p += 4) {
       const Entry ahead = list(p + 4);
-      merge64(t, u, a.top);
-      u = ahead;
+      merge64(t, next, a.top);
+      next = ahead;
     }
     merge_waves(s, t, a.top);
   }
-  all_sums(a, s, m, l, e);
-  finish(a, s, row, target, there, m, l, e);
+  const float top_m = wave_max(m);
+  const float own = rescale_rest(a, m, u, e, top_m);
+  u = wave_sum(u) + (wave_sum(own) - 1.0f);
+  e = wave_sum(e);
+  m = top_m;
+  waves_sums(a, s, m, u, e);
+  finish(a, s, row, target, there, m, u, e);
 }
 
 }  // namespace
