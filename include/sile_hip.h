@@ -663,8 +663,9 @@ int sile_hip_rope_turns(sile_rope_scaling scaling, int64_t rot_dim, double base,
  * and dims from rot_dim on are copied; fp32, rounded once.  Negative turns turn back.  dtype f32, f16
  * or bf16; tokens at q + t * ldq, k + t * ldk, [heads][head_dim] (leading dimensions up to 2^25), any
  * alignment and head_dim up to 2048 (16-byte aligned and rot_dim a multiple of 16 is fastest); q_heads or kv_heads may be
- * 0.  An output is its input (same pointer and leading dimension) or apart from it.  A token
- * at a position below 0 is left out: its outputs stay as they are. */
+ * 0.  An output is its input (same pointer and leading dimension) or apart from it, and apart from
+ * everything else of the call (rows may lie between another's, as in a fused projection):
+ * refused otherwise.  A token at a position below 0 is left out: its outputs stay as they are. */
 int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, int64_t q_heads,
                   int64_t kv_heads, int64_t head_dim, int64_t rot_dim, const void *q, int64_t ldq,
                   void *q_out, int64_t ldqo, const void *k, int64_t ldk, void *k_out, int64_t ldko,
@@ -674,7 +675,8 @@ int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, i
 /* sile_hip_rope of the queries, and sile_hip_kv_append of the rotated keys and of the values, in
  * one launch: the keys are rounded once, to the cache's type (e4m3: k / scale of the fp32
  * result).  Arguments and what is left out as for the two; a token without a page in the
- * cache still has its queries turned. */
+ * cache still has its queries turned.  The pages, K's and V's, are apart from each other and from
+ * everything else of the call, as q_out is: refused otherwise. */
 int sile_hip_rope_append(sile_dtype dtype, sile_dtype cache_type, sile_rope_layout layout,
                          int64_t n_tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                          int64_t rot_dim, const void *q, int64_t ldq, void *q_out, int64_t ldqo,

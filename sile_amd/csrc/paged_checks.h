@@ -88,6 +88,53 @@ inline int check_in_out(const int32_t* in, const int32_t* out, int64_t n, const 
   return SILE_OK;
 }
 
+// Memory of an operand: `rows` runs of `width` bytes, `pitch` bytes apart (an array: one).
+struct Region {
+  const char* name;
+  const void* p;
+  int64_t rows, pitch, width;
+};
+inline Region array_of(const char* name, const void* p, int64_t bytes) { return {name, p, 1, 0, bytes}; }
+// Whether two share a byte.  Rows may lie in the gaps of the other's, as a fused projection's queries and
+// keys do.
+inline bool regions_share(const Region& x, const Region& y) {
+  if (!x.p || !y.p || x.rows <= 0 || y.rows <= 0 || x.width <= 0 || y.width <= 0) return false;
+  const int64_t px = x.rows > 1 ? x.pitch : 0, py = y.rows > 1 ? y.pitch : 0;
+  const int64_t x0 = 0, y0 = (int64_t)(reinterpret_cast<uintptr_t>(y.p) - reinterpret_cast<uintptr_t>(x.p));
+  if (x0 + (x.rows - 1) * px + x.width <= y0 || y0 + (y.rows - 1) * py + y.width <= x0) return false;
+  // apart at every row, if they are so modulo a step of both
+  int64_t step = px, rest = py;
+  while (rest != 0) {
+    const int64_t r = step % rest;
+    step = rest;
+    rest = r;
+  }
+  if (step == 0) return true;   // two arrays
+  const int64_t off = (y0 % step + step) % step;
+  if (off >= x.width && off + y.width <= step) return false;
+  // row by row, past those that end before the other's next
+  for (int64_t i = 0, j = 0; i < x.rows && j < y.rows;) {
+    const int64_t xs = i * px, ys = y0 + j * py;
+    if (xs + x.width <= ys)
+      i = px == 0 ? x.rows : i + (ys - xs - x.width) / px + 1;
+    else if (ys + y.width <= xs)
+      j = py == 0 ? y.rows : j + (xs - ys - y.width) / py + 1;
+    else
+      return true;
+  }
+  return false;
+}
+// what a call writes apart from each other and from what it reads
+inline int check_written(std::initializer_list<Region> written, std::initializer_list<Region> read) {
+  for (const Region* x = written.begin(); x != written.end(); ++x) {
+    for (const Region* y = x + 1; y != written.end(); ++y)
+      if (regions_share(*x, *y)) return fail(SILE_ERR_SHAPE, "%s overlaps %s", x->name, y->name);
+    for (const Region& y : read)
+      if (regions_share(*x, y)) return fail(SILE_ERR_SHAPE, "%s overlaps %s", x->name, y.name);
+  }
+  return SILE_OK;
+}
+
 inline int check_heads(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
   if (batch < 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || q_heads % kv_heads != 0)
     return fail(SILE_ERR_SHAPE, "batch %lld, %lld query heads over %lld key heads of %lld",

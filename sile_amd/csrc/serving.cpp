@@ -213,9 +213,15 @@ int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, i
   if (std::max({ldq, ldqo, ldk, ldko}) > (1 << 25)) return fail(SILE_ERR_SHAPE, "leading dimension past 2^25");
   for (const void* p : {q, (const void*)q_out, k, (const void*)k_out})
     if (!aligned_to(p, es)) return fail(SILE_ERR_SHAPE, "tokens not aligned to their type");
-  if ((q_heads > 0 && !in_place_or_apart(q, ldq, q_out, ldqo, n_tokens, nq, es)) ||
-      (kv_heads > 0 && !in_place_or_apart(k, ldk, k_out, ldko, n_tokens, nk, es)))
+  const Region rq{"q", q, n_tokens, ldq * es, nq * es}, ro{"q's output", q_out, n_tokens, ldqo * es, nq * es};
+  const Region rk{"k", k, n_tokens, ldk * es, nk * es}, rp{"k's output", k_out, n_tokens, ldko * es, nk * es};
+  if ((q_heads > 0 && !(q == q_out && ldq == ldqo) && regions_share(rq, ro)) ||
+      (kv_heads > 0 && !(k == k_out && ldk == ldko) && regions_share(rk, rp)))
     return fail(SILE_ERR_SHAPE, "an output overlaps its input without being the same");
+  const Region angles = array_of("turns", turns, 4 * rot_dim), at = array_of("positions", positions, 4 * n_tokens);
+  if ((rc = check_written({ro, rp}, {at, angles})) != SILE_OK || (rc = check_written({ro}, {rk})) != SILE_OK ||
+      (rc = check_written({rp}, {rq})) != SILE_OK)
+    return rc;
   RopeArgs a{};
   if (q_heads > 0) {
     a.q = q;
@@ -264,8 +270,18 @@ int sile_hip_rope_append(sile_dtype dtype, sile_dtype cache_type, sile_rope_layo
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) || ldk % 8 || ldv % 8 ||
       (q_heads > 0 && (!aligned16(q) || !aligned16(q_out) || ldq % 8 || ldqo % 8)))
     return fail(SILE_ERR_SHAPE, "tokens and pages have to be 16-byte aligned");
-  if (q_heads > 0 && !in_place_or_apart(q, ldq, q_out, ldqo, n_tokens, nq, 2))
+  const Region rq{"q", q, n_tokens, ldq * 2, nq * 2}, ro{"q's output", q_out, n_tokens, ldqo * 2, nq * 2};
+  const Region rk{"k", k, n_tokens, ldk * 2, nk * 2}, rv{"v", v, n_tokens, ldv * 2, nk * 2};
+  if (q_heads > 0 && !(q == q_out && ldq == ldqo) && regions_share(rq, ro))
     return fail(SILE_ERR_SHAPE, "an output overlaps its input without being the same");
+  const int64_t page = kv_heads * page_size * head_dim * es;
+  const Region kp{"K's pages", k_pages, num_pages, page_stride * es, page};
+  const Region vp{"V's pages", v_pages, num_pages, page_stride * es, page};
+  const Region angles = array_of("turns", turns, 4 * rot_dim), at = array_of("positions", positions, 4 * n_tokens);
+  const Region of = array_of("rows", rows, 4 * n_tokens), pages = array_of("tables", tables, 4 * n_rows * ld_table);
+  if ((rc = check_written({ro, kp, vp}, {rk, rv, at, of, angles, pages})) != SILE_OK ||
+      (rc = check_written({kp, vp}, {rq})) != SILE_OK)
+    return rc;
   RopeArgs a{};
   if (q_heads > 0) {
     a.q = q;

@@ -1,0 +1,88 @@
+"""What the serving step's calls write overlaps nothing else of the call: refused before any device
+work.  Memory that only lies between another's rows is none of it, and no call is refused for it."""
+import ctypes
+
+import pytest
+
+from sile_amd import _abi
+from tests.test_serving_abi import APPEND, P, ROPE, refused
+
+
+def passes(f, **kw):
+    """The checks let the call pass, which without a GPU ends at its first look at the device."""
+    count = ctypes.c_int(0)
+    _abi.call("sile_hip_device_count", ctypes.byref(count))
+    if count.value:
+        pytest.skip("made-up addresses: only where no kernel can run")
+    with pytest.raises(_abi.SileError) as e:
+        f(**kw)
+    assert e.value.kind != "Shape", str(e.value)
+
+
+# tokens of a fused projection: 4 query heads, 2 key heads and 2 value heads of 64, 512 elements of 2 bytes
+FUSED = dict(q=P, ldq=512, k=P + 512, ldk=512)
+
+
+def test_rope():
+    f = _abi.rope
+    for change in (dict(q_out=3 * P), dict(q_out=3 * P + 64), dict(k_out=P), dict(k_out=P + 3 * 512 + 256), dict(k_out=2 * P),
+                   dict(q_out=4 * P - 512), dict(q_out=5 * P - 1536), dict(k_out=5 * P), dict(q_out=6 * P), dict(k_out=6 * P - 1008),
+                   {**FUSED, "k_out": P + 256, "ldko": 512}, {**FUSED, "q_out": P + 256, "ldqo": 512},
+                   {**FUSED, "q_out": P, "ldqo": 512, "k_out": P + 384, "ldko": 512},
+                   {**FUSED, "q_out": P + 640, "ldqo": 1024}):
+        refused("Shape", f, **{**ROPE, **change})
+
+
+def test_rope_between_rows():
+    f = _abi.rope
+    for change in ({**FUSED, "q_out": P, "ldqo": 512, "k_out": P + 512, "ldko": 512},   # in place
+                   {**FUSED, "k_out": P + 768, "ldko": 512},                            # over the values
+                   {**FUSED, "k_out": P + 768, "ldko": 1024},                           # over every other token's
+                   dict(q=P, ldq=512, q_out=P + 512, ldqo=512),
+                   dict(q_out=3 * P - 2048), dict(q_out=3 * P + 1024)):                 # end to end
+        passes(f, **{**ROPE, **change})
+
+
+def test_rope_append():
+    f = _abi.rope_append
+    page = 2048 * 2
+    for change in (dict(q_out=3 * P), dict(q_out=4 * P + 256), dict(q_out=5 * P), dict(q_out=6 * P), dict(q_out=7 * P + 512),
+                   dict(q_out=8 * P + 9 * page), dict(q_out=9 * P), dict(rows=2 * P), dict(v_pages=7 * P), dict(v_pages=7 * P + 9 * page),
+                   dict(k_pages=P), dict(v_pages=P + 512), dict(k_pages=3 * P), dict(v_pages=4 * P), dict(k_pages=5 * P), dict(v_pages=6 * P),
+                   dict(k_pages=9 * P), dict(k_pages=4 * P - 9 * page), dict(rows=8 * P),
+                   dict(page_stride=2 * 2048, v_pages=7 * P + page // 2), dict(page_stride=3 * 2048, v_pages=7 * P + 2 * page + 16)):
+        refused("Shape", f, **{**APPEND, **change})
+
+
+def test_rope_append_between_rows():
+    f = _abi.rope_append
+    page = 2048 * 2
+    for change in (dict(page_stride=2 * 2048, v_pages=7 * P + page),                   # K and V of a page side by side
+                   dict(page_stride=2 * 2048, k_pages=7 * P + page, v_pages=7 * P),
+                   dict(q=P, ldq=512, k=P + 512, ldk=512, v=P + 768, ldv=512),         # a fused projection
+                   dict(q=P, ldq=512, q_out=P, ldqo=512, k=P + 512, ldk=512, v=P + 768, ldv=512),
+                   dict(num_pages=0, v_pages=7 * P), dict(q_heads=0, q_out=3 * P), dict(v_pages=7 * P + 10 * page)):
+        passes(f, **{**APPEND, **change})
+
+
+def test_rows_as_sets():
+    """Whether rows of any pitch share a byte, against counting them."""
+    import random
+    rng = random.Random(3)
+    seen = [0, 0]
+    for _ in range(3000):
+        n, width = rng.randint(1, 6), 2 * rng.randint(1, 4)
+        lx, ly = width + rng.randint(0, 20), width + rng.randint(0, 20)
+        off = rng.randint(-60, 60)
+        if off == 0 and lx == ly:
+            continue
+        rows = lambda at, ld: {at + i * ld + j for i in range(n) for j in range(width)}   # noqa: E731
+        want = bool(rows(0, lx) & rows(off, ly))
+        seen[want] += 1
+        kw = dict(dtype=_abi.F32, layout=0, n_tokens=n, q_heads=1, kv_heads=0, head_dim=width, rot_dim=width, q=P, ldq=lx,
+                  q_out=P + 4 * off, ldqo=ly, k=0, ldk=0, k_out=0, ldko=0, positions=5 * P, turns=6 * P)
+        if want:
+            refused("Shape", _abi.rope, **kw)
+        else:
+            passes(_abi.rope, **kw)
+    assert min(seen) > 500
