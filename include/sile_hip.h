@@ -621,7 +621,8 @@ int sile_hip_paged_attn_chunk_workspace(int64_t n_rows, int64_t n_tokens, int64_
  * has are left as they are; a token at a position below 0 (lengths[r] below its tokens), or without any
  * seen key, gives zeros.  Everything else as for sile_hip_paged_attn_decode: q, o, the cache and
  * its e4m3 form, missing pages, NaN and Inf in keys that a token does not see, splitting and its
- * rounding; at most 2^29 keys a row.  o overlaps nothing that the call reads.  The
+ * rounding; at most 2^29 keys a row.  o overlaps nothing that the call reads (its rows may lie between
+ * q's), the workspace nothing at all: refused otherwise.  The
  * probabilities enter the second product in 16 bits (one part, where sile_hip_paged_attn_decode has
  * two), as in sile_hip_flash_attn_window_fwd; a token whose result is not finite, or that meets
  * Inf or NaN in V of a masked key of its blocks, is taken again in fp32: right, but slow. */

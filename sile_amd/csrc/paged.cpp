@@ -535,14 +535,18 @@ int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n
   if (ldq < width || ldo < width) return fail(SILE_ERR_SHAPE, "leading dimension smaller than a token's heads");
   if (!aligned16(q) || !aligned16(o) || !aligned16(k_pages) || !aligned16(v_pages) || ldq % 8 || ldo % 8)
     return fail(SILE_ERR_SHAPE, "q, o and the pages have to be 16-byte aligned");
-  if (ldq > (1ll << 40) || ldo > (1ll << 40)) return fail(SILE_ERR_SHAPE, "leading dimension too large");
+  if (std::max(ldq, ldo) > (1ll << 45) / n_tokens) return fail(SILE_ERR_SHAPE, "leading dimension too large");
   if (ld_table * page_size > (1ll << 29))
     return fail(SILE_ERR_SHAPE, "a table of %lld pages of %lld keys: at most 2^29 keys a row", (long long)ld_table,
                 (long long)page_size);
-  if (o < static_cast<const char*>(q) + ((n_tokens - 1) * ldq + width) * 2 &&
-      static_cast<const char*>(q) < static_cast<const char*>(o) + ((n_tokens - 1) * ldo + width) * 2)
-    return fail(SILE_ERR_SHAPE, "o overlaps q");
   ChunkPlan plan{};
+  const Region out{"o", o, n_tokens, ldo * 2, width * 2}, in{"q", q, n_tokens, ldq * 2, width * 2};
+  const int64_t page = kv_heads * page_size * head_dim * es;
+  const Region kp{"K's pages", k_pages, num_pages, page_stride * es, page};
+  const Region vp{"V's pages", v_pages, num_pages, page_stride * es, page};
+  const Region list = array_of("starts", starts, 4 * (n_rows + 1)), of = array_of("lengths", lengths, 4 * n_rows);
+  const Region pages = array_of("tables", tables, 4 * n_rows * ld_table);
+  if ((rc = check_written({out}, {in, kp, vp, list, of, pages})) != SILE_OK) return rc;
   const int block = head_dim <= 64 ? 64 : 32;
   // without a page every row is empty
   const int64_t capacity = num_pages > 0 ? ld_table * page_size : 0;
@@ -558,6 +562,8 @@ int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n
                 (long long)n_tokens, (long long)n_rows, (long long)seen);
   if ((rc = chunk_plan(n_rows, n_tokens, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, plan.bytes)) != SILE_OK) return rc;
+  if ((rc = check_written({array_of("workspace", workspace, plan.bytes)}, {out, in, kp, vp, list, of, pages})) != SILE_OK)
+    return rc;
   ChunkArgs a{};
   a.q = q;
   a.k = k_pages;

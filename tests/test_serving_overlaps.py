@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from sile_amd import _abi
-from tests.test_serving_abi import APPEND, P, ROPE, refused
+from tests.test_serving_abi import APPEND, CHUNK, P, ROPE, refused
 
 
 def passes(f, **kw):
@@ -86,3 +86,31 @@ def test_rows_as_sets():
         else:
             passes(_abi.rope, **kw)
     assert min(seen) > 500
+
+
+def test_chunk():
+    f = _abi.paged_attn_chunk
+    page = 2048 * 2
+    for change in (dict(o=P), dict(o=P + 29 * 512), dict(o=2 * P), dict(o=3 * P + page), dict(o=4 * P + 9 * page), dict(o=5 * P - 512),
+                   dict(o=6 * P), dict(o=3 * P - 29 * 512), dict(q=P, ldq=512, o=P + 256, ldo=1024),
+                   dict(page_stride=2 * 2048, o=3 * P + page, ldo=256)):
+        refused("Shape", f, **{**CHUNK, **change})
+    for change in (dict(q=P, ldq=512, o=P + 512, ldo=512), dict(o=P + 30 * 512), dict(o=4 * P - 30 * 512), dict(o=4 * P + 10 * page),
+                   dict(page_stride=2 * 2048, v_pages=3 * P + page), dict(num_pages=0, o=3 * P)):
+        passes(f, **{**CHUNK, **change})
+
+
+@pytest.mark.gpu
+def test_chunk_workspace(hip):
+    """A workspace over any operand of the call (its size is the device's to say).  Operands and workspaces
+    all lie in one allocation."""
+    need = hip.paged_attn_chunk_workspace(4, 30, 4, 2, 64)
+    far = (need + (1 << 20)) // 16 * 16
+    arena = hip.DeviceBuffer(10 * far)
+    arena.fill_bytes(0)
+    x = lambda i: arena.ptr + i * far   # noqa: E731
+    base = dict(q=x(1), starts=x(2), k_pages=x(3), v_pages=x(4), tables=x(5), lengths=x(6), o=x(7), workspace_bytes=need)
+    for at, over in ((1, 16), (2, 0), (3, 4096), (4, 9 * 4096), (5, 32), (6, 0), (7, 256)):
+        refused("Shape", hip.paged_attn_chunk, **{**CHUNK, **base, "workspace": x(at) + over})
+        refused("Shape", hip.paged_attn_chunk, **{**CHUNK, **base, "workspace": x(at) - need + 16})
+    arena.close()
