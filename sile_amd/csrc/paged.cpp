@@ -425,7 +425,12 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
     return fail(SILE_ERR_SHAPE, "leading dimension smaller than a token's heads");
   if (!aligned16(q) || !aligned16(o) || !aligned16(k_pages) || !aligned16(v_pages) || ldq % 8 || ldo % 8)
     return fail(SILE_ERR_SHAPE, "q, o and the pages have to be 16-byte aligned");
-  if (ldq > (1ll << 40) || ldo > (1ll << 40)) return fail(SILE_ERR_SHAPE, "leading dimension too large");
+  if (std::max(ldq, ldo) > (1ll << 45) / batch) return fail(SILE_ERR_SHAPE, "leading dimension too large");
+  const Region out{"o", o, batch, ldo * 2, q_heads * head_dim * 2}, in{"q", q, batch, ldq * 2, q_heads * head_dim * 2};
+  const int64_t page = kv_heads * page_size * head_dim * es;
+  const Region kp{"K's pages", k_pages, num_pages, page_stride * es, page};
+  const Region vp{"V's pages", v_pages, num_pages, page_stride * es, page};
+  const Region of = array_of("lengths", lengths, 4 * batch), pages = array_of("tables", tables, 4 * batch * ld_table);
   PagedPlan plan;
   paged_shape(q_heads, kv_heads, head_dim, &plan);
   // without a page every row is empty
@@ -438,8 +443,10 @@ int sile_hip_paged_attn_decode(sile_dtype dtype, sile_dtype cache_type, int64_t 
   if (batch > (kIntMax - (1 << 20)) / row_tiles || batch * kv_heads * plan.head_groups > kMaxRows)
     return fail(SILE_ERR_SHAPE, "%lld rows of up to %lld keys: too many for one call", (long long)batch,
                 (long long)seen);
+  if ((rc = check_written({out}, {in, kp, vp, of, pages})) != SILE_OK) return rc;
   if ((rc = paged_plan(es == 1, batch, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, plan.bytes)) != SILE_OK) return rc;
+  if ((rc = check_written({array_of("workspace", workspace, plan.bytes)}, {out, in, kp, vp, of, pages})) != SILE_OK) return rc;
   PagedArgs a{};
   a.q = q;
   a.k = k_pages;

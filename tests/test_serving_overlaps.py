@@ -114,3 +114,32 @@ def test_chunk_workspace(hip):
         refused("Shape", hip.paged_attn_chunk, **{**CHUNK, **base, "workspace": x(at) + over})
         refused("Shape", hip.paged_attn_chunk, **{**CHUNK, **base, "workspace": x(at) - need + 16})
     arena.close()
+
+
+DECODE = {k: v for k, v in CHUNK.items() if k not in ("n_rows", "n_tokens", "starts")}
+
+
+def test_decode():
+    f = _abi.paged_attn_decode
+    page = 2048 * 2
+    base = {**DECODE, "batch": 4}
+    for change in (dict(o=P), dict(o=P + 3 * 512), dict(o=3 * P + page), dict(o=4 * P + 9 * page), dict(o=5 * P - 512), dict(o=6 * P),
+                   dict(q=P, ldq=512, o=P + 256, ldo=1024)):
+        refused("Shape", f, **{**base, **change})
+    for change in (dict(q=P, ldq=512, o=P + 512, ldo=512), dict(o=P + 4 * 512), dict(o=4 * P - 4 * 512), dict(num_pages=0, o=3 * P)):
+        passes(f, **{**base, **change})
+
+
+@pytest.mark.gpu
+def test_decode_workspace(hip):
+    need = hip.paged_attn_workspace(4, 4, 2, 64)
+    far = (need + (1 << 20)) // 16 * 16
+    arena = hip.DeviceBuffer(10 * far)
+    arena.fill_bytes(0)
+    x = lambda i: arena.ptr + i * far   # noqa: E731
+    base = {**DECODE, "batch": 4, "q": x(1), "k_pages": x(3), "v_pages": x(4), "tables": x(5), "lengths": x(6), "o": x(7),
+            "workspace_bytes": need}
+    for at, over in ((1, 16), (3, 4096), (4, 9 * 4096), (5, 32), (6, 0), (7, 256)):
+        refused("Shape", hip.paged_attn_decode, **{**base, "workspace": x(at) + over})
+        refused("Shape", hip.paged_attn_decode, **{**base, "workspace": x(at) - (need + 15) // 16 * 16 + 16})
+    arena.close()
