@@ -564,7 +564,8 @@ int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n
                                                                     std::min<int64_t>(sinks, kIntMax))
                                   : capacity;
   const int64_t unit = seen / block + 4 + sile::kChunkUnit;
-  if (tiles > (1 << 24) / kv_heads || tiles > (kIntMax - (1 << 20)) / (unit * kv_heads))
+  // (units: of 256 threads each, rounded up to a multiple of 8; a launch has less than 2^32)
+  if (tiles > ((1 << 24) - 8) / kv_heads || tiles > (kIntMax - (1 << 20)) / (unit * kv_heads))
     return fail(SILE_ERR_SHAPE, "%lld tokens of %lld rows of up to %lld keys: too many for one call",
                 (long long)n_tokens, (long long)n_rows, (long long)seen);
   if ((rc = chunk_plan(n_rows, n_tokens, q_heads, kv_heads, head_dim, &plan)) != SILE_OK) return rc;
