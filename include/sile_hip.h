@@ -696,7 +696,7 @@ int sile_hip_rope_append(sile_dtype dtype, sile_dtype cache_type, sile_rope_layo
  * row) as max |y| / 448, the maximum at least 2^-100, and stored in scales [rows][cols / group].
  * sum may be x or residual, and y (of in_type) x or residual, with the same leading
  * dimension; else outputs overlap nothing.  A row with a NaN gives NaN; with an Inf NaN
- * there and 0 elsewhere, as the formula.  Fastest: cols a multiple of 8 up to 16384, rows 16-byte
+ * there and 0 elsewhere, as the formula; finite rows are right at any size of their values.  Fastest: cols a multiple of 8 up to 16384, rows 16-byte
  * aligned, group 0, cols or a power of two from 8 to 512. */
 int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows, int64_t cols,
                           const void *x, int64_t ldx, const void *residual, int64_t ldr, void *sum,

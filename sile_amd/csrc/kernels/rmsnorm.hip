@@ -5,7 +5,9 @@
 //
 // fp32 throughout: s goes into the norm unrounded and is stored rounded once, y is rounded once
 // (to e4m3: to the fp32 quotient and then to the code).  A scale is the given one, or max |y| of
-// each `group` columns over 448 (the maximum counts as at least 2^-100).
+// each `group` columns over 448 (the maximum counts as at least 2^-100).  Where the sum of squares
+// leaves fp32 (a value past 1.8e19; with eps below 2^-100 also where it is below 2^-80, and squares
+// lose digits or vanish), it is taken again of values scaled by a power of two.
 //
 // Every element is read once and written once, so memory bounds it: a row stays in the
 // registers of its threads between the sum and the result.  Rows of up to 512 columns take a
@@ -133,6 +135,16 @@ SILE_DEV float lanes_max(float v, int lanes) {
   return v;
 }
 
+// Whether a sum of squares is outside fp32, and the power of two whose square brings the values back: a
+// finite row's squares, of up to 2^30 columns, then add up to less than 2^126, and a row's least
+// sum is 2^-138; a row with Inf stays Inf.
+SILE_DEV bool out_of_range(float ss, float eps) {
+  return ss == __builtin_inff() || (ss < 0x1p-80f && eps < 0x1p-100f);
+}
+SILE_DEV float back_in_range(float ss) { return ss > 1.0f ? 0x1p-40f : 0x1p40f; }
+// a value that all lanes of a wave have, in a scalar register
+SILE_DEV float scalar(float v) { return bits_f32((uint32_t)__builtin_amdgcn_readfirstlane((int)f32_bits(v))); }
+
 SILE_DEV float scale_of(float top) { return __builtin_fmaxf(top, kLeast) / kTop; }
 SILE_DEV float rcp_of(float scale) { return scale >= 0x1p-60f && scale <= 0x1p60f ? 1.0f / scale : 0.0f; }
 
@@ -141,7 +153,7 @@ SILE_DEV float rcp_of(float scale) { return scale >= 0x1p-60f && scale <= 0x1p60
 // us, 106 without; 8000 x 8191 through the form for any width 277, 136 here.)
 template <int kType, bool kF8, int kThreads, int kV, int kWg, bool kPart>
 SILE_DEV void norm_rows(const NormArgs& a) {
-  __shared__ float lds[2][2][16];
+  __shared__ float lds[3][2][16];
   const int tid = threadIdx.x % kThreads, cols = a.cols;
   float w[kV][8];
   Vec<kType> wv[kV];
@@ -185,8 +197,23 @@ SILE_DEV void norm_rows(const NormArgs& a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(s[v][j], s[v][j], ss);
     }
-    ss = row_reduce<kThreads, false>(ss, lds[0][turn]);
-    const float inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, a.inv_cols, a.eps));
+    ss = scalar(row_reduce<kThreads, false>(ss, lds[0][turn]));
+    float eps = a.eps, back = 1.0f;
+    if (out_of_range(ss, eps)) {   // (all of the row's threads)
+      back = back_in_range(ss);
+      eps = eps * back * back * back * back;
+      ss = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kV; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          s[v][j] *= back;
+          const float t = s[v][j] * back;
+          ss = __builtin_fmaf(t, t, ss);
+        }
+      ss = row_reduce<kThreads, false>(ss, lds[2][turn]);
+    }
+    const float inv = back / __builtin_sqrtf(__builtin_fmaf(ss, a.inv_cols, eps));
     float top = 0.0f;
 #pragma unroll
     for (int v = 0; v < kV; ++v) {
@@ -256,7 +283,7 @@ SILE_DEV void norm_rows(const NormArgs& a) {
 // so it is written by the last pass, each element by the thread that reads it there.
 template <int kType, bool kF8>
 SILE_DEV void norm_any(const NormArgs& a) {
-  __shared__ float lds[2][2][16];
+  __shared__ float lds[3][2][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int turn = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
@@ -269,9 +296,21 @@ SILE_DEV void norm_any(const NormArgs& a) {
       const float s = at(c);
       ss = __builtin_fmaf(s, s, ss);
     }
-    ss = row_reduce<256, false>(ss, lds[0][turn]);
-    const float inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(ss, a.inv_cols, a.eps));
+    ss = scalar(row_reduce<256, false>(ss, lds[0][turn]));
+    float eps = a.eps, back = 1.0f;
+    if (out_of_range(ss, eps)) {
+      back = back_in_range(ss);
+      eps = eps * back * back * back * back;
+      ss = 0.0f;
+      for (int c = tid; c < a.cols; c += 256) {
+        const float t = at(c) * back * back;
+        ss = __builtin_fmaf(t, t, ss);
+      }
+      ss = row_reduce<256, false>(ss, lds[2][turn]);
+    }
+    const float inv = back / __builtin_sqrtf(__builtin_fmaf(ss, a.inv_cols, eps));
     auto norm = [&](float s, int c) {
+      if (back != 1.0f) s *= back;
       s *= inv;
       return a.weight ? s * load1<kType>(a.weight, c) : s;
     };
@@ -308,11 +347,14 @@ SILE_DEV void norm_any(const NormArgs& a) {
 }  // namespace
 
 // t<threads of a row>_v<vectors of a thread>, p: columns that are no whole vectors
+// (Waves a SIMD: without the second bound the parts' form of 16 bits has registers for three, and 8000 x 8191
+// takes 157 us for 136; the form for any width takes 730 for 454, 4000 x 17000 into codes in groups of 1000.
+// Asked for four, the parts' forms into codes and of f32 would spill.)
 #define SILE_NORM(NAME, TYPE, F8, T, V, WG)                                                         \
   extern "C" __global__ __launch_bounds__(WG) void sile_rmsnorm_##NAME##_t##T##_v##V(NormArgs a) {  \
     norm_rows<TYPE, F8, T, V, WG, false>(a);                                                        \
   }                                                                                                 \
-  extern "C" __global__ __launch_bounds__(WG) void sile_rmsnorm_##NAME##_t##T##_v##V##p(NormArgs a) { \
+  extern "C" __global__ __launch_bounds__(WG, TYPE == 0 || F8 ? 1 : 4) void sile_rmsnorm_##NAME##_t##T##_v##V##p(NormArgs a) { \
     norm_rows<TYPE, F8, T, V, WG, true>(a);                                                         \
   }
 #define SILE_NORM_TYPES(NAME, TYPE, F8)                                                        \
@@ -321,7 +363,7 @@ SILE_DEV void norm_any(const NormArgs& a) {
   SILE_NORM(NAME, TYPE, F8, 256, 2, 256)                                                       \
   SILE_NORM(NAME, TYPE, F8, 256, 4, 256)                                                       \
   SILE_NORM(NAME, TYPE, F8, 1024, 2, 1024)                                                     \
-  extern "C" __global__ __launch_bounds__(256) void sile_rmsnorm_##NAME##_any(NormArgs a) {    \
+  extern "C" __global__ __launch_bounds__(256, 8) void sile_rmsnorm_##NAME##_any(NormArgs a) {    \
     norm_any<TYPE, F8>(a);                                                                     \
   }
 SILE_NORM_TYPES(f32, 0, false)
