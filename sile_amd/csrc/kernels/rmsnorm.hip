@@ -253,11 +253,12 @@ SILE_DEV void norm_rows(const NormArgs& a) {
         if (c < cols) {
           float f[8];
           // a group's own scale leaves no quotient past 448 but by a rounding, which the code takes back
+          // (the remainder as q scale - s, whose zero is +0, and taken off: so a -0 stays one)
           if (a.group != 0 && rcp != 0.0f) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float q = s[v][j] * rcp;
-              f[j] = __builtin_fmaf(__builtin_fmaf(-q, scale, s[v][j]), rcp, q);
+              f[j] = __builtin_fmaf(-__builtin_fmaf(q, scale, -s[v][j]), rcp, q);
             }
           } else {
 #pragma unroll

@@ -60,3 +60,18 @@ def test_zeros_without_eps(hip, cols):
     y = c.dy.download(np.float32, (3, cols))
     assert np.isnan(y[0]).all() and (np.abs(y[1] - 1) <= 50 * ref.EPS).all()
     assert np.isnan(y[2, 5]) and (np.delete(y[2], 5) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols,group", [(256, 0), (256, 64), (256, 256), (2048, 128), (255, 255), (18000, 1000), (18000, 18000), (18000, 0)])
+def test_signs_of_zeros(hip, dtype, cols, group):
+    """Codes keep the sign of a zero, and of what rounds to one, whatever the scale is from."""
+    x = rng(cols).normal(size=(4, cols)).astype(np.float32)
+    x[:, ::3] = 0.0
+    x[:, 1::6] = -0.0
+    x[:, 2::9] = 1e-7 * np.where(np.arange(len(range(2, cols, 9))) % 2, 1, -1)
+    c = Norm(hip, 1, dtype, "fp8", 4, cols, residual=False, weight=False, group=group, x=x)
+    c.run()
+    c.check()
+    code = c.dy.download(np.uint8, (4, cols))
+    assert np.array_equal(code >> 7 != 0, np.signbit(c.x))
