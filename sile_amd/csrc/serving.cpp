@@ -55,20 +55,6 @@ constexpr int64_t kLogitChunk = 8192;
 
 bool aligned_to(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
 
-// whether the bytes [x, x + nx) and [y, y + ny) share any
-bool share(const void* x, int64_t nx, const void* y, int64_t ny) {
-  const char *a = static_cast<const char*>(x), *b = static_cast<const char*>(y);
-  return a && b && nx > 0 && ny > 0 && a < b + ny && b < a + nx;
-}
-// bytes from the first to the last element of a matrix
-int64_t extent(int64_t rows, int64_t ld, int64_t cols, int64_t es) { return rows > 0 ? ((rows - 1) * ld + cols) * es : 0; }
-// an output over an input: the same rows in the same places, or apart
-bool in_place_or_apart(const void* in, int64_t ld_in, const void* out, int64_t ld_out, int64_t rows,
-                       int64_t cols, int64_t es) {
-  return (in == out && ld_in == ld_out) ||
-         !share(in, extent(rows, ld_in, cols, es), out, extent(rows, ld_out, cols, es));
-}
-
 // What sile_hip_rope and sile_hip_rope_append have in common: checks, and the kernel's vector
 // width (8, 4 or 1 elements; 8 only of 16 bits).
 int check_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, int64_t q_heads, int64_t kv_heads,
@@ -333,6 +319,7 @@ int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows,
   if (group < 0 || (group > 0 && (!fp8 || cols % group != 0)))
     return fail(SILE_ERR_SHAPE, "groups of %lld columns: of an 8-bit output, a divisor of %lld", (long long)group, (long long)cols);
   if (!(eps >= 0)) return fail(SILE_ERR_SHAPE, "eps is negative");
+  int rc = SILE_OK;
   if (rows == 0 || cols == 0) return ok();
   if (!x || !y || (group > 0 && !scales)) return fail(SILE_ERR_SHAPE, "NULL operand");
   const int64_t es = (int64_t)dtype_bytes(in_type), ys = (int64_t)dtype_bytes(out_type);
@@ -343,17 +330,18 @@ int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows,
     if (!aligned_to(p, es)) return fail(SILE_ERR_SHAPE, "operand not aligned to its type");
   if (!aligned_to(y, ys) || !aligned_to(scales, 4)) return fail(SILE_ERR_SHAPE, "operand not aligned to its type");
   // a row is read before it is written, element by element where the rows coincide
-  const int64_t ny = extent(rows, ldy, cols, ys), ns = extent(rows, lds, cols, es);
-  const int64_t n_scales = group > 0 ? 4 * rows * (cols / group) : 0;
-  const bool y_own = ys == es && ldx == ldy && y == x, y_own_r = ys == es && ldr == ldy && y == residual;
-  if ((!y_own && share(x, extent(rows, ldx, cols, es), y, ny)) ||
-      (!y_own_r && residual && share(residual, extent(rows, ldr, cols, es), y, ny)) ||
-      (sum && (!in_place_or_apart(x, ldx, sum, lds, rows, cols, es) ||
-               (residual && !in_place_or_apart(residual, ldr, sum, lds, rows, cols, es)) || share(sum, ns, y, ny) ||
-               share(weight, cols * es, sum, ns) || share(scales, n_scales, sum, ns))) ||
-      share(weight, cols * es, y, ny) || share(scales, n_scales, y, ny) ||
-      share(scales, n_scales, x, extent(rows, ldx, cols, es)) || share(scales, n_scales, weight, cols * es) ||
-      (residual && share(scales, n_scales, residual, extent(rows, ldr, cols, es))))
+  const Region in{"x", x, rows, ldx * es, cols * es}, add{"residual", residual, rows, ldr * es, cols * es};
+  const Region to_sum{"sum", sum, rows, lds * es, cols * es}, out{"y", y, rows, ldy * ys, cols * ys};
+  const Region by = array_of("weight", weight, cols * es);
+  const Region to_scales = array_of("scales", group > 0 ? scales : nullptr, group > 0 ? 4 * rows * (cols / group) : 0);
+  auto own = [&](const void* to, int64_t ld, int64_t bytes, const void* from, int64_t ld_from) {
+    return bytes == es && to == from && ld == ld_from;
+  };
+  if ((rc = check_written({to_sum, out, to_scales}, {by})) != SILE_OK || (rc = check_written({to_scales}, {in, add})) != SILE_OK)
+    return rc;
+  if ((!own(y, ldy, ys, x, ldx) && regions_share(out, in)) || (!own(y, ldy, ys, residual, ldr) && regions_share(out, add)) ||
+      (!own(sum, lds, es, x, ldx) && regions_share(to_sum, in)) ||
+      (!own(sum, lds, es, residual, ldr) && regions_share(to_sum, add)))
     return fail(SILE_ERR_SHAPE, "an output overlaps another operand without being its rows");
   NormArgs a{x, residual, weight, sum, y, scales, rows, ldx, ldr, lds, ldy, (int32_t)cols, (int32_t)group,
              eps, 1.0f / (float)cols, scale, reciprocal(scale)};
@@ -361,8 +349,7 @@ int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows,
   const bool vectors =
       cols <= 16384 && (group == 0 || group == cols || (group <= 512 && group >= 8 && (group & (group - 1)) == 0));
   int cus = 0;
-  int rc = device_cus(&cus);
-  if (rc != SILE_OK) return rc;
+  if ((rc = device_cus(&cus)) != SILE_OK) return rc;
   int threads = 256, per = 0, wg = 256;
   char name[64], form[16];
   if (vectors) {
@@ -427,20 +414,15 @@ int sile_hip_logprobs_rows(sile_dtype in_type, int64_t rows, int64_t cols, const
   if (!aligned_to(x, es) || !aligned_to(targets, 4) || !aligned_to(logp, 4) || !aligned_to(entropy, 4) ||
       !aligned_to(top_logp, 4) || !aligned_to(top_ids, 4))
     return fail(SILE_ERR_SHAPE, "operand not aligned to its type");
-  struct { const void* p; int64_t n; bool written; } all[] = {
-      {x, extent(rows, ldx, cols, es), false}, {logp ? targets : nullptr, 4 * rows, false}, {logp, 4 * rows, true},
-      {entropy, 4 * rows, true}, {top_k ? top_logp : nullptr, 4 * rows * top_k, true},
-      {top_k ? top_ids : nullptr, 4 * rows * top_k, true}};
-  for (auto& p : all)
-    for (auto& q : all)
-      if (&p != &q && p.written && share(p.p, p.n, q.p, q.n))
-        return fail(SILE_ERR_SHAPE, "an output overlaps another operand");
+  const Region in{"x", x, rows, ldx * es, cols * es}, of = array_of("targets", logp ? targets : nullptr, 4 * rows);
+  const Region one = array_of("logp", logp, 4 * rows), two = array_of("entropy", entropy, 4 * rows);
+  const Region top = array_of("top_logp", top_logp, 4 * rows * top_k), ids = array_of("top_ids", top_ids, 4 * rows * top_k);
+  if ((rc = check_written({one, two, top, ids}, {in, of})) != SILE_OK) return rc;
   int64_t chunks, per, parts;
   if ((rc = logprob_parts(rows, cols, &chunks, &per, &parts)) != SILE_OK) return rc;
   const int64_t need = parts > 1 ? rows * parts * (16 + 8 * top_k) : 0;
   if (need > 0 && (rc = check_workspace(workspace, workspace_bytes, need)) != SILE_OK) return rc;
-  for (auto& p : all)
-    if (need > 0 && share(p.p, p.n, workspace, need)) return fail(SILE_ERR_SHAPE, "the workspace overlaps an operand");
+  if ((rc = check_written({array_of("workspace", workspace, need)}, {in, of, one, two, top, ids})) != SILE_OK) return rc;
   LogprobArgs a{};
   a.x = x;
   a.targets = targets;

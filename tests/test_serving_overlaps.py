@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 from sile_amd import _abi
-from tests.test_serving_abi import APPEND, CHUNK, P, ROPE, refused
+from tests.test_serving_abi import APPEND, CHUNK, LOGPROBS, NORM, P, ROPE, refused
 
 
 def passes(f, **kw):
@@ -143,3 +143,40 @@ def test_decode_workspace(hip):
         refused("Shape", hip.paged_attn_decode, **{**base, "workspace": x(at) + over})
         refused("Shape", hip.paged_attn_decode, **{**base, "workspace": x(at) - (need + 15) // 16 * 16 + 16})
     arena.close()
+
+
+def test_norm_between_rows():
+    """Rows of 64 elements of 2 bytes, in slices of wider ones."""
+    f = _abi.rmsnorm_rows
+    wide = dict(x=P, ldx=256, residual=P + 128, ldr=256)
+    for change in ({**wide, "sum_out": P + 256, "lds": 256, "y": P + 384, "ldy": 256}, {**wide, "sum_out": P + 128, "lds": 256, "y": P, "ldy": 256},
+                   {**wide, "y": P, "ldy": 256}, {**wide, "out_type": _abi.F8E4M3, "y": P + 256, "ldy": 512},
+                   {**wide, "out_type": _abi.F8E4M3, "y": P + 448, "ldy": 1024, "group": 16, "scales": 6 * P}):
+        passes(f, **{**NORM, **change})
+    for change in ({**wide, "y": P + 64, "ldy": 256}, {**wide, "sum_out": P + 256, "lds": 256, "y": P + 320, "ldy": 256},
+                   {**wide, "out_type": _abi.F8E4M3, "y": P, "ldy": 512}, {**wide, "out_type": _abi.F8E4M3, "y": P + 450, "ldy": 300},
+                   {**wide, "sum_out": P, "lds": 128}, {**wide, "weight": P, "y": P, "ldy": 256}):
+        refused("Shape", f, **{**NORM, **change})
+
+
+def test_logprobs_between_rows():
+    """Outputs behind the columns of padded rows."""
+    f = _abi.logprobs_rows
+    for change in (dict(ldx=164, logp=P + 400, entropy=P + 416, top_logp=P + 432), dict(top_k=0, top_logp=P, top_ids=P), dict(logp=None, targets=3 * P, entropy=4 * P)):
+        passes(f, **{**LOGPROBS, **change})
+    for change in (dict(ldx=164, logp=P + 644), dict(ldx=164, top_ids=P + 656 + 400 - 76)):
+        refused("Shape", f, **{**LOGPROBS, **change})
+
+
+@pytest.mark.gpu
+def test_norm_of_slices(hip):
+    """Sum and result of a slice of wide rows to other slices of them, as to arrays of their own."""
+    import numpy as np
+    x = np.random.default_rng(0).normal(size=(50, 4, 256)).astype(np.float32)
+    wide, apart = hip.DeviceBuffer.from_array(x), hip.DeviceBuffer(50 * 512 * 4)
+    args = (hip.F32, hip.F32, 50, 256, wide.ptr, 1024, wide.ptr + 1024, 1024)
+    hip.rmsnorm_rows(*args, apart.ptr, 512, 0, 1e-5, apart.ptr + 1024, 512)
+    hip.rmsnorm_rows(*args, wide.ptr + 2048, 1024, 0, 1e-5, wide.ptr + 3072, 1024)
+    hip.synchronize()
+    got, want = wide.download(np.float32, (50, 4, 256)), apart.download(np.float32, (50, 2, 256))
+    assert np.array_equal(got[:, 2:], want) and np.array_equal(got[:, :2], x[:, :2])
