@@ -153,6 +153,7 @@ SILE_DEV void chunk_row(const ChunkArgs& a, int32_t seq, int kvh, int32_t p, con
   // lanes 0 .. 31 and 32 .. 63 a key each, 8 dims a lane
   const int half = lane >> 5, dim = 8 * (lane & 31);
   float acc[8], m = kLowest, l = 0.0f;
+  bool any = false;   // a key is there: its page may not be
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
   const int64_t n = (int64_t)span.sink_end + span.len - span.first;
@@ -161,6 +162,9 @@ SILE_DEV void chunk_row(const ChunkArgs& a, int32_t seq, int kvh, int32_t p, con
     const int key = (int)(i < span.sink_end ? i : i - span.sink_end + span.first);
     const int32_t id = table[key >> a.page_shift];
     const bool ok = i0 + lane < n && (uint32_t)id < (uint32_t)a.num_pages;
+    const uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
+    if (seen == 0) continue;
+    any = true;
     // (a key that is not seen: page 0's row of its slot, which is there)
     const int64_t off = ((int64_t)(ok ? id : 0) * a.page_stride +
                          (((int64_t)kvh << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * d) * kEs;
@@ -185,7 +189,6 @@ SILE_DEV void chunk_row(const ChunkArgs& a, int32_t seq, int kvh, int32_t p, con
     l = l * alpha + wave_sum(pr);
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] *= alpha;
-    const uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
     for (int k0 = 0; k0 < 64; k0 += 2) {
       const int from = k0 + half;
       const float pu = __shfl(pr, from);
@@ -204,23 +207,21 @@ SILE_DEV void chunk_row(const ChunkArgs& a, int32_t seq, int kvh, int32_t p, con
     if (half == 0) lds->acc[wave][dim + j] = acc[j] + other;
   }
   if (lane == 0) {
-    lds->ml[wave][0] = m;
+    lds->ml[wave][0] = any ? m : -__builtin_inff();
     lds->ml[wave][1] = l;
   }
   __syncthreads();
   if ((int)threadIdx.x < d) {
     float top = kLowest, sum = 0.0f, r = 0.0f;
-    for (int w = 0; w < 4; ++w) top = __builtin_fmaxf(top, lds->ml[w][0]);
-    bool any = false;
+    any = false;
+    for (int w = 0; w < 4; ++w) {
+      top = __builtin_fmaxf(top, lds->ml[w][0]);
+      any |= lds->ml[w][0] > -__builtin_inff();
+    }
     for (int w = 0; w < 4; ++w) {
       const float f = exp2_fast(lds->ml[w][0] - top);
       sum += f * lds->ml[w][1];
       r += f * lds->acc[w][threadIdx.x];
-    }
-    // (whether a key is there: its page may not be)
-    for (int64_t i = 0; i < n && !any; ++i) {
-      const int key = (int)(i < span.sink_end ? i : i - span.sink_end + span.first);
-      any = (uint32_t)table[key >> a.page_shift] < (uint32_t)a.num_pages;
     }
     r = any ? r * (a.v_scale / sum) : 0.0f;
     if ((int)threadIdx.x >= dim0 && (int)threadIdx.x < dim1) o[threadIdx.x] = kBF16 ? bf16_rne(r) : f16_rne(r);
