@@ -75,3 +75,22 @@ def test_signs_of_zeros(hip, dtype, cols, group):
     c.check()
     code = c.dy.download(np.uint8, (4, cols))
     assert np.array_equal(code >> 7 != 0, np.signbit(c.x))
+
+
+@pytest.mark.parametrize("dtype,out,rows,cols,group", [
+    # a wave a row (8192 rows are one launch's, on 256 CUs), a workgroup of 256 (2048) and of 1024 (512), any width
+    ("bf16", "bf16", 17001, 40, 0), ("f32", "f32", 9000, 100, 0), ("f16", "fp8", 9001, 256, 64), ("bf16", "fp8", 20000, 33, 33),
+    ("bf16", "bf16", 4500, 1000, 0), ("bf16", "fp8", 6200, 600, 600), ("f32", "fp8", 4200, 1024, 128), ("f16", "f16", 2100, 4097, 0),
+    ("bf16", "fp8", 4100, 8192, 8192), ("f32", "fp8", 2050, 3001, 3001),
+    ("bf16", "bf16", 1100, 8200, 0), ("f16", "fp8", 1600, 8200, 8200), ("f32", "fp8", 520, 16384, 256),
+    ("f32", "f32", 2060, 16386, 0), ("bf16", "fp8", 4500, 999, 333), ("f16", "fp8", 2100, 16400, 16400)])
+def test_many_rows(hip, dtype, out, rows, cols, group):
+    """Workgroups that go on to further rows, some of which are summed again."""
+    say(f"norm {dtype} -> {out} {rows} x {cols}, groups of {group}")
+    r = rng(rows + cols)
+    x = r.normal(size=(rows, cols)).astype(np.float32) * r.choice([0.01, 1.0, 50.0], rows).astype(np.float32)[:, None]
+    if dtype != "f16":
+        x[r.random(rows) < 0.2, 0] = 1e25
+    c = Norm(hip, rows, dtype, out, rows, cols, weight=cols < 5000, group=group, x=x)
+    c.run()
+    c.check()
