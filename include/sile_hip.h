@@ -625,7 +625,10 @@ int sile_hip_paged_attn_chunk_workspace(int64_t n_rows, int64_t n_tokens, int64_
  * q's), the workspace nothing at all: refused otherwise.  The
  * probabilities enter the second product in 16 bits (one part, where sile_hip_paged_attn_decode has
  * two), as in sile_hip_flash_attn_window_fwd; a token whose result is not finite, or that meets
- * Inf or NaN in V of a masked key of its blocks, is taken again in fp32: right, but slow. */
+ * Inf or NaN in V of a masked key of its blocks, is taken again in fp32: right, but slow.  One call
+ * takes fewer than 2^30 tokens x query heads a key head, fewer than 2^24 units (128 of those, and one
+ * more a sequence, times the key heads) and, of the table's width or the window, some 2^36 keys over
+ * all units. */
 int sile_hip_paged_attn_chunk(sile_dtype dtype, sile_dtype cache_type, int64_t n_rows,
                               int64_t n_tokens, int64_t q_heads, int64_t kv_heads,
                               int64_t head_dim, const void *q, int64_t ldq, const int32_t *starts,
@@ -662,9 +665,9 @@ int sile_hip_rope_turns(sile_rope_scaling scaling, int64_t rot_dim, double base,
  * x = 2 pi turns[j] positions[t] (turns: device, 64 bits, kept there to its fraction of a turn),
  *   (a, b) -> magnitude * (a cos x - b sin x, b cos x + a sin x),
  * and dims from rot_dim on are copied; fp32, rounded once.  Negative turns turn back.  dtype f32, f16
- * or bf16; tokens at q + t * ldq, k + t * ldk, [heads][head_dim] (leading dimensions up to 2^25), any
- * alignment and head_dim up to 2048 (16-byte aligned and rot_dim a multiple of 16 is fastest); q_heads or kv_heads may be
- * 0.  An output is its input (same pointer and leading dimension) or apart from it, and apart from
+ * or bf16; tokens at q + t * ldq, k + t * ldk, [heads][head_dim] (at most 2^15 heads of either, 2^24
+ * dims a token and leading dimensions of 2^25), any alignment and head_dim up to 2048 (16-byte aligned
+ * and rot_dim a multiple of 16 is fastest); q_heads or kv_heads may be 0.  An output is its input (same pointer and leading dimension) or apart from it, and apart from
  * everything else of the call (rows may lie between another's, as in a fused projection):
  * refused otherwise.  A token at a position below 0 is left out: its outputs stay as they are. */
 int sile_hip_rope(sile_dtype dtype, sile_rope_layout layout, int64_t n_tokens, int64_t q_heads,
@@ -696,8 +699,9 @@ int sile_hip_rope_append(sile_dtype dtype, sile_dtype cache_type, sile_rope_layo
  * row) as max |y| / 448, the maximum at least 2^-100, and stored in scales [rows][cols / group].
  * sum may be x or residual, and y (of in_type) x or residual, with the same leading
  * dimension; else outputs overlap nothing.  A row with a NaN gives NaN; with an Inf NaN
- * there and 0 elsewhere, as the formula; finite rows are right at any size of their values.  Fastest: cols a multiple of 8 up to 16384, rows 16-byte
- * aligned, group 0, cols or a power of two from 8 to 512. */
+ * there and 0 elsewhere, as the formula; finite rows are right at any size of their values.
+ * Fastest: cols a multiple of 8 up to 16384, rows 16-byte aligned, group 0, cols or a power of two
+ * from 8 to 512. */
 int sile_hip_rmsnorm_rows(sile_dtype in_type, sile_dtype out_type, int64_t rows, int64_t cols,
                           const void *x, int64_t ldx, const void *residual, int64_t ldr, void *sum,
                           int64_t lds, const void *weight, float eps, void *y, int64_t ldy,

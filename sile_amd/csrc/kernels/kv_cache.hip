@@ -105,7 +105,8 @@ constexpr int kSlotTokens = 1024;   // of the list, a workgroup
 // 8.7 (14.5 with a quarter of the threads, and four times the rows in each).
 SILE_DEV void slots(const SlotsArgs& a) {
   __shared__ int64_t wave_sum[kSlotTokens / 64];
-  __shared__ int32_t mark_row[kSlotTokens], mark_base[kSlotTokens];   // by token: row + 1 that begins there, length - start
+  // by token: row + 1 that begins there, length - start
+  __shared__ int32_t mark_row[kSlotTokens], mark_base[kSlotTokens];
   __shared__ int32_t wave_top[kSlotTokens / 64], first_row, first_base;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (a.n_rows + kSlotTokens - 1) / kSlotTokens;

@@ -30,9 +30,9 @@
 //
 // The loads are non-temporal (below 54 -> 52, without top ones 45 -> 41 and 27 -> 25).
 //
-// Measured: 64 rows of 131072 in bf16, 20 top ones, 20 us (14 and the join 6; without top ones 9), one
-// row 14; 2000 rows of 32001 in f32, 5 top ones, 55 (4.6 TB/s; without 42), of 32000 in bf16, 20 top ones,
-// 50 (without 27).  What holds them is the latency of the list's steps, then instructions: a quarter
+// Measured: 64 rows of 131072 in bf16, 20 top ones, 20 us (14 and the join 7; without top ones 9.5), one
+// row 15; 2000 rows of 32001 in f32, 5 top ones, 53 - 55 (4.8 TB/s; without 42), of 32000 in bf16, 20 top
+// ones, 50 (without 27).  What holds them is the latency of the list's steps, then instructions: a quarter
 // of the time without top ones is exp2's.
 #include <type_traits>
 

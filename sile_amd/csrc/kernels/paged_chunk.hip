@@ -34,9 +34,11 @@
 // their sum is of the rounded ones); f16 ones carry a factor 2^7 beside the up to 2^8 that the lazy
 // maximum allows, so that those far below the maximum keep their bits.
 //
-// Measured, 32 query heads of 128 over 8 key heads: 2048 tokens behind 30000 keys 1.19 ms (875 TFLOP/s, the
-// matrix cores and their power), 8192 from none 0.71 ms; 32 pieces of 8 tokens over up to 8192 keys 115 us
-// (4.8 TB/s), as e4m3 codes 86 us; 1 piece of 4 over 300 13 us.
+// Measured, 32 query heads of 128 over 8 key heads: 2048 tokens behind 30000 keys 1.13 to 1.2 ms by card (870 to 920
+// TFLOP/s: the matrix cores are busy for 41 % of the cycles, a third of the waves' cycles waits to issue and a
+// quarter for data, and their power leaves 2.0 GHz of 2.4), 8192 from none 0.71 ms; 32 pieces of 8 tokens over up
+// to 8192 keys 115 us (4.8 TB/s), as e4m3 codes 86 us; 1 piece of 4 over 300 13 us.  The kernels spill 70 to 290
+// scalar registers into vector ones, the e4m3 forms at 256 dims also 21 vector registers to memory.
 #include <type_traits>
 
 #include "common.h"
@@ -238,7 +240,8 @@ SILE_DEV void chunk_again(const ChunkArgs& a, ChunkLds* lds) {
   const int lane = threadIdx.x & 63, G = a.shape.group;
   while (next_unit(a, at, u)) {
     if (u.b0 != 0 || u.b1 < u.tile.blocks) continue;   // in parts: the join's
-    for (int r = 0; r < u.tile.rows; ++r) {   // (every wave sees the same: a row is stored anew behind a barrier)
+    // (every wave sees the same: a row is stored anew behind a barrier)
+    for (int r = 0; r < u.tile.rows; ++r) {
       const int64_t packed = (int64_t)(at.tile - u.first) * kChunkRows + r;
       const int32_t token = (int32_t)(packed / G), head = at.kvh * G + (int32_t)(packed - (int64_t)token * G);
       const int64_t t = u.seq.start + token;
@@ -698,9 +701,11 @@ __device__ __forceinline__ bool chunk_units(const ChunkArgs& a, const uint16_t* 
       // the four waves' results: in their own tiles' place, then a wave a quarter of the dims
       static_assert(kDT * 4096 <= kStageB, "O in the place of K and V");
       asm volatile("" ::: "memory");
-      __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));   // vmcnt(0) lgkmcnt(0): nothing more is written there
+      // vmcnt(0) lgkmcnt(0): nothing more is written there
+      __builtin_amdgcn_s_waitcnt(0 | (7 << 4) | (0 << 8));
       asm volatile("" ::: "memory");
-      int el = lane;   // (through an empty asm: addresses worked out here are not kept in registers through the blocks)
+      // (through an empty asm: addresses worked out here are not kept in registers through the blocks)
+      int el = lane;
       asm volatile("" : "+v"(el));
 #pragma unroll
       for (int t = 0; t < 4 * kDT; ++t) {

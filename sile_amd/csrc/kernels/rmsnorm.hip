@@ -15,8 +15,9 @@
 // further rows.
 //
 // Measured, bf16 with residual and stored sum: 8000 rows of 8192 100 us (5.2 TB/s), into e4m3 codes in groups
-// 106 (4.3 TB/s: the codes' conversion is 35 % of the vector units' cycles), 64 rows of 8192 5; rows of
-// 8191, which are no whole vectors, 136.
+// 107 (4.3 TB/s: the codes' conversion is 36 % of the vector units' cycles), 64 rows of 8192 5; rows of
+// 8191, which are no whole vectors, 136.  The form for any width reads an element a load, the row twice or,
+// for a scale of its own, three times: 4000 rows of 16392 280 us, of 17000 into codes in groups of 1000 455.
 #include "common.h"
 #include "e4m3.h"
 
@@ -149,8 +150,8 @@ SILE_DEV float scale_of(float top) { return __builtin_fmaxf(top, kLeast) / kTop;
 SILE_DEV float rcp_of(float scale) { return scale >= 0x1p-60f && scale <= 0x1p60f ? 1.0f / scale : 0.0f; }
 
 // Columns in vectors of 8, the last one (kPart) perhaps in part: a row takes kThreads threads of kV vectors.
-// kF8: codes out.  kWg: threads of the workgroup.  (With the parts' code in the way, 8000 x 8192 into codes took 125
-// us, 106 without; 8000 x 8191 through the form for any width 277, 136 here.)
+// kF8: codes out.  kWg: threads of the workgroup.  (With the parts' code in the way, 8000 x 8192 into codes
+// took 125 us, 106 without; 8000 x 8191 through the form for any width 277, 136 here.)
 template <int kType, bool kF8, int kThreads, int kV, int kWg, bool kPart>
 SILE_DEV void norm_rows(const NormArgs& a) {
   __shared__ float lds[3][2][16];
@@ -364,7 +365,7 @@ SILE_DEV void norm_any(const NormArgs& a) {
   SILE_NORM(NAME, TYPE, F8, 256, 2, 256)                                                       \
   SILE_NORM(NAME, TYPE, F8, 256, 4, 256)                                                       \
   SILE_NORM(NAME, TYPE, F8, 1024, 2, 1024)                                                     \
-  extern "C" __global__ __launch_bounds__(256, 8) void sile_rmsnorm_##NAME##_any(NormArgs a) {    \
+  extern "C" __global__ __launch_bounds__(256, 8) void sile_rmsnorm_##NAME##_any(NormArgs a) { \
     norm_any<TYPE, F8>(a);                                                                     \
   }
 SILE_NORM_TYPES(f32, 0, false)

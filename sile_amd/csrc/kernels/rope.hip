@@ -18,7 +18,9 @@
 //
 // Measured: 16382 tokens of 32 + 2 x 8 heads of 128, bf16, with append 90 us (4.5 TB/s), into e4m3 pages
 // 97 (3.8 TB/s: the vector units are busy for 61 % of it); 5000 tokens of f16, 32 of 128 dims rotated, 38.5
-// (4.3 TB/s); 64 tokens 5.  The loads are non-temporal: 96, 100 and 41 us without.
+// (4.3 TB/s); 64 tokens 5.  The loads are non-temporal: 96, 100 and 41 us without.  Rows that lie on no whole
+// vectors go an element a load: 5000 tokens of 32 + 8 heads of 128, bf16, 24 us, from an odd element on, or of
+// 126 dims, 71.
 #include "common.h"
 #include "e4m3.h"
 

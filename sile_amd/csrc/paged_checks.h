@@ -146,8 +146,8 @@ inline int check_heads(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t
 
 // int32 workspaces, each part on a 16-byte boundary
 inline int64_t ints16(int64_t n) { return (n + 3) / 4 * 4; }
-       
-       inline int check_workspace(const void* ws, size_t have, int64_t need) {
+
+inline int check_workspace(const void* ws, size_t have, int64_t need) {
   if (!ws || !aligned16(ws)) return fail(SILE_ERR_SHAPE, "workspace NULL or not 16-byte aligned");
   if ((int64_t)have < need)
     return fail(SILE_ERR_SHAPE, "workspace of %zu bytes, %lld needed", have, (long long)need);
