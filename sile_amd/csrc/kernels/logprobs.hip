@@ -15,8 +15,8 @@
 // one of 1e-3 good to 1e-4).  A wave whose l is below 1.25 works its u out anew: the other lanes' l, and the
 // columns of one lane that has the maximum again, a 64th of the wave's, without it; above, l - 1 has
 // lost two or three bits at most.  (Of the rows of 32000 below a quarter has such a wave: without top
-// ones 25.5 -> 27.5 us in bf16 and 41.2 -> 42 in f32.  In every wave it took 29.5 and 46, a sum of its own
-// of what is below the maximum, in every lane, 30 and 44.)
+// ones 25.5 -> 27.5 us in bf16 and 41.2 -> 42 in f32; where every row has one 28 and 44.  In every wave
+// it took 29.5 and 46, a sum of its own of what is below the maximum, in every lane, 30 and 44.)
 //
 // What the top ones cost beside that: every wave keeps the k best of its columns in order, an
 // entry a lane, and a chunk's largest value of a lane is compared with the k-th; where one passes
