@@ -176,7 +176,7 @@ def test_norm_of_slices(hip):
     wide, apart = hip.DeviceBuffer.from_array(x), hip.DeviceBuffer(50 * 512 * 4)
     args = (hip.F32, hip.F32, 50, 256, wide.ptr, 1024, wide.ptr + 1024, 1024)
     hip.rmsnorm_rows(*args, apart.ptr, 512, 0, 1e-5, apart.ptr + 1024, 512)
-    hip.rmsnorm_rows(*args, wide.ptr + 2048, 1024, 0, 1e-5, wide.ptr + 3072, 1024)
+    hip.rmsnorm_rows(*args, wide.ptr + 2 * 1024, 1024, 0, 1e-5, wide.ptr + 3 * 1024, 1024)
     hip.synchronize()
     got, want = wide.download(np.float32, (50, 4, 256)), apart.download(np.float32, (50, 2, 256))
     assert np.array_equal(got[:, 2:], want) and np.array_equal(got[:, :2], x[:, :2])
